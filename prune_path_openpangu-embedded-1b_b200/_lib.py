@@ -21,6 +21,9 @@ _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
 _c_size_t = ctypes.c_size_t
 _c_float = ctypes.c_float
+_c_int64 = ctypes.c_int64
+
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 
 # name -> (restype, argtypes); mirrors include/ppmoe.h
 SIGNATURES = {
@@ -65,6 +68,20 @@ SIGNATURES = {
     "ppmoe_decode_host": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_float,
                                    _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size_t,
                                    _c_void_p]),
+    "ppmoe_rotary": (_c_int, [_c_void_p, _c_int64, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_int64,
+                              _c_int, _c_void_p, _c_int64, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64,
+                              _c_int64, _c_int, _c_int, _c_int64, _c_int, _c_int, _c_int, _c_void_p, _c_float,
+                              _c_int, _c_void_p, _c_int, _c_int64, _c_int64, _c_int, _c_void_p]),
+    "ppmoe_kv_append": (_c_int, [_c_void_p, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_int, _c_void_p,
+                                 _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_int, _c_void_p, _c_int64,
+                                 _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_int64, _c_int, _c_int,
+                                 _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int, _c_int, _c_int,
+                                 _c_int, _c_void_p, _c_float, _c_int, _c_void_p, _c_void_p]),
+    "ppmoe_attend_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int64]),
+    "ppmoe_attend": (_c_int, [_c_void_p, _c_int64, _c_int64, _c_int, _c_int, _c_void_p, _c_int64, _c_int64, _c_int64,
+                              _c_void_p, _c_int64, _c_int64, _c_int64, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+                              _c_void_p, _c_void_p, _c_int64, _c_int, _c_int, _c_float, _c_int, _c_int64, _c_void_p,
+                              _c_int64, _c_int64, _c_int, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
 }
 
 _lib = None

@@ -131,6 +131,10 @@ int ppmoe_workspace_status(void* ws, void* stream) {
     set_error("device: a bounded wait timed out (status 0x%x)", word);
     return PPMOE_ERR_TIMEOUT;
   }
+  if (!(word & DEVERR_OVERFLOW) && (word & DEVERR_PAGE)) {
+    set_error("device: a position without a page of the cache (status 0x%x)", word);
+    return PPMOE_ERR_INVALID_ARG;
+  }
   set_error("device: capacity exceeded (status 0x%x)", word);
   return PPMOE_ERR_WORKSPACE;
 }

@@ -29,6 +29,7 @@ int cuda_fail(cudaError_t e, const char* what);
 enum : uint32_t {
   DEVERR_TIMEOUT = 1u,      // a bounded mbarrier wait ran out
   DEVERR_OVERFLOW = 2u,     // a capacity bound was exceeded (work skipped)
+  DEVERR_PAGE = 4u,         // a sequence needs a page that its table or the cache does not have
 };
 
 // Size-bounded spin: ~2^22 polls with a short sleep ≈ well under a second.

@@ -1,0 +1,353 @@
+// Rotary position embedding of queries and keys (forward and gradient), and the append of new
+// keys and values to a paged cache with the rotation applied on the way.
+//
+// Pair i of a head at position p turns by 2 pi p turns[i]:
+//   y1 = g (x1 cos - x2 sin),  y2 = g (x2 cos + x1 sin)     (gradient: the same with -angle)
+// The angle is reduced in fp64 (p turns[i] minus the nearest integer), so far positions lose
+// nothing, and its sine and cosine are taken in fp32; values are rounded once, at the store.
+#include <cuda_fp16.h>
+#include "seqs.cuh"
+
+namespace ppmoe {
+
+constexpr int kMaxPairs = 128;  // head_dim <= 256
+constexpr int kRotThreads = 256;
+constexpr int kRotTokens = 8;   // most tokens of one CTA
+
+// One tensor of heads: rows of head_dim contiguous values; strides in elements.
+struct HeadsView {
+  const void* in;
+  void* out;
+  int64_t in_b, in_t, in_h, out_b, out_t, out_h;
+  int heads;
+};
+
+struct RotaryArgs {
+  HeadsView q, k, v;  // v: append only (copied)
+  double turns[kMaxPairs];
+  const void* positions;  // rotary only
+  int64_t pos_b, pos_t;
+  int pos64;
+  int batch;
+  int64_t length, tokens;  // tokens = batch * length
+  int head_dim, pairs;     // rotated values: 2 * pairs of head_dim
+  float gain, sign;
+  int per_cta;
+  Seqs seqs;    // append only
+  Pages pages;  // append only
+  uint32_t* status;
+};
+
+template <typename T, int V>
+struct Chunk {
+  T x[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Chunk<T, V> load_chunk(const T* p) {
+  Chunk<T, V> c;
+  if constexpr (V == 1) {
+    c.x[0] = *p;
+  } else {
+    static_assert(sizeof(T) * V == 16, "16-byte chunks");
+    *reinterpret_cast<uint4*>(c.x) = *reinterpret_cast<const uint4*>(p);
+  }
+  return c;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_chunk(T* p, const Chunk<T, V>& c) {
+  if constexpr (V == 1)
+    *p = c.x[0];
+  else
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(c.x);
+}
+
+// A unit is V pairs (two 16-byte chunks of a head, or 2 values where alignment allows no
+// more): units [0, pairs / V) of a head are rotated, the rest copied.
+template <typename T, int V, bool INTERLEAVED, bool APPEND>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  __shared__ __align__(16) float s_cos[kRotTokens * kMaxPairs], s_sin[kRotTokens * kMaxPairs];
+  __shared__ long long s_pos[kRotTokens];
+  __shared__ int64_t s_k[kRotTokens], s_v[kRotTokens];  // append: cache offsets, -1: not stored
+  __shared__ int s_live[kRotTokens];
+  const int tid = threadIdx.x;
+  const int64_t t0 = (int64_t)blockIdx.x * a.per_cta;
+  const int nt = (int)(a.tokens - t0 < a.per_cta ? a.tokens - t0 : a.per_cta);
+
+  // positions (and, for an append, the place in the cache) of this CTA's tokens
+  if constexpr (APPEND) {
+    const int w = tid >> 5;
+    static_assert(kRotThreads / 32 >= kRotTokens, "a warp a token");
+    if (w < nt) {
+      const int t = (int)(t0 + w);
+      const int b = find_seq_warp(a.seqs.starts, a.seqs.batch, t);
+      if ((tid & 31) == 0) {
+        const bool live = b >= 0 && b < a.seqs.batch;
+        long long pos = 0;
+        int64_t ko = -1, vo = -1;
+        if (live) {
+          pos = (long long)a.seqs.lengths[b] - a.seqs.starts[b + 1] + t;
+          const long long pi = pos >> a.pages.page_shift;
+          int page = -1;
+          if (pos >= 0 && pi < a.seqs.max_pages) page = a.seqs.table[b * a.seqs.table_stride + pi];
+          if (page >= 0 && page < a.pages.num_pages) {
+            const int64_t row = pos & ((1ll << a.pages.page_shift) - 1);
+            ko = page * a.pages.k_page + row * a.pages.k_row;
+            vo = page * a.pages.v_page + row * a.pages.v_row;
+          } else {
+            atomicOr(a.status, DEVERR_PAGE);
+          }
+        }
+        s_live[w] = live;
+        s_pos[w] = pos;
+        s_k[w] = ko;
+        s_v[w] = vo;
+      }
+    }
+  } else {
+    if (tid < nt) {
+      const int64_t t = t0 + tid;
+      const int64_t i = (t / a.length) * a.pos_b + (t % a.length) * a.pos_t;
+      s_pos[tid] = a.pos64 ? static_cast<const long long*>(a.positions)[i]
+                           : (long long)static_cast<const int32_t*>(a.positions)[i];
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < nt * a.pairs; i += kRotThreads) {
+    const int t = i / a.pairs, p = i - t * a.pairs;
+    const double turn = (double)s_pos[t] * a.turns[p];
+    float s, c;
+    sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
+    s_cos[t * a.pairs + p] = c * a.gain;
+    s_sin[t * a.pairs + p] = s * (a.gain * a.sign);
+  }
+  __syncthreads();
+
+  const int units = a.head_dim / (2 * V), turned = a.pairs / V;
+  const int heads = a.q.heads + a.k.heads + (APPEND ? a.v.heads : 0);
+  const int per_token = heads * units;
+  for (int i = tid; i < nt * per_token; i += kRotThreads) {
+    const int t = i / per_token;
+    const int r = i - t * per_token;
+    int h = r / units;
+    const int u = r - h * units;
+    const int64_t tok = t0 + t;
+    const int64_t b = APPEND ? 0 : tok / a.length, l = APPEND ? tok : tok - b * a.length;
+    const T* in;
+    T* out;
+    bool rotate = u < turned;
+    if (h < a.q.heads) {
+      if (APPEND && !s_live[t]) continue;
+      in = static_cast<const T*>(a.q.in) + b * a.q.in_b + l * a.q.in_t + h * a.q.in_h;
+      out = static_cast<T*>(a.q.out) + b * a.q.out_b + l * a.q.out_t + h * a.q.out_h;
+    } else if (h -= a.q.heads; h < a.k.heads) {
+      in = static_cast<const T*>(a.k.in) + b * a.k.in_b + l * a.k.in_t + h * a.k.in_h;
+      if constexpr (APPEND) {
+        if (s_k[t] < 0) continue;
+        out = static_cast<T*>(a.pages.k) + s_k[t] + h * a.pages.k_head;
+      } else {
+        out = static_cast<T*>(a.k.out) + b * a.k.out_b + l * a.k.out_t + h * a.k.out_h;
+      }
+    } else {
+      h -= a.k.heads;
+      if (s_v[t] < 0) continue;
+      in = static_cast<const T*>(a.v.in) + l * a.v.in_t + h * a.v.in_h;
+      out = static_cast<T*>(a.pages.v) + s_v[t] + h * a.pages.v_head;
+      rotate = false;
+    }
+    // element offsets of the unit's two chunks
+    int e1, e2;
+    if (!INTERLEAVED && u < turned) {
+      e1 = u * V;
+      e2 = a.pairs + u * V;
+    } else {
+      e1 = u * 2 * V;
+      e2 = e1 + V;
+    }
+    Chunk<T, V> x = load_chunk<T, V>(in + e1), y = load_chunk<T, V>(in + e2);
+    if (rotate) {
+      const float* cs = s_cos + t * a.pairs + u * V;
+      const float* sn = s_sin + t * a.pairs + u * V;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        T& p1 = INTERLEAVED ? (2 * j < V ? x.x[2 * j] : y.x[2 * j - V]) : x.x[j];
+        T& p2 = INTERLEAVED ? (2 * j + 1 < V ? x.x[2 * j + 1] : y.x[2 * j + 1 - V]) : y.x[j];
+        const float f1 = to_f32<T>(p1), f2 = to_f32<T>(p2), c = cs[j], s = sn[j];
+        p1 = from_f32<T>(f1 * c - f2 * s);
+        p2 = from_f32<T>(f2 * c + f1 * s);
+      }
+    }
+    store_chunk<T, V>(out + e1, x);
+    store_chunk<T, V>(out + e2, y);
+  }
+}
+
+template <typename T, int V, bool APPEND>
+static int launch_v(RotaryArgs& a, bool interleaved, cudaStream_t st) {
+  const int64_t ctas = (a.tokens + a.per_cta - 1) / a.per_cta;
+  if (interleaved)
+    rotary_kernel<T, V, true, APPEND><<<(unsigned)ctas, kRotThreads, 0, st>>>(a);
+  else
+    rotary_kernel<T, V, false, APPEND><<<(unsigned)ctas, kRotThreads, 0, st>>>(a);
+  PPMOE_CHECK_CUDA(cudaGetLastError());
+  return PPMOE_OK;
+}
+
+template <bool APPEND>
+static int launch(RotaryArgs& a, bool interleaved, int dtype, bool wide, cudaStream_t st) {
+  a.per_cta = a.tokens <= 1024 ? 1 : 4;
+  if (dtype == PPMOE_BF16)
+    return wide ? launch_v<__nv_bfloat16, 8, APPEND>(a, interleaved, st)
+                : launch_v<__nv_bfloat16, 1, APPEND>(a, interleaved, st);
+  if (dtype == PPMOE_F16)
+    return wide ? launch_v<__half, 8, APPEND>(a, interleaved, st) : launch_v<__half, 1, APPEND>(a, interleaved, st);
+  if constexpr (!APPEND)
+    return wide ? launch_v<float, 4, false>(a, interleaved, st) : launch_v<float, 1, false>(a, interleaved, st);
+  return PPMOE_ERR_UNSUPPORTED;
+}
+
+// Whether every row of the view starts on a 16-byte boundary.
+static bool wide_view(const void* p, int64_t sb, int64_t st, int64_t sh, int size) {
+  const int64_t v = 16 / size;
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && sb % v == 0 && st % v == 0 && sh % v == 0;
+}
+
+static int check_rotation(const char* fn, int head_dim, int rotary_dim, const double* turns, RotaryArgs& a) {
+  if (head_dim < 2 || head_dim > 2 * kMaxPairs || head_dim % 2 || rotary_dim < 0 || rotary_dim > head_dim ||
+      rotary_dim % 2) {
+    set_error("%s: head_dim=%d must be even and in [2, %d], rotary_dim=%d even and in [0, head_dim]", fn, head_dim,
+              2 * kMaxPairs, rotary_dim);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
+  if (rotary_dim && !turns) {
+    set_error("%s: null turns", fn);
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  a.head_dim = head_dim;
+  a.pairs = rotary_dim / 2;
+  for (int i = 0; i < a.pairs; ++i) a.turns[i] = turns[i];
+  return PPMOE_OK;
+}
+
+int check_pages(const char* fn, const Pages& p, int page_size, int head_dim) {
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) {
+    set_error("%s: page_size=%d must be 16, 32, 64, 128 or 256", fn, page_size);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
+  if (head_dim != 64 && head_dim != 128) {
+    set_error("%s: head_dim=%d must be 64 or 128", fn, head_dim);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
+  if (p.num_pages < 1 || p.kv_heads < 1) {
+    set_error("%s: num_pages=%d and kv_heads=%d must be positive", fn, p.num_pages, p.kv_heads);
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  if (!p.k || !p.v || !wide_view(p.k, p.k_page, p.k_head, p.k_row, 2) ||
+      !wide_view(p.v, p.v_page, p.v_head, p.v_row, 2)) {
+    set_error("%s: cache tensors must be non-null, 16-byte aligned, with strides of whole 16 bytes", fn);
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  return PPMOE_OK;
+}
+
+int check_seqs(const char* fn, const Seqs& s) {
+  if (s.batch < 1 || s.max_pages < 1) {
+    set_error("%s: batch=%d and max_pages=%d must be positive", fn, s.batch, s.max_pages);
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  if (!s.starts || !s.lengths || !s.table) {
+    set_error("%s: null starts, lengths or table", fn);
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  return PPMOE_OK;
+}
+
+}  // namespace ppmoe
+
+using namespace ppmoe;
+
+extern "C" int ppmoe_rotary(const void* q, int64_t q_b, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_b,
+                            int64_t qo_t, int64_t qo_h, int q_heads, const void* k, int64_t k_b, int64_t k_t,
+                            int64_t k_h, void* k_out, int64_t ko_b, int64_t ko_t, int64_t ko_h, int k_heads, int batch,
+                            int64_t length, int head_dim, int rotary_dim, int interleaved, const double* turns,
+                            float gain, int inverse, const void* positions, int positions64, int64_t pos_b,
+                            int64_t pos_t, int dtype, void* stream) {
+  clear_error();
+  RotaryArgs a{};
+  if (int rc = check_rotation("ppmoe_rotary", head_dim, rotary_dim, turns, a)) return rc;
+  if (dtype != PPMOE_BF16 && dtype != PPMOE_F16 && dtype != PPMOE_F32) {
+    set_error("ppmoe_rotary: dtype=%d (0 bf16, 1 fp16, 2 fp32)", dtype);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
+  if (batch < 0 || length < 0 || q_heads < 0 || k_heads < 0 || (batch > 0 && length > (int64_t)INT32_MAX / batch)) {
+    set_error("ppmoe_rotary: batch=%d, length=%lld (batch * length < 2^31), q_heads=%d, k_heads=%d", batch,
+              (long long)length, q_heads, k_heads);
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  if ((int64_t)(q_heads + (int64_t)k_heads) * head_dim > (1 << 24)) {
+    set_error("ppmoe_rotary: %d + %d heads of %d are too many", q_heads, k_heads, head_dim);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
+  a.tokens = batch * length;
+  if (a.tokens == 0 || q_heads + k_heads == 0) return PPMOE_OK;
+  if (!positions || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) {
+    set_error("ppmoe_rotary: null pointer");
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  const int size = dtype == PPMOE_F32 ? 4 : 2, v = 16 / size;
+  a.q = {q, q_out, q_b, q_t, q_h, qo_b, qo_t, qo_h, q_heads};
+  a.k = {k, k_out, k_b, k_t, k_h, ko_b, ko_t, ko_h, k_heads};
+  a.positions = positions;
+  a.pos64 = positions64;
+  a.pos_b = pos_b;
+  a.pos_t = pos_t;
+  a.batch = batch;
+  a.length = length;
+  a.gain = gain;
+  a.sign = inverse ? -1.f : 1.f;
+  const bool wide = head_dim % (2 * v) == 0 && rotary_dim % (2 * v) == 0 &&
+                    (!q_heads || (wide_view(q, q_b, q_t, q_h, size) && wide_view(q_out, qo_b, qo_t, qo_h, size))) &&
+                    (!k_heads || (wide_view(k, k_b, k_t, k_h, size) && wide_view(k_out, ko_b, ko_t, ko_h, size)));
+  return launch<false>(a, interleaved != 0, dtype, wide, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ppmoe_kv_append(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h,
+                               int q_heads, const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t,
+                               int64_t v_h, int tokens, void* k_pages, int64_t kp_page, int64_t kp_head,
+                               int64_t kp_row, void* v_pages, int64_t vp_page, int64_t vp_head, int64_t vp_row,
+                               int num_pages, int page_size, int kv_heads, int head_dim, const int32_t* starts,
+                               const int32_t* lengths, const int32_t* table, int64_t table_stride, int batch,
+                               int max_pages, int rotary_dim, int interleaved, const double* turns, float gain,
+                               int dtype, void* status, void* stream) {
+  clear_error();
+  RotaryArgs a{};
+  a.pages = {k_pages, v_pages, kp_page, kp_head, kp_row, vp_page, vp_head, vp_row, num_pages, 0, kv_heads};
+  a.seqs = {starts, lengths, table, table_stride, batch, max_pages};
+  if (int rc = check_rotation("ppmoe_kv_append", head_dim, rotary_dim, turns, a)) return rc;
+  if (int rc = check_pages("ppmoe_kv_append", a.pages, page_size, head_dim)) return rc;
+  if (int rc = check_seqs("ppmoe_kv_append", a.seqs)) return rc;
+  if (dtype != PPMOE_BF16 && dtype != PPMOE_F16) {
+    set_error("ppmoe_kv_append: dtype=%d (0 bf16, 1 fp16)", dtype);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
+  if (tokens < 0 || q_heads < 0 || (int64_t)(q_heads + 2ll * kv_heads) * head_dim > (1 << 24)) {
+    set_error("ppmoe_kv_append: tokens=%d, q_heads=%d, kv_heads=%d", tokens, q_heads, kv_heads);
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  if (tokens == 0) return PPMOE_OK;
+  if (!k || !v || !status || (q_heads && (!q || !q_out))) {
+    set_error("ppmoe_kv_append: null pointer");
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  while ((1 << a.pages.page_shift) < page_size) ++a.pages.page_shift;
+  a.q = {q, q_out, 0, q_t, q_h, 0, qo_t, qo_h, q_heads};
+  a.k = {k, nullptr, 0, k_t, k_h, 0, 0, 0, kv_heads};
+  a.v = {v, nullptr, 0, v_t, v_h, 0, 0, 0, kv_heads};
+  a.batch = 1;
+  a.length = a.tokens = tokens;
+  a.gain = gain;
+  a.sign = 1.f;
+  a.status = static_cast<uint32_t*>(status);
+  const bool wide = rotary_dim % 16 == 0 && wide_view(k, 0, k_t, k_h, 2) && wide_view(v, 0, v_t, v_h, 2) &&
+                    (!q_heads || (wide_view(q, 0, q_t, q_h, 2) && wide_view(q_out, 0, qo_t, qo_h, 2)));
+  return launch<true>(a, interleaved != 0, dtype, wide, static_cast<cudaStream_t>(stream));
+}

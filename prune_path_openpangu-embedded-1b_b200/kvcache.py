@@ -1,0 +1,187 @@
+"""Paged key/value cache: append with the rotary embedding on the way (``ppmoe_kv_append``) and causal
+attention of the newest tokens over it (``ppmoe_attend``).
+
+A batch is ragged: ``starts [batch + 1]`` cuts the packed rows of ``q``, ``k`` and ``v`` into each
+sequence's newest tokens, ``lengths [batch]`` counts each sequence's positions with these included,
+``table [batch, max_pages]`` names its pages (all int32 on the cache's device).  Rows ``starts[b] + i``
+stand at position ``lengths[b] - (starts[b + 1] - starts[b]) + i``; position ``p`` lies in row
+``p % page_size`` of page ``table[b, p // page_size]``.  The kernels read the three tensors on the
+device, so calls captured into a CUDA graph follow what is written into them.  Rows outside every
+sequence (padding behind ``starts[batch]``) are not read and their outputs not written.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .rotary import RotaryEmbedding, _on, _stream
+
+__all__ = ["PagedKVCache"]
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_PAGE_SIZES = (16, 32, 64, 128, 256)
+
+
+class PagedKVCache:
+    """Keys and values of one layer in pages: ``k``, ``v`` ``[num_pages, kv_heads, page_size, head_dim]``.
+
+    ``page_size`` 16, 32, 64, 128 or 256; ``head_dim`` 64 or 128; bf16 or fp16.  Which page belongs to
+    which sequence is the caller's table; sequences may share pages that neither appends to.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, *,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        if num_pages < 1 or kv_heads < 1:
+            raise ValueError(f"num_pages={num_pages} and kv_heads={kv_heads} must be positive")
+        self._check(page_size, head_dim, dtype)
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        self._mount(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+    @classmethod
+    def from_tensors(cls, k: torch.Tensor, v: torch.Tensor) -> "PagedKVCache":
+        """A cache over given tensors ``[num_pages, kv_heads, page_size, head_dim]``: any strides of whole
+        16 bytes with contiguous heads, so ``[num_pages, page_size, kv_heads, head_dim]`` storage goes in as
+        its ``transpose(1, 2)``."""
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError(f"k {list(k.shape)} {k.dtype} on {k.device} and v {list(v.shape)} {v.dtype} on {v.device} "
+                             "must be alike, [num_pages, kv_heads, page_size, head_dim]")
+        cls._check(k.shape[2], k.shape[3], k.dtype)
+        if k.numel() == 0:
+            raise ValueError("the cache has no pages")
+        for t in (k, v):
+            if t.stride(3) != 1 or any(s % 8 or s == 0 for n, s in zip(t.shape[:3], t.stride()) if n > 1) or t.data_ptr() % 16:
+                raise ValueError("cache tensors need contiguous heads, 16-byte alignment and strides of whole 16 bytes")
+        self = cls.__new__(cls)
+        self._mount(k, v)
+        return self
+
+    @staticmethod
+    def _check(page_size, head_dim, dtype):
+        if page_size not in _PAGE_SIZES:
+            raise ValueError(f"page_size={page_size} must be one of {_PAGE_SIZES}")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim={head_dim} must be 64 or 128")
+        if dtype not in _DTYPES:
+            raise TypeError(f"the cache holds bf16 or fp16, got {dtype}")
+
+    def _mount(self, k, v):
+        if k.device.type != "cuda":
+            raise RuntimeError("PagedKVCache runs on CUDA only; got " + str(k.device))
+        self.k, self.v = k, v
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self.dtype, self.device = k.dtype, k.device
+        self._code = _DTYPES[k.dtype]
+        self._status = torch.zeros(256, dtype=torch.uint8, device=k.device)
+
+        def strides(t):  # a size of one has any stride: give it a harmless one
+            return tuple(s if n > 1 else 8 for n, s in zip(t.shape[:3], t.stride()))
+
+        self._pages = (k.data_ptr(), *strides(k), v.data_ptr(), *strides(v), self.num_pages, self.page_size,
+                       self.kv_heads, self.head_dim)
+
+    # ------------------------------------------------------------------ checks
+    def _rows(self, name, x, heads=None):
+        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
+            raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {self.head_dim}], got {list(x.shape)}")
+        if x.dtype is not self.dtype or x.device != self.device:
+            raise ValueError(f"{name} must be {self.dtype} on {self.device}, got {x.dtype} on {x.device}")
+        return x if x.stride(2) == 1 else x.contiguous()
+
+    def _batch(self, starts, lengths, table):
+        for name, t, dim in (("starts", starts, 1), ("lengths", lengths, 1), ("table", table, 2)):
+            if t.dtype is not torch.int32 or t.device != self.device or t.dim() != dim:
+                raise ValueError(f"{name} must be int32 of {dim} dimension(s) on {self.device}, "
+                                 f"got {t.dtype} {list(t.shape)} on {t.device}")
+        B = lengths.shape[0]
+        if starts.shape[0] != B + 1 or table.shape[0] != B or B < 1 or table.shape[1] < 1:
+            raise ValueError(f"starts {list(starts.shape)}, lengths {list(lengths.shape)} and table {list(table.shape)} "
+                             "must be [batch + 1], [batch] and [batch, max_pages]")
+        if starts.stride(0) != 1 or (B > 1 and lengths.stride(0) != 1) or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError("starts, lengths and the rows of table must be contiguous")
+        return (starts.data_ptr(), lengths.data_ptr(), table.data_ptr(), table.stride(0), B, table.shape[1])
+
+    # ------------------------------------------------------------------ calls
+    @torch.no_grad()
+    def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
+               lengths: torch.Tensor, table: torch.Tensor, *, rotary: Optional[RotaryEmbedding] = None,
+               out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """Writes the rows of ``k`` (rotated to their positions where ``rotary`` is given) and ``v``
+        ``[tokens, kv_heads, head_dim]`` to their places, and returns ``q [tokens, q_heads, head_dim]``
+        rotated likewise: a new tensor, or ``out`` (which may be ``q``).  ``q`` None returns None.  Rows
+        outside every sequence are not written, in ``out`` neither.  The rows of one call must go to
+        different places.  Records no gradients."""
+        k, v = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
+        T = k.shape[0]
+        if v.shape[0] != T or (q is not None and q.shape[0] != T):
+            raise ValueError("q, k and v must have the same number of rows")
+        if rotary is not None and rotary.head_dim != self.head_dim:
+            raise ValueError(f"rotary has head_dim={rotary.head_dim}, the cache {self.head_dim}")
+        batch = self._batch(starts, lengths, table)
+        if q is not None:
+            q = self._rows("q", q)
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            else:
+                self._out(out, q)
+        elif out is not None:
+            raise ValueError("out without q")
+        qa = (None, 0, 0, None, 0, 0, 0) if q is None else (
+            q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), q.shape[1])
+        rot = (0, 0, None, 1.0) if rotary is None else (
+            rotary.rotary_dim, rotary.layout == "interleaved", rotary._turns_ptr, rotary.gain)
+        with _on(self.device):
+            rc = _lib.load().ppmoe_kv_append(
+                *qa, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), T, *self._pages,
+                *batch, *rot, self._code, self._status.data_ptr(), _stream(self.device))
+        if rc:
+            raise _lib.PPMoEError("ppmoe_kv_append", rc, _lib.load().ppmoe_last_error().decode())
+        return out
+
+    @torch.no_grad()
+    def attend(self, q: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, *,
+               max_new: Optional[int] = None, max_length: Optional[int] = None, scale: Optional[float] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of the rows ``q [tokens, q_heads, head_dim]`` over their sequences' positions up to
+        their own (``q_heads`` a multiple of ``kv_heads``; query head ``h`` reads kv head
+        ``h // (q_heads / kv_heads)``).  A row at a negative position gives zeros; rows outside every
+        sequence are not written.  ``max_new`` / ``max_length``: the most new rows and the greatest length of
+        a sequence as far as the host knows (default: the largest possible); they choose how the work is
+        laid out, never what is computed.  ``scale`` defaults to ``head_dim ** -0.5``.  Records no gradients."""
+        q = self._rows("q", q)
+        T, Hq, D = q.shape
+        if Hq < 1 or Hq % self.kv_heads:
+            raise ValueError(f"q has {Hq} heads: not a multiple of the cache's {self.kv_heads}")
+        batch = self._batch(starts, lengths, table)
+        B, cap = batch[4], batch[5] * self.page_size
+        new = T if max_new is None else max(1, min(int(max_new), T))
+        length = cap if max_length is None else max(1, min(int(max_length), cap))
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            self._out(out, q)
+        lib = _lib.load()
+        with _on(self.device):
+            n = lib.ppmoe_attend_workspace_bytes(T, Hq, self.kv_heads, D, B, new, length)
+            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+            rc = lib.ppmoe_attend(
+                q.data_ptr(), q.stride(0), q.stride(1), Hq, T, *self._pages, *batch,
+                D ** -0.5 if scale is None else float(scale), new, length, out.data_ptr(), out.stride(0), out.stride(1),
+                self._code, self._status.data_ptr(), _lib.ptr(ws), n, _stream(self.device))
+        if rc:
+            raise _lib.PPMoEError("ppmoe_attend", rc, lib.ppmoe_last_error().decode())
+        return out
+
+    def _out(self, out, q):
+        if out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or (out.numel() and out.stride(2) != 1):
+            raise ValueError(f"out must be {list(q.shape)} {q.dtype} on {q.device} with contiguous heads")
+        if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+            raise ValueError("out repeats elements")
+
+    def check_device_status(self) -> None:
+        """Synchronise and raise if a call met a position without a page (its row was not stored, or what
+        it gave is not defined); clears the status."""
+        with _on(self.device):
+            _lib.call("ppmoe_workspace_status", self._status.data_ptr(), _stream(self.device))

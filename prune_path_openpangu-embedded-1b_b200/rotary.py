@@ -1,0 +1,200 @@
+"""Rotary position embedding on the GPU (``ppmoe_rotary``), forward and backward.
+
+A head's first ``rotary_dim`` values are pairs; pair ``i`` at position ``p`` is turned by the angle
+``p * f_i``, ``f_i = base ** (-2 i / rotary_dim)``, optionally scaled for contexts longer than the
+trained ones.  The kernel takes the angle from the position itself (reduced in fp64, sine and
+cosine in fp32), so there is no table of a largest position and far positions lose nothing.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+__all__ = ["RotaryEmbedding"]
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+
+
+def _stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _on:
+    """Makes ``device`` current for a launch where it is not (a launch goes to the current device)."""
+
+    def __init__(self, device: torch.device):
+        self.device = device
+
+    def __enter__(self):
+        self.back = torch.cuda.current_device()
+        if self.back != self.device.index:
+            torch.cuda.set_device(self.device)
+
+    def __exit__(self, *exc):
+        if self.back != self.device.index:
+            torch.cuda.set_device(self.back)
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, emb, q, k, positions):
+        ctx.emb = emb
+        ctx.save_for_backward(positions)
+        ctx.set_materialize_grads(False)
+        q2, k2 = emb._launch(q, k, positions, False)
+        return q2, k2
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        (positions,) = ctx.saved_tensors
+        dq, dk = (g if ctx.needs_input_grad[i] else None for i, g in ((1, dq), (2, dk)))
+        if dq is None and dk is None:
+            return None, None, None, None
+        if dq is None:
+            return None, None, ctx.emb._launch(dk, None, positions, True)[0], None
+        dq, dk = ctx.emb._launch(dq, dk, positions, True)
+        return None, dq, dk, None
+
+
+class RotaryEmbedding:
+    """Rotary embedding of ``[..., tokens, heads, head_dim]`` queries and keys.
+
+    ``rotary_dim`` (default ``head_dim``): the leading values of a head that are rotated; even.
+    ``layout``: ``"half"`` pairs value ``i`` with ``i + rotary_dim / 2``, ``"interleaved"`` pairs ``2i``
+    with ``2i + 1``.  ``scaling`` for long contexts, a dict:
+
+    * ``{"type": "linear", "factor": s}``: every frequency divided by ``s``;
+    * ``{"type": "ntk", "factor": s}``: the base multiplied by ``s ** (rotary_dim / (rotary_dim - 2))``,
+      which leaves the fastest pair alone and divides the slowest one by ``s``;
+    * ``{"type": "yarn", "factor": s, "original_length": n}`` (and optionally ``beta_fast`` 32,
+      ``beta_slow`` 1, ``gain``): pairs that turn more than ``beta_fast`` times within ``n`` positions
+      are left alone, those under ``beta_slow`` are divided by ``s``, the ones between are blended by
+      their index; rotated values are multiplied by ``gain`` (default ``0.1 ln s + 1``).
+
+    The object holds numbers only (``turns``: turns per position of each pair, fp64 on the host);
+    a captured launch keeps its own copy of them.  bf16, fp16 and fp32; values are rounded once.
+    """
+
+    def __init__(self, head_dim: int, *, rotary_dim: Optional[int] = None, base: float = 10000.0,
+                 layout: str = "half", scaling: Optional[dict] = None):
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if head_dim < 2 or head_dim > 256 or head_dim % 2:
+            raise ValueError(f"head_dim={head_dim} must be even and in [2, 256]")
+        if rotary_dim < 2 or rotary_dim > head_dim or rotary_dim % 2:
+            raise ValueError(f"rotary_dim={rotary_dim} must be even and in [2, head_dim={head_dim}]")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"layout={layout!r} must be 'half' or 'interleaved'")
+        if not (base > 0 and math.isfinite(base)):
+            raise ValueError(f"base={base} must be positive and finite")
+        self.head_dim, self.rotary_dim, self.layout = head_dim, rotary_dim, layout
+        self.gain = 1.0
+        pair = torch.arange(rotary_dim // 2, dtype=torch.float64)
+        sc = dict(scaling or {})
+        kind = sc.pop("type", None)
+        if scaling is not None and kind not in ("linear", "ntk", "yarn"):
+            raise ValueError(f"scaling type {kind!r} must be 'linear', 'ntk' or 'yarn'")
+        factor = float(sc.pop("factor", 1.0))
+        if not (factor > 0 and math.isfinite(factor)):
+            raise ValueError(f"scaling factor {factor} must be positive and finite")
+        if kind == "ntk":
+            if rotary_dim == 2:
+                raise ValueError("ntk scaling needs rotary_dim > 2")
+            base = base * factor ** (rotary_dim / (rotary_dim - 2))
+        freq = base ** (-2.0 * pair / rotary_dim)
+        if kind == "linear":
+            freq = freq / factor
+        elif kind == "yarn":
+            if "original_length" not in sc or base == 1.0:
+                raise ValueError("yarn scaling needs original_length, and a base other than 1")
+            n = float(sc.pop("original_length"))
+            fast, slow = float(sc.pop("beta_fast", 32.0)), float(sc.pop("beta_slow", 1.0))
+            if not (n > 0 and fast > 0 and slow > 0):
+                raise ValueError("yarn scaling needs positive original_length, beta_fast and beta_slow")
+
+            def index(turns):  # the pair (a fraction) that turns so often within the trained length
+                return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+            low, high = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rotary_dim - 1)
+            keep = 1.0 - ((pair - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+            freq = freq * keep + freq / factor * (1.0 - keep)
+            self.gain = float(sc.pop("gain", 0.1 * math.log(factor) + 1.0))
+        if sc:
+            raise ValueError(f"unknown scaling entries {sorted(sc)}")
+        self.turns = freq / (2.0 * math.pi)
+        self._turns_c = (ctypes.c_double * (rotary_dim // 2))(*self.turns.tolist())
+        self._turns_ptr = ctypes.addressof(self._turns_c)
+
+    # ------------------------------------------------------------------ calls
+    def __call__(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor
+                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """Rotated copies of ``q [(batch,) tokens, q_heads, head_dim]`` and ``k`` (same leading sizes, its
+        own number of heads; or None).  ``positions [(batch,) tokens]`` or ``[tokens]``, int64 or int32.
+        Any strides with contiguous heads; differentiable in ``q`` and ``k``."""
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            return _Rotate.apply(self, q, k, positions)
+        return self._launch(q, k, positions, False)
+
+    def rotate_(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor) -> None:
+        """The same in place (no gradients)."""
+        for x in (q, k):
+            if x is not None and torch.is_grad_enabled() and x.requires_grad:
+                raise RuntimeError("rotate_ records no gradients: call the embedding itself, or use torch.no_grad()")
+            if x is not None and any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+                raise ValueError("rotate_ needs tensors without repeated elements")
+        if k is not None and k.untyped_storage().data_ptr() == q.untyped_storage().data_ptr() and k.data_ptr() == q.data_ptr():
+            raise ValueError("rotate_ needs q and k of their own")
+        self._launch(q, k, positions, False, (q, k))
+
+    def _launch(self, q, k, positions, inverse, out=None):
+        dev = q.device
+        if dev.type != "cuda":
+            raise RuntimeError("RotaryEmbedding runs on CUDA only; got a tensor on " + str(dev))
+        shape = q.shape
+        if len(shape) not in (3, 4) or shape[-1] != self.head_dim:
+            raise ValueError(f"q must be [(batch,) tokens, heads, {self.head_dim}], got {list(shape)}")
+        code = _DTYPES.get(q.dtype)
+        if code is None:
+            raise TypeError(f"RotaryEmbedding takes bf16, fp16 or fp32, got {q.dtype}")
+        if k is not None and (k.dtype != q.dtype or k.device != dev or k.shape[:-2] != shape[:-2]
+                              or k.shape[-1] != self.head_dim):
+            raise ValueError(f"k {list(k.shape)} {k.dtype} on {k.device} does not go with q {list(shape)} {q.dtype} on {dev}")
+        if positions.device != dev or positions.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"positions must be int64 or int32 on {dev}, got {positions.dtype} on {positions.device}")
+        if positions.shape != shape[:-2] and positions.shape != shape[-3:-2]:
+            raise ValueError(f"positions {list(positions.shape)} do not go with q {list(shape)}")
+        if q.stride(-1) != 1:
+            q = q.contiguous()
+        if k is not None and k.stride(-1) != 1:
+            k = k.contiguous()
+        if out is None:
+            q2 = torch.empty(shape, dtype=q.dtype, device=dev)
+            k2 = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+        else:
+            q2, k2 = out
+            if q2.data_ptr() != q.data_ptr() or (k is not None and k2.data_ptr() != k.data_ptr()):
+                raise ValueError("rotate_ needs contiguous heads")
+        four = len(shape) == 4
+        B, L, Hq = (shape[0] if four else 1), shape[-3], shape[-2]
+
+        def strides(t):
+            if t is None:
+                return 0, 0, 0
+            s = t.stride()
+            return (s[0], s[1], s[2]) if four else (0, s[0], s[1])
+
+        pb, pt = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
+        with _on(dev):
+            rc = _lib.load().ppmoe_rotary(
+                q.data_ptr(), *strides(q), q2.data_ptr(), *strides(q2), Hq,
+                _lib.ptr(k), *strides(k), _lib.ptr(k2), *strides(k2), 0 if k is None else k.shape[-2],
+                B, L, self.head_dim, self.rotary_dim, self.layout == "interleaved", self._turns_ptr, self.gain,
+                inverse, positions.data_ptr(), positions.dtype is torch.int64, pb, pt, code, _stream(dev))
+        if rc:
+            raise _lib.PPMoEError("ppmoe_rotary", rc, _lib.load().ppmoe_last_error().decode())
+        return q2, k2

@@ -1,0 +1,392 @@
+"""Paged key/value cache: append and attention against fp64, alone and as a decoder uses them; refusals."""
+import math
+
+import pytest
+import torch
+
+from conftest import pkg
+from paged_helpers import GARBAGE, Batch, assert_attention, assert_rotation, exact_attention, exact_rotation, half_step
+
+HEADS = [(12, 12), (8, 2), (8, 1), (15, 3)]
+
+
+def emb(*a, **k):
+    return pkg().rotary.RotaryEmbedding(*a, **k)
+
+
+# ------------------------------------------------------------------ CPU
+def test_constructor_refusals():
+    C = pkg().kvcache.PagedKVCache
+    for bad in [dict(num_pages=0), dict(page_size=8), dict(page_size=48), dict(page_size=512), dict(kv_heads=0), dict(head_dim=96)]:
+        with pytest.raises(ValueError):
+            C(**{**dict(num_pages=4, page_size=16, kv_heads=2, head_dim=64, device="cpu"), **bad})
+    with pytest.raises(TypeError):
+        C(4, 16, 2, 64, dtype=torch.float32, device="cpu")
+    with pytest.raises(RuntimeError, match="CUDA only"):
+        C(4, 16, 2, 64, device="cpu")
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    for bad in [(k, k[:3]), (k, k.half()), (k[0], k[0]), (k[:0], k[:0]), (k[..., :32], k[..., :32]),
+                (k[:1].expand(4, 2, 16, 64), k), (k, k.transpose(2, 3).contiguous().transpose(2, 3))]:
+        with pytest.raises(ValueError):
+            C.from_tensors(*bad)
+
+
+def test_host_validation_without_gpu():
+    lib = pkg()._lib.load()
+
+    def append(tokens=1, page=16, dim=64, num=4, kvh=2, kp=1024, batch=1, mp=4, rot=0, dtype=0, k=16, status=256, starts=16):
+        return lib.ppmoe_kv_append(None, 0, 0, None, 0, 0, 0, k, 128, 64, 16, 128, 64, tokens, kp, 2048, 1024, 64, 1024, 2048,
+                                   1024, 64, num, page, kvh, dim, starts, 16, 16, mp, batch, mp, rot, 0, None, 1.0, dtype,
+                                   status, None)
+
+    assert append(tokens=0) == 0
+    assert append(page=8) == -2 and append(page=24) == -2 and append(page=512) == -2 and append(dim=96) == -2
+    assert append(num=0) == -1 and append(kvh=0) == -1 and append(kp=1032) == -1 and append(kp=None) == -1
+    assert append(batch=0) == -1 and append(mp=0) == -1 and append(starts=None) == -1
+    assert append(rot=64) == -1 and append(rot=3) == -2 and append(dtype=2) == -2
+    assert append(k=None) == -1 and append(status=None) == -1 and append(tokens=-1) == -1
+
+    def attend(tokens=1, hq=4, page=16, dim=64, kvh=2, dtype=0, q=16, ws=None, n=0, batch=1, new=1, length=64, q_t=256):
+        return lib.ppmoe_attend(q, q_t, 64, hq, tokens, 1024, 2048, 1024, 64, 1024, 2048, 1024, 64, 4, page, kvh, dim, 16, 16,
+                                16, 4, batch, 4, 0.125, new, length, 16, 256, 64, dtype, 256, ws, n, None)
+
+    assert attend(tokens=0) == 0
+    assert attend(hq=3) == -1 and attend(hq=0) == -1 and attend(page=40) == -2 and attend(dim=32) == -2
+    assert attend(dtype=2) == -2 and attend(q=None) == -1 and attend(tokens=-1) == -1 and attend(batch=0) == -1
+
+
+# ------------------------------------------------------------------ GPU: append
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,dim,rot,layout", [(16, 128, 128, "half"), (64, 64, 32, "interleaved"), (256, 128, 4, "half"), (32, 64, 0, "half")])
+@pytest.mark.parametrize("hq,hk", HEADS)
+def test_append(cuda, dtype, page, dim, rot, layout, hq, hk):
+    """Every row lands rotated in its place and nothing else changes; rows behind the last sequence, and
+    their outputs, are left as they were."""
+    e = emb(dim, rotary_dim=rot, layout=layout) if rot else None
+    b = Batch([3, 0, 40, 1, 257], [3, 9, 100, 640, 1000], hk, dim, page, dtype, cuda, seed=1, pad=5)
+    cache = b.cache()
+    fused = b.normal(hq + 2 * hk)
+    q, k, v = fused[:, :hq], fused[:, hq:hq + hk], fused[:, hq + hk:]
+    out = torch.full_like(q.contiguous(), 7.0)
+    want_k, want_v = b.k.clone(), b.v.clone()
+    got = cache.append(q, k, v, b.starts, b.lens, b.table, rotary=e, out=out)
+    assert got is out
+    t = 0
+    for s, (n, length) in enumerate(zip(b.new, b.lengths)):
+        pos = torch.arange(length - n, length, device=cuda)
+        pg, row = b.table[s][pos // page].long(), pos % page
+        if e is not None:
+            assert_rotation(out[t:t + n], *exact_rotation(e, q[t:t + n], pos))
+            assert_rotation(b.k[pg, :, row], *exact_rotation(e, k[t:t + n], pos))
+        else:
+            assert torch.equal(out[t:t + n], q[t:t + n]) and torch.equal(b.k[pg, :, row], k[t:t + n])
+        assert torch.equal(b.v[pg, :, row], v[t:t + n])
+        want_k[pg, :, row], want_v[pg, :, row] = b.k[pg, :, row], b.v[pg, :, row]
+        t += n
+    assert torch.equal(b.k.view(torch.int16), want_k.view(torch.int16))
+    assert torch.equal(b.v.view(torch.int16), want_v.view(torch.int16))
+    assert (out[t:] == 7).all()
+    cache.check_device_status()
+
+
+@pytest.mark.gpu
+def test_append_layouts_and_alignment(cuda):
+    """[page, row, head] storage, no queries, in-place queries, rows at 2-byte offsets."""
+    e = emb(64)
+    b = Batch([20, 7], [30, 40], 2, 64, 16, torch.bfloat16, cuda, nhd=True)
+    cache = b.cache()
+    k, v, q = b.normal(2), b.normal(2), b.normal(4)
+    assert cache.append(None, k, v, b.starts, b.lens, b.table, rotary=e) is None
+    first = b.k.clone()
+    odd = torch.zeros(27 * 2 * 64 + 1, dtype=torch.bfloat16, device=cuda)[1:].view(27, 2, 64).copy_(k)
+    want = cache.append(q, odd, v, b.starts, b.lens, b.table, rotary=e)
+    assert torch.equal(first.view(torch.int16), b.k.view(torch.int16))
+    q2 = q.clone()
+    assert cache.append(q2, k, v, b.starts, b.lens, b.table, rotary=e, out=q2) is q2
+    assert torch.equal(q2, want)
+    pos = torch.arange(10, 30, device=cuda)
+    assert_rotation(b.k[b.table[0][pos // 16].long(), :, pos % 16], *exact_rotation(e, k[:20], pos))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 31, 32, 33, 1000, 1025, 3000])
+def test_append_many_sequences(cuda, batch):
+    """The search for a row's sequence, empty sequences among them."""
+    r = torch.Generator().manual_seed(batch)
+    new = torch.randint(0, 3, (batch,), generator=r).tolist()
+    new[0] += 1
+    b = Batch(new, [n + 5 for n in new], 1, 64, 16, torch.bfloat16, cuda)
+    cache = b.cache()
+    k, v = b.normal(1), b.normal(1)
+    cache.append(None, k, v, b.starts, b.lens, b.table)
+    seq = torch.repeat_interleave(torch.arange(batch, device=cuda), torch.tensor(new, device=cuda))
+    pos = 5 + torch.arange(b.tokens, device=cuda) - b.starts[seq].long()
+    assert torch.equal(b.k[b.table[seq, pos // 16].long(), :, pos % 16], k)
+    assert torch.equal(b.v[b.table[seq, pos // 16].long(), :, pos % 16], v)
+
+
+@pytest.mark.gpu
+def test_append_without_a_page(cuda):
+    """Negative positions, positions behind the table, ids the cache does not have: not stored, reported."""
+    P = pkg()
+    cache = P.kvcache.PagedKVCache(4, 16, 1, 64, device=cuda)
+    k = torch.ones(3, 1, 64, dtype=torch.bfloat16, device=cuda)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    for lengths, table in [([2], [[0, 1]]), ([34], [[0, 1]]), ([3], [[-1, 1]]), ([3], [[4, 1]]), ([3], [[GARBAGE, 1]])]:
+        cache.k.zero_()
+        cache.append(None, k, k, i32(0, 3), i32(*lengths), i32(*table))
+        with pytest.raises(P._lib.PPMoEError, match="without a page"):
+            cache.check_device_status()
+        cache.check_device_status()  # cleared
+        stored = {2: 2, 34: 1, 3: 0}[lengths[0]]
+        assert int((cache.k != 0).any(-1).sum()) == stored
+
+
+# ------------------------------------------------------------------ GPU: attention
+BATCHES = {
+    "one": ([1], [1]),
+    "one page": ([1], [16]),
+    "a key more": ([1], [17]),
+    "steps": ([1] * 7, [1, 15, 16, 17, 128, 129, 1000]),
+    "steps, some idle": ([1, 0, 1, 0], [500, 7, 3, 0]),
+    "proposals": ([5, 1, 3, 4], [300, 1, 129, 4]),
+    "prompts": ([130, 17, 64], [130, 17, 64]),
+    "a prompt": ([257], [257]),
+    "chunks": ([40, 0, 130, 1], [100, 9, 700, 641]),
+    "a chunk": ([300], [1500]),
+    "positions before the start": ([6, 140, 2], [4, 100, 0]),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", BATCHES)
+@pytest.mark.parametrize("dtype,dim,page", [(torch.bfloat16, 128, 16), (torch.float16, 64, 32), (torch.bfloat16, 64, 256), (torch.float16, 128, 64)])
+@pytest.mark.parametrize("hq,hk", HEADS)
+def test_attend(cuda, name, dtype, dim, page, hq, hk):
+    """Every row against fp64, with NaN in all places of the cache that no position has, and padding
+    rows left as they were."""
+    new, lengths = BATCHES[name]
+    b = Batch(new, lengths, hk, dim, page, dtype, cuda, seed=3, pad=2)
+    cache = b.cache()
+    q = b.normal(hq, 2.0)
+    out = torch.full_like(q, 7.0)
+    cache.attend(q, b.starts, b.lens, b.table, max_new=max(new), max_length=max(lengths), out=out)
+    n = sum(new)
+    assert (out[n:] == 7).all()
+    assert_attention(out[:n], *(x[:n] for x in exact_attention(b, q)), what=name)
+    cache.check_device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hk", [(34, 1), (144, 1), (21, 7), (16, 1), (17, 1)])
+@pytest.mark.parametrize("new", [1, 9])
+def test_attend_group_sizes(cuda, hq, hk, new):
+    b = Batch([new, 1], [200, 333], hk, 64, 16, torch.bfloat16, cuda, seed=4)
+    q = b.normal(hq, 2.0)
+    assert_attention(b.cache().attend(q, b.starts, b.lens, b.table, max_new=new), *exact_attention(b, q))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 128, 256])
+@pytest.mark.parametrize("new,length,hq,hk", [(1, 40001, 4, 2), (16, 20003, 4, 2), (64, 9000, 2, 1), (200, 5000, 4, 2), (700, 2777, 3, 1)])
+def test_attend_long(cuda, page, new, length, hq, hk):
+    """Few rows over a long axis (split work), chunks behind a long context."""
+    b = Batch([new, min(new, 2)], [length, 301], hk, 128, page, torch.bfloat16, cuda, seed=5)
+    q = b.normal(hq, 1.5)
+    assert_attention(b.cache().attend(q, b.starts, b.lens, b.table, max_new=new, max_length=length), *exact_attention(b, q))
+
+
+@pytest.mark.gpu
+def test_hints_never_change_what_is_computed(cuda):
+    """max_new and max_length too small, too large and absent."""
+    b = Batch([130, 1, 20], [700, 3000, 20], 2, 128, 32, torch.bfloat16, cuda, seed=6)
+    cache, q = b.cache(), b.normal(8, 2.0)
+    want = exact_attention(b, q)
+    for hints in [{}, dict(max_new=1, max_length=1), dict(max_new=1, max_length=3000), dict(max_new=130, max_length=16),
+                  dict(max_new=4, max_length=10**9), dict(max_new=10**9, max_length=3000), dict(max_new=40, max_length=100)]:
+        out = torch.full_like(q, 7.0)
+        assert_attention(cache.attend(q, b.starts, b.lens, b.table, out=out, **hints), *want, what=str(hints))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_attend_strides_and_scale(cuda, new):
+    """Queries inside a fused projection, [page, row, head] storage, an output with gaps, a scale of its own."""
+    b = Batch([new, 1], [90, 250], 2, 128, 16, torch.float16, cuda, seed=7, nhd=True)
+    fused = b.normal(8, 1.0)
+    q = fused[:, 1:5]
+    wide = torch.full((b.tokens, 6, 128), 7.0, dtype=torch.float16, device=cuda)
+    out = b.cache().attend(q, b.starts, b.lens, b.table, scale=0.21, out=wide[:, 1:5], max_new=new)
+    assert_attention(out, *exact_attention(b, q, 0.21))
+    assert (wide[:, 0] == 7).all() and (wide[:, 5] == 7).all()
+    odd = torch.zeros(q.numel() + 1, dtype=torch.float16, device=cuda)[1:].view(q.shape).copy_(q)
+    gap = torch.zeros(q.numel() + 1, dtype=torch.float16, device=cuda)[1:].view(q.shape)
+    assert torch.equal(b.cache().attend(odd, b.starts, b.lens, b.table, scale=0.21, out=gap, max_new=new), out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 5, 40, 300])
+def test_attend_wide_ranges(cuda, new):
+    """Scores that grow along the keys (the running maximum moves at every step), large negative ones,
+    and one key that takes all the weight."""
+    b = Batch([new], [900], 1, 128, 64, torch.bfloat16, cuda, seed=8)
+    q = torch.zeros(new, 2, 128, dtype=torch.bfloat16, device=cuda)
+    q[:, 0, 0], q[:, 1, 0] = 8.0, -8.0
+    k = b.keys[0]
+    k.zero_()
+    k[:, 0, 0] = torch.arange(900, device=cuda) // 4
+    pos = torch.arange(900, device=cuda)
+    b.k[b.table[0][pos // 64].long(), :, pos % 64] = k
+    assert_attention(b.cache().attend(q, b.starts, b.lens, b.table, scale=1.0, max_new=new), *exact_attention(b, q, 1.0))
+    assert_attention(b.cache().attend(q, b.starts, b.lens, b.table, scale=-0.01, max_new=new), *exact_attention(b, q, -0.01))
+    assert_attention(b.cache().attend(q, b.starts, b.lens, b.table, scale=0.0, max_new=new), *exact_attention(b, q, 0.0))
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(cuda):
+    """A cache of more than 2^31 values whose used pages lie at its end."""
+    pages, page, hk = 140_000, 256, 1
+    C = pkg().kvcache.PagedKVCache
+    k = torch.empty(pages, hk, page, 64, dtype=torch.bfloat16, device=cuda)
+    v = torch.empty_like(k)
+    assert k.numel() > 2**31
+    g = torch.Generator(device=cuda).manual_seed(1)
+    b = Batch([1, 40], [600, 500], hk, 64, page, torch.bfloat16, cuda, seed=9)
+    used = b.k.shape[0]
+    b.table = torch.where(b.table == GARBAGE, b.table, b.table + (pages - used))
+    k[-used:], v[-used:] = b.k, b.v
+    cache = C.from_tensors(k, v)
+    q = b.normal(4, 2.0)
+    for hint in (1, 40):
+        assert_attention(cache.attend(q, b.starts, b.lens, b.table, max_new=hint), *exact_attention(b, q))
+    nk, nv = b.normal(1), b.normal(1)
+    cache.append(None, nk, nv, b.starts, b.lens, b.table)
+    assert torch.equal(k[b.table[0, 2].long(), 0, 599 % 256], nk[0, 0]) and torch.equal(v[b.table[1, 1].long(), 0, 499 % 256], nv[40, 0])
+    del k, v, cache
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_attend_without_a_page(cuda, new):
+    """Lengths beyond the table and ids that the cache does not have are reported; other sequences are
+    computed as ever."""
+    P = pkg()
+    b = Batch([new, new], [100, 90], 1, 64, 16, torch.bfloat16, cuda, seed=10)
+    cache, q = b.cache(), b.normal(2, 2.0)
+    want = exact_attention(b, q)
+    for spoil in ("id", "negative", "length"):
+        table, lens = b.table.clone(), b.lens.clone()
+        if spoil == "length":
+            lens[0] = 10_000
+        else:
+            table[0, 2] = GARBAGE if spoil == "id" else -1
+        out = cache.attend(q, b.starts, lens, table, max_new=new)
+        with pytest.raises(P._lib.PPMoEError, match="without a page"):
+            cache.check_device_status()
+        assert_attention(out[new:], want[0][new:], want[1][new:])
+    cache.check_device_status()
+
+
+@pytest.mark.gpu
+def test_same_bits_every_time(cuda):
+    b = Batch([1, 1, 5, 300], [9000, 17, 4000, 2000], 2, 128, 32, torch.bfloat16, cuda, seed=11)
+    cache, q = b.cache(), b.normal(8, 2.0)
+    for new in (1, 16, 300):
+        first = cache.attend(q, b.starts, b.lens, b.table, max_new=new)
+        for _ in range(5):
+            assert torch.equal(first, cache.attend(q, b.starts, b.lens, b.table, max_new=new))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 20])
+def test_graphs_and_streams(cuda, new):
+    """Two captured calls on one cache replayed at once on two streams, following the batch's contents."""
+    b = Batch([new, new], [3000, 2000], 2, 128, 32, torch.bfloat16, cuda, seed=12)
+    cache, q1 = b.cache(), b.normal(8, 2.0)
+    q2 = b.normal(8, 1.0)
+    lens = b.lens.clone()
+    cache.attend(q1, b.starts, lens, b.table, max_new=new)
+    graphs, outs = [], []
+    for q in (q1, q2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(cache.attend(q, b.starts, lens, b.table, max_new=new, max_length=3000))
+        graphs.append(g)
+    lens.copy_(torch.tensor([2500, 1900], device=cuda))
+    shorter = Batch([new, new], [3000, 2000], 2, 128, 32, torch.bfloat16, cuda, seed=12)
+    shorter.lengths = [2500, 1900]
+    shorter.keys = [k[:n] for k, n in zip(shorter.keys, shorter.lengths)]
+    shorter.values = [v[:n] for v, n in zip(shorter.values, shorter.lengths)]
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for q, out in zip((q1, q2), outs):
+        assert_attention(out, *exact_attention(shorter, q))
+
+
+@pytest.mark.gpu
+def test_refusals(cuda):
+    b = Batch([3, 1], [30, 20], 2, 64, 16, torch.bfloat16, cuda)
+    cache, q = b.cache(), b.normal(4)
+    k = b.normal(2)
+    ok = (b.starts, b.lens, b.table)
+    for bad in [(b.starts.long(), b.lens, b.table), (b.starts, b.lens.cpu(), b.table), (b.starts[:-1], b.lens, b.table),
+                (b.starts, b.lens, b.table[:1]), (b.starts, b.lens, b.table[0]), (b.starts, b.lens, b.table[:, :0]),
+                (b.starts[:1], b.lens[:0], b.table[:0]), (b.starts, b.lens, b.table.repeat(1, 2)[:, ::2])]:
+        with pytest.raises(ValueError):
+            cache.attend(q, *bad)
+        with pytest.raises(ValueError):
+            cache.append(q, k, k, *bad)
+    for bad in [q[:, :3], q[..., :32], q.half(), q[0], q.cpu(), q[:, :0]]:
+        with pytest.raises(ValueError):
+            cache.attend(bad, *ok)
+    for out in [q[:3], q.half(), torch.empty(4, 4, 64, device=cuda, dtype=torch.bfloat16).cpu(), k[:, :1].expand(4, 4, 64)]:
+        with pytest.raises(ValueError):
+            cache.attend(q, *ok, out=out)
+    for args in [(q, k, k[:3]), (q[:3], k, k), (q, q, q), (q, k[:, :1], k)]:
+        with pytest.raises(ValueError):
+            cache.append(*args, *ok)
+    with pytest.raises(ValueError):
+        cache.append(q, k, k, *ok, rotary=emb(128))
+    with pytest.raises(ValueError):
+        cache.append(None, k, k, *ok, out=q)
+
+
+# ------------------------------------------------------------------ GPU: together
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hq,hk,dim", [(torch.bfloat16, 12, 12, 128), (torch.float16, 8, 2, 64)])
+def test_chunks_and_steps_together(cuda, dtype, hq, hk, dim):
+    """Prompts taken in chunks and then token by token, appended and attended in turn, against causal
+    attention in fp64 over the same rotated keys."""
+    e = emb(dim)
+    cache = pkg().kvcache.PagedKVCache(64, 16, hk, dim, dtype=dtype, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    total = [150, 61]
+    q, k, v = ([torch.randn(n, h, dim, generator=g, device=cuda).to(dtype) for n in total] for h in (hq, hk, hk))
+    table = torch.randperm(64, generator=g, device=cuda)[:2 * 12].view(2, 12).to(torch.int32)
+    done = [0, 0]
+    outs = [[], []]
+    for new in [(40, 40), (90, 1), (0, 9), (1, 1), (1, 1), (3, 0), (1, 1), (14, 8)]:
+        cut = lambda x: torch.cat([x[s][done[s]:done[s] + new[s]] for s in (0, 1)])  # noqa: E731
+        starts = torch.tensor([0, new[0], sum(new)], dtype=torch.int32, device=cuda)
+        rows = cut(q), cut(k), cut(v)
+        done = [done[s] + new[s] for s in (0, 1)]
+        lens = torch.tensor(done, dtype=torch.int32, device=cuda)
+        q2 = cache.append(*rows, starts, lens, table, rotary=e)
+        o = cache.attend(q2, starts, lens, table, max_new=max(new), max_length=max(done))
+        outs[0].append(o[:new[0]])
+        outs[1].append(o[new[0]:])
+    assert done == total
+    for s in (0, 1):
+        pos = torch.arange(total[s], device=cuda)
+        # the rows as stored: rotated, rounded once
+        qr, kr = e(q[s], k[s], pos)
+        whole = Batch([total[s]], [total[s]], hk, dim, 16, dtype, cuda)
+        whole.keys, whole.values = [kr], [v[s]]
+        assert_attention(torch.cat(outs[s]), *exact_attention(whole, qr))
