@@ -3,9 +3,21 @@
 //   out[t, h] = sum_{j <= p(t)} w_j v_j,  w = softmax_j(scale q[t, h] . k_j),  p(t) = position of t
 // and 0 where no key is left (p(t) < 0).
 //
-// One warp per (token, head): one pass over the keys with the running maximum m and sum l of
-// the softmax; every lane holds head_dim / 32 values of the query and of the sum.
+// All query rows of a sequence that read one kv head (its new tokens x the `group` query heads of
+// that head) are one matrix of n * group rows; row r is token r / group, head r % group of the group.
+// Scores are kept in base 2: x = c q.k with c = |scale| log2 e (a negative scale turns the sign of
+// q, which is exact), w = 2^(x - m) / sum.  One pass over the keys keeps the running maximum m
+// and sum l in fp32; weights are rounded once to the cache's type for the second product.
+//
+// A masked key must not reach a row even where its value is not finite (0 * inf = NaN): tiles that
+// some row sees in part are searched for such values.  They are taken out of the product, and
+// added (they are what the sum becomes) to the rows that see their key.
+#include <math_constants.h>
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
 #include "seqs.cuh"
+#include "umma.cuh"
 
 namespace ppmoe {
 
@@ -15,59 +27,516 @@ struct AttendArgs {
   void* out;
   int64_t o_t, o_h;
   int tokens, q_heads, group;
-  float scale;
+  float c;         // |scale| log2 e (1 where scale is 0)
+  int q_sign;      // -1, 0, 1: what q is multiplied by
+  int q_wide;      // rows of q start on 4-byte (thin kernel) / 16-byte boundaries
+  int o_wide;      // rows of out start on 16-byte boundaries
+  int nsplit;      // parts of the keys; above 1 they meet in ws
+  float* part_o;   // [nsplit][tokens][q_heads][D]: sum of 2^(x - m) v
+  float* part_ml;  // [nsplit][tokens][q_heads][2]: m, l
   Seqs seqs;
   Pages pages;
   uint32_t* status;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_rows_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int t = (int)(item / a.q_heads), h = (int)(item % a.q_heads);
-  if (t >= a.tokens) return;
-  const int b = find_seq_warp(a.seqs.starts, a.seqs.batch, t);
-  if (b < 0 || b >= a.seqs.batch) return;
-  const int pos = a.seqs.lengths[b] - a.seqs.starts[b + 1] + t;
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Sequence b as the kernels see it: its first packed row, its new rows, its length held to what the
+// table can name (reported), and to what `tokens` rows can hold.
+struct Seq {
+  int first, rows, length;
+};
+__device__ __forceinline__ Seq load_seq(const AttendArgs& a, int b) {
+  Seq s;
+  s.first = a.seqs.starts[b];
+  int end = a.seqs.starts[b + 1];
+  s.length = a.seqs.lengths[b];
+  if (s.first < 0) s.first = 0;
+  if (end > a.tokens) end = a.tokens;
+  s.rows = end - s.first;
+  return s;
+}
+// Position of the sequence's first new row; keys a row at position pos may see.
+__device__ __forceinline__ int key_cap(const AttendArgs& a, int length) {
   const int64_t cap = (int64_t)a.seqs.max_pages << a.pages.page_shift;
-  const int keys = (int)(pos + 1 < cap ? pos + 1 : cap);
-  float q[N], o[N], m = -INFINITY, l = 0.f;
+  return length < cap ? length : (int)cap;
+}
+
+
+// C rounded values of one row piece, scaled by inv.
+template <typename T, int C>
+__device__ __forceinline__ void store_row(T* out, const float (&v)[C], float inv, bool wide) {
+  if (wide) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    q[i] = to_f32<T>(static_cast<const T*>(a.q)[t * a.q_t + h * a.q_h + lane + 32 * i]) * a.scale;
-    o[i] = 0.f;
+    for (int i = 0; i < C; i += 8)
+      *reinterpret_cast<uint4*>(out + i) =
+          make_uint4(pack2<T>(v[i] * inv, v[i + 1] * inv), pack2<T>(v[i + 2] * inv, v[i + 3] * inv),
+                     pack2<T>(v[i + 4] * inv, v[i + 5] * inv), pack2<T>(v[i + 6] * inv, v[i + 7] * inv));
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) out[i] = from_f32<T>(v[i] * inv);
   }
-  for (int j = 0; j < keys; ++j) {
-    const int page = a.seqs.table[b * a.seqs.table_stride + (j >> a.pages.page_shift)];
-    if (page < 0 || page >= a.pages.num_pages) {
-      atomicOr(a.status, DEVERR_PAGE);
-      continue;
-    }
-    const int64_t row = j & ((1 << a.pages.page_shift) - 1);
-    const T* k = static_cast<const T*>(a.pages.k) + page * a.pages.k_page + row * a.pages.k_row + (h / a.group) * a.pages.k_head;
-    const T* v = static_cast<const T*>(a.pages.v) + page * a.pages.v_page + row * a.pages.v_row + (h / a.group) * a.pages.v_head;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) s += q[i] * to_f32<T>(k[lane + 32 * i]);
-    s = warp_sum(s);
-    const float m2 = fmaxf(m, s), c = m2 == -INFINITY ? 1.f : __expf(m - m2), p = m2 == -INFINITY ? 0.f : __expf(s - m2);
-    m = m2;
-    l = l * c + p;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * c + p * to_f32<T>(v[lane + 32 * i]);
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    static_cast<T*>(a.out)[t * a.o_t + h * a.o_h + lane + 32 * i] = from_f32<T>(l != 0.f ? o[i] / l : 0.f);
+}
+
+// ======================================================================== few rows
+// Up to 16 rows at a time per (sequence, kv head): one token per sequence up to a few.  Bound by
+// the cache's bytes.  Each warp takes 32 keys at a time through a ring of its own (cp.async, no block
+// barrier), m16n8k16 products (rows padded to 16: the tensor pipe has room, it is the loads that
+// count), and the warps' and then the parts' (m, l, sum) are joined at the end.
+constexpr int kThinWarps = 4;
+constexpr int kThinKeys = 32;
+constexpr int kThinStages = 3;
+
+template <int D>
+struct ThinSmem {
+  static constexpr int kTile = kThinKeys * D * 2;         // bytes of K (or V) of one stage
+  static constexpr int kWarp = kThinStages * 2 * kTile;   // bytes of one warp's ring
+  static constexpr int kJoin = kThinWarps * (16 * (D + 4) + 32) * 4;
+  static constexpr int kBytes = kThinWarps * kWarp > kJoin ? kThinWarps * kWarp : kJoin;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes global -> shared, or 16 zero bytes (the source is then not read).
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
+// What q is multiplied by (-1, 0 or 1), on a packed pair.
+__device__ __forceinline__ uint32_t q_pair(uint32_t v, int sign) {
+  return sign > 0 ? v : sign < 0 ? v ^ 0x80008000u : 0u;
+}
+
+// Fp16 weights below 2^-24 would vanish; lifting every weight by 2^8 (it cancels against l) keeps
+// those down to 2^-32 of the largest.  bf16 has fp32's exponents and needs none.
+template <typename T>
+constexpr float kLift = 0.f;
+template <>
+constexpr float kLift<__half> = 8.f;
+
+// Exponent field all ones: inf or NaN.
+template <typename T>
+__device__ __forceinline__ bool not_finite16(uint32_t v) {  // v: the 16 bits
+  constexpr uint32_t m = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (v & m) == m;
+}
+template <typename T>
+__device__ __forceinline__ bool not_finite2(uint32_t v) {
+  return not_finite16<T>(v) || not_finite16<T>(v >> 16);
 }
 
 template <typename T, int D>
-static int launch(const AttendArgs& a, cudaStream_t st) {
+__global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const __grid_constant__ AttendArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  using S = ThinSmem<D>;
+  constexpr int KS = D / 16;     // k-steps of q.k
+  constexpr int NT = D / 8;      // n-tiles of the output
+  constexpr int CH = D / 8;      // 16-byte chunks of a row
+  constexpr int RPI = 32 / CH;   // rows one copy instruction of the warp takes
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int split = blockIdx.x % a.nsplit;
+  const int kvh = (blockIdx.x / a.nsplit) % a.pages.kv_heads;
+  const int b = blockIdx.x / (a.nsplit * a.pages.kv_heads);
+  pdl_launch_dependents();
+  const Seq sq = load_seq(a, b);
+  if (sq.rows <= 0) return;
+  const int cap = key_cap(a, sq.length);
+  if (cap < sq.length && tid == 0) atomicOr(a.status, DEVERR_PAGE);
+  const int pos0 = sq.length - (a.seqs.starts[b + 1] - a.seqs.starts[b]);  // position of row 0
+  const int rows = sq.rows * a.group;
+  const int32_t* table = a.seqs.table + b * a.seqs.table_stride;
+  const int shift = a.pages.page_shift;
+  const uint32_t ring = smem_u32(smem) + warp * S::kWarp;
+  float* j_o = reinterpret_cast<float*>(smem);              // [warps][16][D + 4]
+  float* j_ml = j_o + kThinWarps * 16 * (D + 4);            // [warps][16][2]
+
+  for (int r0 = 0; r0 < rows; r0 += 16) {
+    const int last = r0 + 15 < rows ? r0 + 15 : rows - 1;
+    const int pos_lo = pos0 + r0 / a.group, pos_hi = pos0 + last / a.group;
+    const int keys = pos_hi + 1 < cap ? pos_hi + 1 : cap;  // keys some row sees
+    const int blocks = keys > 0 ? (keys + kThinKeys - 1) / kThinKeys : 0;
+    const int per = (blocks + a.nsplit - 1) / a.nsplit;
+    const int blk_end = min(blocks, (split + 1) * per);
+    int blk = split * per + warp;
+
+    // this thread's two rows: how far they see (-1: nothing), their q fragments
+    const int ra = r0 + (lane >> 2), rb = ra + 8;
+    const int lim_a = ra < rows ? pos0 + ra / a.group : -1, lim_b = rb < rows ? pos0 + rb / a.group : -1;
+    uint32_t qf[KS][4];
+    {
+      const T* qa = nullptr;
+      const T* qb = nullptr;
+      if (ra < rows)
+        qa = static_cast<const T*>(a.q) + (int64_t)(sq.first + ra / a.group) * a.q_t + (int64_t)(kvh * a.group + ra % a.group) * a.q_h;
+      if (rb < rows)
+        qb = static_cast<const T*>(a.q) + (int64_t)(sq.first + rb / a.group) * a.q_t + (int64_t)(kvh * a.group + rb % a.group) * a.q_h;
+      auto pair = [&](const T* p, int e) -> uint32_t {
+        if (!p) return 0u;
+        if (a.q_wide) return q_pair(__ldg(reinterpret_cast<const uint32_t*>(p + e)), a.q_sign);
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(p + e);
+        return q_pair(h[0] | (uint32_t)h[1] << 16, a.q_sign);
+      };
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int e = k * 16 + (lane & 3) * 2;
+        qf[k][0] = pair(qa, e);
+        qf[k][1] = pair(qb, e);
+        qf[k][2] = pair(qa, e + 8);
+        qf[k][3] = pair(qb, e + 8);
+      }
+    }
+
+    // pages of a block's two halves of 16 keys (one page, or two of 16 rows)
+    auto ids = [&](int bk, int& p0, int& p1) {
+      const int key = bk * kThinKeys;
+      p0 = bk < blk_end ? __ldg(table + (key >> shift)) : -1;
+      p1 = bk < blk_end && key + 16 < keys ? __ldg(table + ((key + 16) >> shift)) : -1;
+    };
+    auto fetch = [&](int bk, int stage, int p0, int p1) {
+      if (bk < blk_end) {
+        const int key = bk * kThinKeys;
+        const uint32_t kd = ring + stage * 2 * S::kTile, vd = kd + S::kTile;
+        const bool ok0 = (uint32_t)p0 < (uint32_t)a.pages.num_pages;
+        const bool ok1 = (uint32_t)p1 < (uint32_t)a.pages.num_pages;
+        if (lane == 0 && (!ok0 || (!ok1 && key + 16 < keys))) atomicOr(a.status, DEVERR_PAGE);
+        const int in = key & ((1 << shift) - 1), in1 = (key + 16) & ((1 << shift) - 1);
+        const int c = lane % CH, rr = lane / CH;
+        const T* kb0 = static_cast<const T*>(a.pages.k) + kvh * a.pages.k_head + c * 8;
+        const T* vb0 = static_cast<const T*>(a.pages.v) + kvh * a.pages.v_head + c * 8;
+        const T* kb1 = kb0 + (ok1 ? p1 * a.pages.k_page + (in1 + rr) * a.pages.k_row : 0);
+        const T* vb1 = vb0 + (ok1 ? p1 * a.pages.v_page + (in1 + rr) * a.pages.v_row : 0);
+        kb0 += ok0 ? p0 * a.pages.k_page + (in + rr) * a.pages.k_row : 0;
+        vb0 += ok0 ? p0 * a.pages.v_page + (in + rr) * a.pages.v_row : 0;
+#pragma unroll
+        for (int i = 0; i < kThinKeys / RPI; ++i) {
+          const int row = i * RPI + rr;
+          const bool hi = i * RPI >= 16;
+          const bool real = (hi ? ok1 : ok0) && key + row < keys;
+          const int64_t off = (i * RPI) & 15;
+          const uint32_t d = row * (D * 2) + ((c ^ (row & 7)) << 4);
+          cp_async16_or_zero(kd + d, (hi ? kb1 : kb0) + (real ? off * a.pages.k_row : 0), real);
+          cp_async16_or_zero(vd + d, (hi ? vb1 : vb0) + (real ? off * a.pages.v_row : 0), real);
+        }
+      }
+      cp_async_commit();
+    };
+
+    float o[NT][4], m_a = -CUDART_INF_F, m_b = -CUDART_INF_F, l_a = 0.f, l_b = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+
+    int p0, p1;
+#pragma unroll
+    for (int s = 0; s < kThinStages - 1; ++s) {
+      ids(blk + s * kThinWarps, p0, p1);
+      fetch(blk + s * kThinWarps, s, p0, p1);
+    }
+    ids(blk + (kThinStages - 1) * kThinWarps, p0, p1);
+    int stage = 0;
+#pragma unroll 1
+    for (; blk < blk_end; blk += kThinWarps) {
+      {
+        const int ahead = blk + (kThinStages - 1) * kThinWarps;
+        int st = stage + kThinStages - 1;
+        if (st >= kThinStages) st -= kThinStages;
+        fetch(ahead, st, p0, p1);
+        ids(ahead + kThinWarps, p0, p1);
+      }
+      cp_async_wait<kThinStages - 1>();
+      __syncwarp();
+      const uint32_t kd = ring + stage * 2 * S::kTile, vd = kd + S::kTile;
+      const int key = blk * kThinKeys;
+
+      float s[4][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // matrices: keys h*16 + 0..7 (two k halves), then keys + 8
+          const int row = h * 16 + (lane & 7) + ((lane >> 4) << 3);
+          const int ch = k * 2 + ((lane >> 3) & 1);
+          uint32_t f[4];
+          ldsm4(f, kd + row * (D * 2) + ((ch ^ (row & 7)) << 4));
+          mma16<T>(s[2 * h], qf[k], f[0], f[1]);
+          mma16<T>(s[2 * h + 1], qf[k], f[2], f[3]);
+        }
+      }
+      const bool partly = key + kThinKeys > pos_lo + 1 || key + kThinKeys > keys;
+      float mx_a = m_a, mx_b = m_b;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] *= a.c;
+        if (partly) {
+          const int j = key + n * 8 + (lane & 3) * 2;
+          if (j > lim_a || j >= cap) s[n][0] = -CUDART_INF_F;
+          if (j + 1 > lim_a || j + 1 >= cap) s[n][1] = -CUDART_INF_F;
+          if (j > lim_b || j >= cap) s[n][2] = -CUDART_INF_F;
+          if (j + 1 > lim_b || j + 1 >= cap) s[n][3] = -CUDART_INF_F;
+        }
+        mx_a = fmaxf(mx_a, fmaxf(s[n][0], s[n][1]));
+        mx_b = fmaxf(mx_b, fmaxf(s[n][2], s[n][3]));
+      }
+#pragma unroll
+      for (int x = 1; x < 4; x <<= 1) {
+        mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, x));
+        mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, x));
+      }
+      if (__any_sync(0xffffffffu, mx_a > m_a || mx_b > m_b)) {
+        // old sums to the new maxima (a row without keys so far has sums of 0)
+        const float f_a = m_a == -CUDART_INF_F ? 0.f : exp2_ftz(m_a - mx_a);
+        const float f_b = m_b == -CUDART_INF_F ? 0.f : exp2_ftz(m_b - mx_b);
+        l_a *= f_a;
+        l_b *= f_b;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          o[n][0] *= f_a;
+          o[n][1] *= f_a;
+          o[n][2] *= f_b;
+          o[n][3] *= f_b;
+        }
+        m_a = mx_a;
+        m_b = mx_b;
+      }
+      const float sub_a = (m_a == -CUDART_INF_F ? 0.f : m_a) - kLift<T>;
+      const float sub_b = (m_b == -CUDART_INF_F ? 0.f : m_b) - kLift<T>;
+      uint32_t pf[2][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float e0 = exp2_ftz(s[n][0] - sub_a), e1 = exp2_ftz(s[n][1] - sub_a);
+        const float e2 = exp2_ftz(s[n][2] - sub_b), e3 = exp2_ftz(s[n][3] - sub_b);
+        l_a += e0 + e1;
+        l_b += e2 + e3;
+        pf[n >> 1][(n & 1) * 2] = pack2<T>(e0, e1);
+        pf[n >> 1][(n & 1) * 2 + 1] = pack2<T>(e2, e3);
+      }
+      if (partly) {  // values that are not finite, of keys that some row does not see
+        bool bad = false;
+#pragma unroll 4
+        for (int i = lane; i < kThinKeys * D / 2; i += 32) {
+          uint32_t v;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(vd + i * 4) : "memory");
+          bad |= not_finite2<T>(v);
+        }
+        if (__any_sync(0xffffffffu, bad)) {
+          for (int j = 0; j < kThinKeys; ++j) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint32_t at = vd + j * (D * 2) + ((n ^ (j & 7)) << 4) + (lane & 3) * 4;
+              uint32_t v;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+              __syncwarp();
+              uint32_t keep = v;
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint16_t bits = (uint16_t)(v >> (16 * e));
+                if (not_finite16<T>(bits)) {
+                  const float f = to_f32<T>(*reinterpret_cast<const T*>(&bits));
+                  if (key + j <= lim_a) o[n][e] += f;
+                  if (key + j <= lim_b) o[n][2 + e] += f;
+                  keep &= e ? 0xffffu : 0xffff0000u;
+                }
+              }
+              if (lane < 4 && keep != v) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(keep) : "memory");
+            }
+          }
+          __syncwarp();
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          // matrices: keys h*16 + 0..7 and + 8 of columns n, then of columns n + 1
+          const int row = h * 16 + (lane & 15), ch = n + (lane >> 4);
+          uint32_t f[4];
+          ldsm4_t(f, vd + row * (D * 2) + ((ch ^ (row & 7)) << 4));
+          mma16<T>(o[n], pf[h], f[0], f[1]);
+          mma16<T>(o[n + 1], pf[h], f[2], f[3]);
+        }
+      }
+      __syncwarp();
+      stage = stage + 1 == kThinStages ? 0 : stage + 1;
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      l_a += __shfl_xor_sync(0xffffffffu, l_a, x);
+      l_b += __shfl_xor_sync(0xffffffffu, l_b, x);
+    }
+    __syncthreads();  // every warp is through with its ring
+    {
+      float* oa = j_o + (warp * 16 + (lane >> 2)) * (D + 4) + (lane & 3) * 2;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        *reinterpret_cast<float2*>(oa + n * 8) = make_float2(o[n][0], o[n][1]);
+        *reinterpret_cast<float2*>(oa + 8 * (D + 4) + n * 8) = make_float2(o[n][2], o[n][3]);
+      }
+      if ((lane & 3) == 0) {
+        float* ml = j_ml + (warp * 16 + (lane >> 2)) * 2;
+        ml[0] = m_a;
+        ml[1] = l_a;
+        ml[16] = m_b;
+        ml[17] = l_b;
+      }
+    }
+    __syncthreads();
+    {
+      constexpr int C = D / 8;  // columns of one thread
+      const int row = tid >> 3, col = (tid & 7) * C, r = r0 + row;
+      if (r < rows) {
+        float m = -CUDART_INF_F, l = 0.f, f[kThinWarps], acc[C];
+#pragma unroll
+        for (int w = 0; w < kThinWarps; ++w) m = fmaxf(m, j_ml[(w * 16 + row) * 2]);
+#pragma unroll
+        for (int w = 0; w < kThinWarps; ++w) {
+          const float mw = j_ml[(w * 16 + row) * 2];
+          f[w] = mw == -CUDART_INF_F ? 0.f : exp2_ftz(mw - m);
+          l += f[w] * j_ml[(w * 16 + row) * 2 + 1];
+        }
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          acc[i] = 0.f;
+#pragma unroll
+          for (int w = 0; w < kThinWarps; ++w) acc[i] += f[w] * j_o[(w * 16 + row) * (D + 4) + col + i];
+        }
+        const int64_t t = sq.first + r / a.group;
+        const int h = kvh * a.group + r % a.group;
+        if (a.nsplit == 1) {
+          store_row<T, C>(static_cast<T*>(a.out) + t * a.o_t + h * a.o_h + col, acc, l > 0.f ? 1.f / l : l == l ? 0.f : l,
+                          a.o_wide);
+        } else {
+          const int64_t at = ((int64_t)split * a.tokens + t) * a.q_heads + h;
+#pragma unroll
+          for (int i = 0; i < C; i += 4)
+            *reinterpret_cast<float4*>(a.part_o + at * D + col + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+          if (col == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+        }
+      }
+    }
+    __syncthreads();  // before the next rows' copies
+  }
+}
+
+// ======================================================================== joining the parts
+// One warp per (token, head): out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, in part order.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int C = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int64_t items = (int64_t)a.tokens * a.q_heads;
-  attend_rows_kernel<T, D><<<(unsigned)((items + 3) / 4), 128, 0, st>>>(a);
+  if (item >= items) return;
+  const int t = (int)(item / a.q_heads), h = (int)(item % a.q_heads);
+  const int first = a.seqs.starts[0], end = a.seqs.starts[a.seqs.batch];
+  pdl_wait();  // the parts are complete and visible
+  if (t < first || t >= end) return;
+  float m = -CUDART_INF_F;
+  for (int s = lane; s < a.nsplit; s += 32) m = fmaxf(m, a.part_ml[(s * items + item) * 2]);
+  m = warp_max(m);
+  float l = 0.f, acc[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) acc[i] = 0.f;
+  for (int s0 = 0; s0 < a.nsplit; s0 += 32) {
+    float ms = -CUDART_INF_F, ls = 0.f;
+    if (s0 + lane < a.nsplit) {
+      const float2 v = *reinterpret_cast<const float2*>(a.part_ml + ((s0 + lane) * items + item) * 2);
+      ms = v.x;
+      ls = v.y;
+    }
+    const float fs = ms == -CUDART_INF_F ? 0.f : exp2_ftz(ms - m);
+    const int n = min(32, a.nsplit - s0);
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float f = __shfl_sync(0xffffffffu, fs, s), ll = __shfl_sync(0xffffffffu, ls, s);
+      l += f * ll;
+      const float* p = a.part_o + ((s0 + s) * items + item) * D + lane * C;
+      if constexpr (C == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        acc[0] += f * v.x;
+        acc[1] += f * v.y;
+        acc[2] += f * v.z;
+        acc[3] += f * v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(p);
+        acc[0] += f * v.x;
+        acc[1] += f * v.y;
+      }
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
+  T* out = static_cast<T*>(a.out) + t * a.o_t + h * a.o_h + lane * C;
+#pragma unroll
+  for (int i = 0; i < C; ++i) out[i] = from_f32<T>(acc[i] * inv);
+}
+
+// ======================================================================== host
+struct Plan {
+  int nsplit;
+};
+
+// How many parts the keys of a (sequence, kv head) are cut into.  Up to a CTA per half an SM a part
+// may be as short as 128 keys (one block of each warp): there latency counts; beyond, parts of 512 keys or more up
+// to four times that many, so that ragged lengths even out.
+static Plan make_plan(int tokens, int q_heads, int kv_heads, int batch, int max_new, int64_t max_length) {
+  const int64_t base = (int64_t)batch * kv_heads;
+  auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+  const int64_t n1 = std::min(up(max_length, 128), up(296, base));
+  const int64_t n2 = std::min(up(max_length, 512), up(1184, base));
+  Plan p;
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(128, std::max(n1, n2)));
+  return p;
+}
+
+static size_t plan_bytes(const Plan& p, int tokens, int q_heads, int head_dim) {
+  return p.nsplit > 1 ? (size_t)p.nsplit * tokens * q_heads * (head_dim + 2) * 4 : 0;
+}
+
+template <typename T, int D>
+static int launch(AttendArgs& a, const Plan& p, cudaStream_t st) {
+  auto fn = attend_thin_kernel<T, D>;
+  PPMOE_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, ThinSmem<D>::kBytes));
+  const int64_t ctas = (int64_t)a.nsplit * a.pages.kv_heads * a.seqs.batch;
+  fn<<<(unsigned)ctas, kThinWarps * 32, ThinSmem<D>::kBytes, st>>>(a);
   PPMOE_CHECK_CUDA(cudaGetLastError());
+  if (a.nsplit > 1) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(((int64_t)a.tokens * a.q_heads + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    PPMOE_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D>, a));
+  }
   return PPMOE_OK;
 }
 
@@ -75,9 +544,17 @@ static int launch(const AttendArgs& a, cudaStream_t st) {
 
 using namespace ppmoe;
 
+// What both entry points make of their hints: max_new and max_length held to what can be.
+static Plan plan_of(int tokens, int q_heads, int kv_heads, int batch, int max_new, int64_t max_length) {
+  max_new = max_new < 1 ? 1 : max_new > tokens ? tokens : max_new;
+  max_length = max_length < 1 ? 1 : max_length > INT32_MAX ? INT32_MAX : max_length;
+  return make_plan(tokens, q_heads, kv_heads, batch, max_new, max_length);
+}
+
 extern "C" size_t ppmoe_attend_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim, int batch,
                                                int max_new, int64_t max_length) {
-  return 0;
+  if (tokens < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || batch < 1) return 0;
+  return plan_bytes(plan_of(tokens, q_heads, kv_heads, batch, max_new, max_length), tokens, q_heads, head_dim);
 }
 
 extern "C" int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads, int tokens, const void* k_pages,
@@ -108,6 +585,16 @@ extern "C" int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads
     set_error("ppmoe_attend: null pointer");
     return PPMOE_ERR_INVALID_ARG;
   }
+  if (!std::isfinite(scale)) {
+    set_error("ppmoe_attend: scale is not finite");
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  const Plan p = plan_of(tokens, q_heads, kv_heads, batch, max_new, max_length);
+  const size_t need = plan_bytes(p, tokens, q_heads, head_dim);
+  if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)) {
+    set_error("ppmoe_attend: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, ws ? ws_bytes : 0);
+    return PPMOE_ERR_WORKSPACE;
+  }
   while ((1 << a.pages.page_shift) < page_size) ++a.pages.page_shift;
   a.q = q;
   a.q_t = q_t;
@@ -118,10 +605,19 @@ extern "C" int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads
   a.tokens = tokens;
   a.q_heads = q_heads;
   a.group = q_heads / kv_heads;
-  a.scale = scale;
+  a.c = scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f;
+  a.q_sign = scale > 0.f ? 1 : scale < 0.f ? -1 : 0;
+  auto on = [](const void* x, int64_t s1, int64_t s2, int n) {
+    return reinterpret_cast<uintptr_t>(x) % (2 * n) == 0 && s1 % n == 0 && s2 % n == 0;
+  };
+  a.q_wide = on(q, q_t, q_h, 2);
+  a.o_wide = on(out, o_t, o_h, 8);
+  a.nsplit = p.nsplit;
+  a.part_o = static_cast<float*>(ws);
+  a.part_ml = a.part_o + (size_t)p.nsplit * tokens * q_heads * head_dim;
   a.status = static_cast<uint32_t*>(status);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == PPMOE_BF16)
-    return head_dim == 128 ? launch<__nv_bfloat16, 128>(a, st) : launch<__nv_bfloat16, 64>(a, st);
-  return head_dim == 128 ? launch<__half, 128>(a, st) : launch<__half, 64>(a, st);
+    return head_dim == 128 ? launch<__nv_bfloat16, 128>(a, p, st) : launch<__nv_bfloat16, 64>(a, p, st);
+  return head_dim == 128 ? launch<__half, 128>(a, p, st) : launch<__half, 64>(a, p, st);
 }

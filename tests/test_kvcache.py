@@ -244,6 +244,30 @@ def test_attend_wide_ranges(cuda, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,page", [(torch.bfloat16, 128, 16), (torch.float16, 64, 128)])
+@pytest.mark.parametrize("new,hint", [(5, 5), (40, 40), (40, 1), (150, 150)])
+def test_values_that_are_not_finite(cuda, dtype, dim, page, new, hint):
+    """inf and NaN among the newest values and keys reach the rows that see them and no others."""
+    b = Batch([new, new], [new + 230, new], 2, dim, page, dtype, cuda, seed=13)
+    for s in (0, 1):
+        n = b.lengths[s]
+        k, v = b.keys[s], b.values[s]
+        v[n - 1, 0, 3] = math.nan
+        v[n - 1, 1, dim - 1] = math.inf
+        v[n - 2, 1, 0], v[n - 2, 1, 1] = -math.inf, math.inf
+        v[n - new // 2, 0, 5] = math.inf
+        v[n - new // 2 + 1, 0, 5] = -math.inf
+        k[n - 1, 1, 7] = math.nan  # the last row's scores
+        pos = torch.arange(n, device=cuda)
+        at = b.table[s][pos // page].long(), slice(None), pos % page
+        b.k[at], b.v[at] = k, v
+    q = b.normal(4, 2.0)
+    out, size = exact_attention(b, q)
+    assert out.isfinite().any() and not out.isfinite().all()
+    assert_attention(b.cache().attend(q, b.starts, b.lens, b.table, max_new=hint), out, size)
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits(cuda):
     """A cache of more than 2^31 values whose used pages lie at its end."""
     pages, page, hk = 140_000, 256, 1
