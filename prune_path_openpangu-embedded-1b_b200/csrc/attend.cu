@@ -12,75 +12,9 @@
 // A masked key must not reach a row even where its value is not finite (0 * inf = NaN): tiles that
 // some row sees in part are searched for such values.  They are taken out of the product, and
 // added (they are what the sum becomes) to the rows that see their key.
-#include <math_constants.h>
-#include <algorithm>
-#include <cmath>
-#include <type_traits>
-#include "seqs.cuh"
-#include "umma.cuh"
+#include "attend.cuh"
 
 namespace ppmoe {
-
-struct AttendArgs {
-  const void* q;
-  int64_t q_t, q_h;
-  void* out;
-  int64_t o_t, o_h;
-  int tokens, q_heads, group;
-  float c;         // |scale| log2 e (1 where scale is 0)
-  int q_sign;      // -1, 0, 1: what q is multiplied by
-  int q_wide;      // rows of q start on 4-byte (thin kernel) / 16-byte boundaries
-  int o_wide;      // rows of out start on 16-byte boundaries
-  int nsplit;      // parts of the keys; above 1 they meet in ws
-  float* part_o;   // [nsplit][tokens][q_heads][D]: sum of 2^(x - m) v
-  float* part_ml;  // [nsplit][tokens][q_heads][2]: m, l
-  Seqs seqs;
-  Pages pages;
-  uint32_t* status;
-};
-
-__device__ __forceinline__ float exp2_ftz(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Sequence b as the kernels see it: its first packed row, its new rows, its length held to what the
-// table can name (reported), and to what `tokens` rows can hold.
-struct Seq {
-  int first, rows, length;
-};
-__device__ __forceinline__ Seq load_seq(const AttendArgs& a, int b) {
-  Seq s;
-  s.first = a.seqs.starts[b];
-  int end = a.seqs.starts[b + 1];
-  s.length = a.seqs.lengths[b];
-  if (s.first < 0) s.first = 0;
-  if (end > a.tokens) end = a.tokens;
-  s.rows = end - s.first;
-  return s;
-}
-// Position of the sequence's first new row; keys a row at position pos may see.
-__device__ __forceinline__ int key_cap(const AttendArgs& a, int length) {
-  const int64_t cap = (int64_t)a.seqs.max_pages << a.pages.page_shift;
-  return length < cap ? length : (int)cap;
-}
-
-
-// C rounded values of one row piece, scaled by inv.
-template <typename T, int C>
-__device__ __forceinline__ void store_row(T* out, const float (&v)[C], float inv, bool wide) {
-  if (wide) {
-#pragma unroll
-    for (int i = 0; i < C; i += 8)
-      *reinterpret_cast<uint4*>(out + i) =
-          make_uint4(pack2<T>(v[i] * inv, v[i + 1] * inv), pack2<T>(v[i + 2] * inv, v[i + 3] * inv),
-                     pack2<T>(v[i + 4] * inv, v[i + 5] * inv), pack2<T>(v[i + 6] * inv, v[i + 7] * inv));
-  } else {
-#pragma unroll
-    for (int i = 0; i < C; ++i) out[i] = from_f32<T>(v[i] * inv);
-  }
-}
 
 // ======================================================================== few rows
 // Up to 16 rows at a time per (sequence, kv head): one token per sequence up to a few.  Bound by
@@ -124,29 +58,6 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)
 // 16 bytes global -> shared, or 16 zero bytes (the source is then not read).
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-
-// What q is multiplied by (-1, 0 or 1), on a packed pair.
-__device__ __forceinline__ uint32_t q_pair(uint32_t v, int sign) {
-  return sign > 0 ? v : sign < 0 ? v ^ 0x80008000u : 0u;
-}
-
-// Fp16 weights below 2^-24 would vanish; lifting every weight by 2^8 (it cancels against l) keeps
-// those down to 2^-32 of the largest.  bf16 has fp32's exponents and needs none.
-template <typename T>
-constexpr float kLift = 0.f;
-template <>
-constexpr float kLift<__half> = 8.f;
-
-// Exponent field all ones: inf or NaN.
-template <typename T>
-__device__ __forceinline__ bool not_finite16(uint32_t v) {  // v: the 16 bits
-  constexpr uint32_t m = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return (v & m) == m;
-}
-template <typename T>
-__device__ __forceinline__ bool not_finite2(uint32_t v) {
-  return not_finite16<T>(v) || not_finite16<T>(v >> 16);
 }
 
 template <typename T, int D>
@@ -342,7 +253,7 @@ __global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const _
         for (int i = lane; i < kThinKeys * D / 2; i += 32) {
           uint32_t v;
           asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(vd + i * 4) : "memory");
-          bad |= not_finite2<T>(v);
+          bad |= not_finite2<T>(v) != 0;
         }
         if (__any_sync(0xffffffffu, bad)) {
           for (int j = 0; j < kThinKeys; ++j) {
@@ -498,19 +409,28 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant_
 
 // ======================================================================== host
 struct Plan {
-  int nsplit;
+  int tiles;   // 0: the kernel for few rows; else pairs of 128-row tiles of the longest sequence
+  int nsplit;  // parts the keys of a (sequence, kv head) are cut into
 };
 
-// How many parts the keys of a (sequence, kv head) are cut into.  Up to a CTA per half an SM a part
-// may be as short as 128 keys (one block of each warp): there latency counts; beyond, parts of 512 keys or more up
-// to four times that many, so that ragged lengths even out.
-static Plan make_plan(int tokens, int q_heads, int kv_heads, int batch, int max_new, int64_t max_length) {
-  const int64_t base = (int64_t)batch * kv_heads;
+static Plan make_plan(int q_heads, int kv_heads, int batch, int max_new, int64_t max_length) {
   auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-  const int64_t n1 = std::min(up(max_length, 128), up(296, base));
-  const int64_t n2 = std::min(up(max_length, 512), up(1184, base));
+  const int64_t rows = (int64_t)max_new * (q_heads / kv_heads), base = (int64_t)batch * kv_heads;
   Plan p;
-  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(128, std::max(n1, n2)));
+  if (rows <= 16) {
+    // Up to two CTAs an SM a part may be as short as 128 keys (one block of each warp): there latency
+    // counts; beyond, parts of 512 keys or more, up to 1184 CTAs, so that ragged lengths even out.
+    p.tiles = 0;
+    const int64_t n1 = std::min(up(max_length, 128), up(296, base));
+    const int64_t n2 = std::min(up(max_length, 512), up(1184, base));
+    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(128, std::max(n1, n2)));
+  } else {
+    // One CTA an SM: parts only while they fit in one wave of 148, of 512 keys or more.
+    // (A CTA goes on to further pairs where there are fewer CTAs than pairs: batches so wide that most
+    // of a larger grid would find nothing to do.)
+    p.tiles = (int)std::min(up(rows, 256), std::max<int64_t>(1, (1 << 18) / base));
+    p.nsplit = (int)std::max<int64_t>(1, std::min(max_length / 512, 148 / (base * p.tiles)));
+  }
   return p;
 }
 
@@ -520,11 +440,15 @@ static size_t plan_bytes(const Plan& p, int tokens, int q_heads, int head_dim) {
 
 template <typename T, int D>
 static int launch(AttendArgs& a, const Plan& p, cudaStream_t st) {
-  auto fn = attend_thin_kernel<T, D>;
-  PPMOE_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, ThinSmem<D>::kBytes));
-  const int64_t ctas = (int64_t)a.nsplit * a.pages.kv_heads * a.seqs.batch;
-  fn<<<(unsigned)ctas, kThinWarps * 32, ThinSmem<D>::kBytes, st>>>(a);
-  PPMOE_CHECK_CUDA(cudaGetLastError());
+  if (p.tiles) {
+    if (int rc = attend_tiles_launch(a, D, 1 << a.pages.page_shift, std::is_same<T, __half>::value, p.tiles, st)) return rc;
+  } else {
+    auto fn = attend_thin_kernel<T, D>;
+    PPMOE_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, ThinSmem<D>::kBytes));
+    const int64_t ctas = (int64_t)a.nsplit * a.pages.kv_heads * a.seqs.batch;
+    fn<<<(unsigned)ctas, kThinWarps * 32, ThinSmem<D>::kBytes, st>>>(a);
+    PPMOE_CHECK_CUDA(cudaGetLastError());
+  }
   if (a.nsplit > 1) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(((int64_t)a.tokens * a.q_heads + 3) / 4));
@@ -548,12 +472,12 @@ using namespace ppmoe;
 static Plan plan_of(int tokens, int q_heads, int kv_heads, int batch, int max_new, int64_t max_length) {
   max_new = max_new < 1 ? 1 : max_new > tokens ? tokens : max_new;
   max_length = max_length < 1 ? 1 : max_length > INT32_MAX ? INT32_MAX : max_length;
-  return make_plan(tokens, q_heads, kv_heads, batch, max_new, max_length);
+  return make_plan(q_heads, kv_heads, batch, max_new, max_length);
 }
 
 extern "C" size_t ppmoe_attend_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim, int batch,
                                                int max_new, int64_t max_length) {
-  if (tokens < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || batch < 1) return 0;
+  if (tokens < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || batch < 1) return 0;
   return plan_bytes(plan_of(tokens, q_heads, kv_heads, batch, max_new, max_length), tokens, q_heads, head_dim);
 }
 
@@ -581,6 +505,11 @@ extern "C" int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads
     return PPMOE_ERR_INVALID_ARG;
   }
   if (tokens == 0) return PPMOE_OK;
+  if ((int64_t)batch * kv_heads > (1 << 20) || (int64_t)tokens * q_heads > INT32_MAX) {
+    set_error("ppmoe_attend: batch * kv_heads = %lld (at most 2^20) or tokens * q_heads = %lld (below 2^31)",
+              (long long)batch * kv_heads, (long long)tokens * q_heads);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
   if (!q || !out || !status) {
     set_error("ppmoe_attend: null pointer");
     return PPMOE_ERR_INVALID_ARG;
@@ -611,6 +540,7 @@ extern "C" int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads
     return reinterpret_cast<uintptr_t>(x) % (2 * n) == 0 && s1 % n == 0 && s2 % n == 0;
   };
   a.q_wide = on(q, q_t, q_h, 2);
+  a.q_wide16 = on(q, q_t, q_h, 8);
   a.o_wide = on(out, o_t, o_h, 8);
   a.nsplit = p.nsplit;
   a.part_o = static_cast<float*>(ws);
