@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant_
 
 // ======================================================================== host
 struct Plan {
-  int tiles;   // 0: the kernel for few rows; else pairs of 128-row tiles of the longest sequence
+  int tiles;   // 0: the kernel for few rows; else 128-row tiles of a CTA (1 or 2)
+  int groups;  // CTAs' worth of row tiles of the longest sequence
   int nsplit;  // parts the keys of a (sequence, kv head) are cut into
 };
 
@@ -420,16 +421,18 @@ static Plan make_plan(int q_heads, int kv_heads, int batch, int max_new, int64_t
   if (rows <= 16) {
     // Up to two CTAs an SM a part may be as short as 128 keys (one block of each warp): there latency
     // counts; beyond, parts of 512 keys or more, up to 1184 CTAs, so that ragged lengths even out.
-    p.tiles = 0;
+    p.tiles = p.groups = 0;
     const int64_t n1 = std::min(up(max_length, 128), up(296, base));
     const int64_t n2 = std::min(up(max_length, 512), up(1184, base));
     p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(128, std::max(n1, n2)));
   } else {
-    // One CTA an SM: parts only while they fit in one wave of 148, of 512 keys or more.
-    // (A CTA goes on to further pairs where there are fewer CTAs than pairs: batches so wide that most
+    // (A CTA goes on to further groups where there are fewer CTAs than groups: batches so wide that most
     // of a larger grid would find nothing to do.)
-    p.tiles = (int)std::min(up(rows, 256), std::max<int64_t>(1, (1 << 18) / base));
-    p.nsplit = (int)std::max<int64_t>(1, std::min(max_length / 512, 148 / (base * p.tiles)));
+    p.tiles = rows <= 128 ? 1 : 2;
+    p.groups = (int)std::min(up(rows, 128 * p.tiles), std::max<int64_t>(1, (1 << 18) / base));
+    // parts only while they fit in one wave, of 512 keys or more
+    const int64_t slots = p.tiles == 2 ? 148 : 296;
+    p.nsplit = (int)std::max<int64_t>(1, std::min(max_length / 512, slots / (base * p.groups)));
   }
   return p;
 }
@@ -441,7 +444,7 @@ static size_t plan_bytes(const Plan& p, int tokens, int q_heads, int head_dim) {
 template <typename T, int D>
 static int launch(AttendArgs& a, const Plan& p, cudaStream_t st) {
   if (p.tiles) {
-    if (int rc = attend_tiles_launch(a, D, 1 << a.pages.page_shift, std::is_same<T, __half>::value, p.tiles, st)) return rc;
+    if (int rc = attend_tiles_launch(a, D, 1 << a.pages.page_shift, std::is_same<T, __half>::value, p.tiles, p.groups, st)) return rc;
   } else {
     auto fn = attend_thin_kernel<T, D>;
     PPMOE_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, ThinSmem<D>::kBytes));

@@ -98,6 +98,6 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t v) {  // bits 15 and 31
   return ((v & m) + one) & 0x80008000u;
 }
 
-int attend_tiles_launch(AttendArgs& a, int head_dim, int page_size, bool half, int pairs, cudaStream_t st);
+int attend_tiles_launch(AttendArgs& a, int head_dim, int page_size, bool half, int tiles, int groups, cudaStream_t st);
 
 }  // namespace ppmoe

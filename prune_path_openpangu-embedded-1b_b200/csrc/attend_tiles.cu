@@ -19,18 +19,22 @@
 namespace ppmoe {
 
 constexpr int kTileRows = 128;
-constexpr int kTileKeys = 128;
-constexpr int kTilesThreads = 384;  // 8 softmax warps, products, loads, 2 guards
 
-template <int D>
-struct TilesSmem {
-  static constexpr int kQ = kTileRows * D * 2;     // one q tile: [D / 64][128 rows][128 bytes]
-  static constexpr int kStage = kTileKeys * D * 2; // a K or V tile, the same way
-  static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr int kBars = 2 * kQ + kStages * kStage;
-  static constexpr int kNumBars = 4 * kStages + 6;
+// Shape of a CTA: TILES row tiles, KEYS keys at a time, of D values.
+template <int D, int TILES, int KEYS>
+struct TilesShape {
+  static constexpr int kSoftmaxWarps = 4 * TILES;
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 4);  // and products, loads, 2 guards
+  static constexpr int kCtas = TILES == 2 ? 1 : 2;           // per SM
+  static constexpr int kQ = kTileRows * D * 2;  // one q tile: [D / 64][128 rows][128 bytes]
+  static constexpr int kStage = KEYS * D * 2;   // a K or V tile, the same way
+  static constexpr int kStages = D == 128 ? (TILES == 2 ? 5 : 4) : (TILES == 2 ? 8 : 10);
+  static constexpr int kBars = TILES * kQ + kStages * kStage;
+  static constexpr int kNumBars = 4 * kStages + 8;
   static constexpr int kList = kBars + ((kNumBars * 8 + 16 + 15) / 16) * 16;  // [3][D] ints
   static constexpr int kBytes = kList + 3 * D * 4 + 1024;
+  static constexpr int kTmem = TILES * (KEYS + D) > 256 ? 512 : 256;  // columns: S tiles, then O tiles
+  static constexpr int kEarly = KEYS / 4 * 3;  // keys whose weights are handed on first
 };
 
 // Bounded wait that records a timeout; any earlier timeout ends it soon.
@@ -52,6 +56,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
 }
 
+// One lane of a converged warp.  The compiler knows that a single lane runs what follows; under
+// `lane == 0` every product cost its warp about 100 cycles to issue (1.33 -> 1.08 ms for 2048 rows over
+// 32768 keys, 32 heads).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+
 // D (TMEM) += A (TMEM, 16-bit pairs) * B (shared memory).
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -63,10 +76,11 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, 
 // Descriptor of a V tile as the B operand with its columns contiguous ("MN-major"), 128-byte
 // swizzle: 64 columns x 8 keys are 1024 bytes; 8 keys further on: 1024 bytes; 64 columns further
 // on: a half tile.
+template <int KEYS>
 __device__ __forceinline__ uint64_t desc_v(uint32_t saddr) {
   uint64_t d = 0;
   d |= (uint64_t)((saddr >> 4) & 0x3FFF);
-  d |= (uint64_t)((kTileKeys * 128) >> 4) << 16;
+  d |= (uint64_t)((KEYS * 128) >> 4) << 16;
   d |= (uint64_t)(1024 >> 4) << 32;
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
@@ -81,88 +95,155 @@ constexpr uint32_t idesc_of(int n, bool b_mn) {
          ((uint32_t)(kTileRows >> 4) << 24);
 }
 
+// 32 columns of this thread's TMEM lane; the values are there after tmem_ld_wait, and only what
+// passed tmem_ld_bind after it is safe from being used before it.
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float* v) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld_bind(float* v) {
+  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+               "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+  asm volatile("" : "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+               "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+               "+f"(v[31]));
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
-// What every warp of a CTA derives alike for one pair of tiles.
-struct Pair {
-  int r0, tiles;      // first row, tiles with rows (1 or 2)
-  int b0, count[2];   // first block of keys, blocks of each tile
-  int keys;           // keys some row sees
-  int clear;          // keys every row sees: blocks within need no guard
-  __device__ Pair(const AttendArgs& a, int pair, int rows, int pos0, int cap, int split) {
-    r0 = pair * 2 * kTileRows;
-    tiles = r0 + kTileRows < rows ? 2 : 1;
-    int n[2] = {0, 0};
+// Pairs of fp32 in one 64-bit register.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void untwo(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Largest of three, NaN where one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x for pairs of x <= 2^8 on the FMA pipe: x = n + f with n the nearest integer (its bits fall out of adding
+// 1.5 * 2^23) and |f| <= 1/2, a polynomial for 2^f (minimax in relative error, Remez exchange: degree 3
+// 7.5e-5, 3% of bf16's half step; degree 4 2.7e-6, 1% of fp16's half step), n added to its exponent.
+// Below 2^-126: about 2^-126, and so only where no weight may be exactly zero.
+template <typename T>
+__device__ __forceinline__ void exp2_pair(float x0, float x1, float& e0, float& e1) {
+  x0 = fmaxf(x0, -126.f);
+  x1 = fmaxf(x1, -126.f);
+  const uint64_t x = two(x0, x1);
+  const uint64_t t = add2(x, two(12582912.f, 12582912.f));
+  const uint64_t n = add2(t, two(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, two(-1.f, -1.f), x);
+  uint64_t p;
+  if constexpr (std::is_same<T, __half>::value) {
+    p = fma2(f, two(0.009570102207362652f, 0.009570102207362652f), two(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, two(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, two(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, two(0.9999992847442627f, 0.9999992847442627f));
+  } else {
+    p = fma2(f, two(0.0551716685295105f, 0.0551716685295105f), two(0.2426111251115799f, 0.2426111251115799f));
+    p = fma2(p, f, two(0.6932609677314758f, 0.6932609677314758f));
+    p = fma2(p, f, two(0.9999280571937561f, 0.9999280571937561f));
+  }
+  float t0, t1, p0, p1;
+  untwo(t, t0, t1);
+  untwo(p, p0, p1);
+  e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
+// What every warp of a CTA derives alike for one group of TILES row tiles.
+template <int TILES, int KEYS>
+struct Group {
+  int r0, tiles;         // first row, tiles with rows
+  int b0, count[TILES];  // first block of keys, blocks of each tile
+  int keys;              // keys some row sees
+  int clear;             // keys every row sees: blocks within need no guard
+  __device__ Group(const AttendArgs& a, int64_t group, int rows, int pos0, int cap, int split) {
+    r0 = (int)group * TILES * kTileRows;
+    tiles = TILES == 2 && r0 + kTileRows < rows ? 2 : 1;
+    int n[TILES];
     keys = 0;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < TILES; ++t) {
+      n[t] = 0;
       if (t >= tiles) continue;
       const int last = min(r0 + (t + 1) * kTileRows, rows) - 1;
       keys = max(0, min(pos0 + last / a.group + 1, cap));
-      n[t] = (keys + kTileKeys - 1) / kTileKeys;
+      n[t] = (keys + KEYS - 1) / KEYS;
     }
-    const int most = max(n[0], n[1]), per = (most + a.nsplit - 1) / a.nsplit;
+    const int most = n[tiles - 1], per = (most + a.nsplit - 1) / a.nsplit;
     b0 = split * per;
     const int b1 = min(most, b0 + per);
-    count[0] = max(0, min(b1, n[0]) - b0);
-    count[1] = max(0, min(b1, n[1]) - b0);
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) count[t] = max(0, min(b1, n[t]) - b0);
     clear = min(pos0 + r0 / a.group + 1, cap);
   }
-  __device__ int blocks() const { return max(count[0], count[1]); }
-  __device__ bool guarded(int block) const { return (block + 1) * kTileKeys > clear; }
+  __device__ int blocks() const { return TILES == 2 ? max(count[0], count[TILES - 1]) : count[0]; }
+  __device__ bool guarded(int block) const { return (block + 1) * KEYS > clear; }
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kTilesThreads, 1)
+template <typename T, int D, int TILES, int KEYS>
+__global__ void __launch_bounds__(TilesShape<D, TILES, KEYS>::kThreads, TilesShape<D, TILES, KEYS>::kCtas)
 attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                    const __grid_constant__ AttendArgs a, int box_rows, int pairs_hint) {
+                    const __grid_constant__ AttendArgs a, int box_rows, int groups_hint) {
   extern __shared__ uint8_t smem_raw[];
-  using S = TilesSmem<D>;
-  constexpr int NS = S::kStages;
+  using S = TilesShape<D, TILES, KEYS>;
+  constexpr int NS = S::kStages, SW = S::kSoftmaxWarps;
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   // A V tile that needs a guard arrives at g_full, is handed on at v_ok, and leaves kv_full alone: whoever waits
   // for a barrier waits for every phase of it.
   uint64_t *kv_full = bars, *kv_empty = bars + NS, *g_full = bars + 2 * NS, *v_ok = bars + 3 * NS;
-  uint64_t *s_full = bars + 4 * NS, *p_ready = s_full + 2, *q_full = s_full + 4;
+  uint64_t *s_full = bars + 4 * NS, *p_early = s_full + 2, *p_late = s_full + 4, *q_full = s_full + 6;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::kNumBars);
   int* any_odd = reinterpret_cast<int*>(tmem_slot + 1);
   int* odd = reinterpret_cast<int*>(smem + S::kList);  // [nan, +inf, -inf][D]: first key with one in that column
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
-  // blocks of work, the rows with most keys first: pair (slowest, descending), sequence, kv head, part
+  // blocks of work, the rows with most keys first: group (slowest, descending), sequence, kv head, part
   int x = blockIdx.x;
   const int split = x % a.nsplit;
   x /= a.nsplit;
   const int kvh = x % a.pages.kv_heads;
   x /= a.pages.kv_heads;
   const int b = x % a.seqs.batch;
-  const int pair_of = pairs_hint - 1 - x / a.seqs.batch;
+  const int group_of = groups_hint - 1 - x / a.seqs.batch;
   const Seq sq = load_seq(a, b);
   const int rows = sq.rows > 0 ? sq.rows * a.group : 0;
-  if ((int64_t)pair_of * (2 * kTileRows) >= rows) return;
+  constexpr int kRows = TILES * kTileRows;
+  if ((int64_t)group_of * kRows >= rows) return;
   const int cap = key_cap(a, sq.length);
   if (cap < sq.length && tid == 0) atomicOr(a.status, DEVERR_PAGE);
   const int pos0 = sq.length - (a.seqs.starts[b + 1] - a.seqs.starts[b]);
@@ -176,130 +257,167 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full + t, 1);
-      mbar_init(p_ready + t, kTileRows);
+      mbar_init(p_early + t, kTileRows);
+      mbar_init(p_late + t, kTileRows);
       mbar_init(q_full + t, kTileRows);
     }
     *any_odd = 0;
     fence_mbar_init();
   }
-  for (int i = tid; i < 3 * D; i += kTilesThreads) odd[i] = INT_MAX;
-  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  for (int i = tid; i < 3 * D; i += S::kThreads) odd[i] = INT_MAX;
+  if (warp == SW) tmem_alloc(tmem_slot, S::kTmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t ring = smem_u32(smem) + 2 * S::kQ;
+  const uint32_t ring = smem_u32(smem) + TILES * S::kQ;
 
-  // running counts, alike in every role: ring uses, barrier phases
-  int loads = 0;            // K and V tiles so far
-  uint32_t ph_s[2] = {0, 0}, ph_p[2] = {0, 0}, ph_q[2] = {0, 0};
-  uint32_t ph_full = 0, ph_v = 0;  // a bit a stage: kv_full; g_full (guards) or v_ok (products)
+  // Between two groups of one CTA: everything of the first is over.
+  auto next_group = [&](int64_t group) {
+    tc_fence_before();
+    __syncthreads();
+    if ((group + groups_hint) * kRows < rows) {
+      for (int i = tid; i < 3 * D; i += S::kThreads) odd[i] = INT_MAX;
+      if (tid == 0) *any_odd = 0;
+      __syncthreads();
+    }
+    tc_fence_after();
+  };
 
+  if (warp < SW) {
+    // -------------------------------------------------------------- softmax, tile t, one row a thread
+    if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
+    const uint32_t t_s = tmem + t * KEYS + lanes, t_o = tmem + TILES * KEYS + t * D + lanes;
+    const float c = a.c;
+    uint32_t ph_s = 0;
 #pragma unroll 1
-  for (int64_t pair = pair_of; pair * (2 * kTileRows) < rows; pair += pairs_hint) {
-    const Pair w(a, (int)pair, rows, pos0, cap, split);
-    const int blocks = w.blocks();
-    if (warp < 8) {
-      // ------------------------------------------------------------ softmax, tile t, one row a thread
-      const int t = warp >> 2, row = tid & 127;
+    for (int64_t group = group_of; group * kRows < rows; group += groups_hint) {
+      const Group<TILES, KEYS> w(a, group, rows, pos0, cap, split);
       if (t < w.tiles) {
-        const int r = w.r0 + t * kTileRows + row;
-        {
-          const int base = w.r0 + t * kTileRows;
-          constexpr int CH = D / 8;
+        const int base = w.r0 + t * kTileRows, r = base + row;
+        constexpr int CH = D / 8;
 #pragma unroll 4
-          for (int i = row; i < kTileRows * CH; i += kTileRows) {
-            const int rr = i / CH, c = i % CH, q_row = base + rr;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (q_row < rows) {
-              const int tok = q_row / a.group;
-              const T* p = static_cast<const T*>(a.q) + (int64_t)(sq.first + tok) * a.q_t +
-                           (int64_t)(kvh * a.group + q_row - tok * a.group) * a.q_h + c * 8;
-              if (a.q_wide16) {
-                v = __ldg(reinterpret_cast<const uint4*>(p));
-              } else {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-                v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
-                               h[6] | (uint32_t)h[7] << 16);
-              }
-              v = make_uint4(q_pair(v.x, a.q_sign), q_pair(v.y, a.q_sign), q_pair(v.z, a.q_sign), q_pair(v.w, a.q_sign));
+        for (int i = row; i < kTileRows * CH; i += kTileRows) {
+          const int rr = i / CH, ch = i % CH, q_row = base + rr;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (q_row < rows) {
+            const int tok = q_row / a.group;
+            const T* p = static_cast<const T*>(a.q) + (int64_t)(sq.first + tok) * a.q_t +
+                         (int64_t)(kvh * a.group + q_row - tok * a.group) * a.q_h + ch * 8;
+            if (a.q_wide16) {
+              v = __ldg(reinterpret_cast<const uint4*>(p));
+            } else {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+              v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                             h[6] | (uint32_t)h[7] << 16);
             }
-            *reinterpret_cast<uint4*>(smem + t * S::kQ + (c >> 3) * (kTileRows * 128) + sw128_offset(rr, c & 7)) = v;
+            v = make_uint4(q_pair(v.x, a.q_sign), q_pair(v.y, a.q_sign), q_pair(v.z, a.q_sign), q_pair(v.w, a.q_sign));
           }
-          fence_proxy_async();
-          mbar_arrive(q_full + t);
+          *reinterpret_cast<uint4*>(smem + t * S::kQ + (ch >> 3) * (kTileRows * 128) + sw128_offset(rr, ch & 7)) = v;
         }
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
-        const uint32_t t_s = tmem + t * kTileKeys + lanes, t_o = tmem + 2 * kTileKeys + t * D + lanes;
+        fence_proxy_async();
+        mbar_arrive(q_full + t);
         const int tok = r / a.group;
-        const int lim = r < rows ? min(pos0 + tok, cap - 1) : -1;
-        const int all_see = min(pos0 + (w.r0 + t * kTileRows) / a.group, cap - 1);  // last key the first row sees
-        const float c = a.c;
-        float m = -CUDART_INF_F, l = 0.f;
+        const int lim = r < rows ? min(pos0 + tok, cap - 1) : -1;      // last key this row sees
+        const int all_see = min(pos0 + base / a.group, cap - 1);       // ... the tile's first row
         const int count = w.count[t];
+        float m = -CUDART_INF_F, l = 0.f;
 #pragma unroll 1
         for (int j = 0; j < count; ++j) {
-          float s[kTileKeys];
-          wait_bar(s_full + t, ph_s[t], a.status);
-          ph_s[t] ^= 1;
+          float s[KEYS];
+          wait_bar(s_full + t, ph_s, a.status);
+          ph_s ^= 1;
           tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < kTileKeys; i += 32) tmem_ld32_async(t_s + i, s + i);
+          for (int i = 0; i < KEYS; i += 32) tmem_ld32_async(t_s + i, s + i);
           tmem_ld_wait();
-          const int key0 = (w.b0 + j) * kTileKeys;
-          if (key0 + kTileKeys - 1 > all_see) {
+#pragma unroll
+          for (int i = 0; i < KEYS; i += 32) tmem_ld_bind(s + i);
+          const int key0 = (w.b0 + j) * KEYS;
+          const bool masked = key0 + KEYS - 1 > all_see;
+          if (masked) {
             const int n = lim - key0;  // columns 0 .. n are seen
 #pragma unroll
-            for (int i = 0; i < kTileKeys; ++i) s[i] = i <= n ? s[i] : -CUDART_INF_F;
+            for (int i = 0; i < KEYS; ++i) s[i] = i <= n ? s[i] : -CUDART_INF_F;
           }
-          float mx = s[0], mx2 = s[1];
+          float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int i = 2; i < kTileKeys; i += 2) {
-            mx = fmaxf(mx, s[i]);
-            mx2 = fmaxf(mx2, s[i + 1]);
+          for (int i = 4; i < KEYS; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = i + 4 < KEYS ? max3(mx[e], s[i + e], s[i + 4 + e]) : max3(mx[e], s[i + e], s[i + e]);
           }
-          mx = fmaxf(mx, mx2);
-          const bool move = (mx - m) * c > 8.f;  // false where both are -inf
+          mx[0] = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
+          // false where both are -inf; a NaN takes the row for good
+          const bool move = (mx[0] - m) * c > 8.f || mx[0] != mx[0];
           if (__any_sync(0xffffffffu, move)) {
             if (j > 0) {
-              const float f = move ? exp2_ftz((m - mx) * c) : 1.f;
+              const float f = move ? exp2_ftz((m - mx[0]) * c) : 1.f;
               l *= f;
 #pragma unroll 1
-              for (int i = 0; i < D; i += 32) {
-                float o[32];
-                tmem_ld32_async(t_o + i, o);
-                tmem_ld_wait();
+              for (int i = 0; i < D; i += 16) {
+                uint32_t o[16];
+                asm volatile(
+                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                    "tcgen05.wait::ld.sync.aligned;"
+                    : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
+                      "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+                    : "r"(t_o + i) : "memory");
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= f;
-                tmem_st32(t_o + i, reinterpret_cast<uint32_t*>(o));
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st16(t_o + i, o);
               }
               tmem_st_wait();
             }
-            if (move) m = mx;
+            if (move) m = mx[0];
           }
           const float sub = (m == -CUDART_INF_F ? 0.f : m * c) - kLift<T>;
-          float sum[2] = {0.f, 0.f};
+          const uint64_t c2 = two(c, c), sub2 = two(-sub, -sub);
+          uint64_t sum[2] = {0, 0};
+          // weights, in eights of pairs: the first three quarters are handed on while the last is computed
+          auto weights = [&](auto some, int from, int to) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t p[32];
+            for (int g = from; g < to; g += 16) {
+              uint32_t p[8];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float e0 = exp2_ftz(fmaf(s[h * 64 + 2 * i], c, -sub)), e1 = exp2_ftz(fmaf(s[h * 64 + 2 * i + 1], c, -sub));
-              sum[0] += e0;
-              sum[1] += e1;
-              p[i] = pack2<T>(e0, e1);
+              for (int i = 0; i < 8; ++i) {
+                float x0, x1, e0, e1;
+                untwo(fma2(two(s[g + 2 * i], s[g + 2 * i + 1]), c2, sub2), x0, x1);
+                if (decltype(some)::value && (i & 3) == 3) {
+                  exp2_pair<T>(x0, x1, e0, e1);
+                } else {
+                  e0 = exp2_ftz(x0);
+                  e1 = exp2_ftz(x1);
+                }
+                sum[i & 1] = add2(sum[i & 1], two(e0, e1));
+                p[i] = pack2<T>(e0, e1);
+              }
+              tmem_st8(t_s + g / 2, p);
             }
-            tmem_st32(t_s + h * 32, p);
-          }
-          l += sum[0] + sum[1];
+          };
+          if (masked)
+            weights(std::false_type{}, 0, S::kEarly);
+          else
+            weights(std::true_type{}, 0, S::kEarly);
           tmem_st_wait();
           tc_fence_before();
-          mbar_arrive(p_ready + t);
+          mbar_arrive(p_early + t);
+          if (masked)
+            weights(std::false_type{}, S::kEarly, KEYS);
+          else
+            weights(std::true_type{}, S::kEarly, KEYS);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(p_late + t);
+          float l0, l1;
+          untwo(add2(sum[0], sum[1]), l0, l1);
+          l += l0 + l1;
         }
         // the sums
         if (count > 0) {
-          wait_bar(s_full + t, ph_s[t], a.status);
-          ph_s[t] ^= 1;
+          wait_bar(s_full + t, ph_s, a.status);
+          ph_s ^= 1;
           tc_fence_after();
         }
         const bool listed = *reinterpret_cast<volatile int*>(any_odd) != 0;
@@ -313,6 +431,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           if (count > 0) {
             tmem_ld32_async(t_o + i, o);
             tmem_ld_wait();
+            tmem_ld_bind(o);
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
@@ -341,173 +460,192 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
         }
         if (a.nsplit > 1 && r < rows) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m * c, l);
-        tc_fence_before();
       }
-    } else if (warp == 8) {
+      next_group(group);
+    }
+  } else {
+    if constexpr (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    int loads = 0;  // K and V tiles so far: use i of the ring is in stage i % NS
+    if (warp == SW) {
       // ------------------------------------------------------------ products
-      constexpr uint32_t id_s = idesc_of<T>(kTileKeys, false), id_o = idesc_of<T>(D, true);
-      auto stage_of = [&](int i) { return ring + (uint32_t)((loads + i) % NS) * S::kStage; };
-      auto wait_tile = [&](int st) {
-        wait_bar(kv_full + st, (ph_full >> st) & 1, a.status);
-        ph_full ^= 1u << st;
-      };
-      auto qk = [&](int t, int j) {
-        if (lane == 0) {
-          const uint32_t qa = smem_u32(smem) + t * S::kQ, kb = stage_of(2 * j);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k >> 2) * (kTileRows * 128) + (k & 3) * 32;
-            umma_bf16(tmem + t * kTileKeys, umma_desc_sw128(qa + off), umma_desc_sw128(kb + off), id_s, k > 0);
-          }
-          umma_commit(s_full + t);
-        }
-      };
-      for (int t = 0; t < w.tiles; ++t) {
-        wait_bar(q_full + t, ph_q[t], a.status);
-        ph_q[t] ^= 1;
-      }
-      if (blocks > 0) {
-        wait_tile(loads % NS);
-        tc_fence_after();
-        for (int t = 0; t < w.tiles; ++t)
-          if (w.count[t] > 0) qk(t, 0);
-        if (lane == 0) umma_commit(kv_empty + loads % NS);
-      }
+      constexpr uint32_t id_s = idesc_of<T>(KEYS, false), id_o = idesc_of<T>(D, true);
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(smem)), k_desc = umma_desc_sw128(ring), v_desc = desc_v<KEYS>(ring);
+      uint32_t ph_p[TILES] = {}, ph_q[TILES] = {}, ph_full = 0, ph_v = 0;  // the last two: a bit a stage
 #pragma unroll 1
-      for (int j = 0; j < blocks; ++j) {
-        const int vi = loads + 2 * j + 1, vs = vi % NS;
-        if (w.guarded(w.b0 + j)) {
-          wait_bar(v_ok + vs, (ph_v >> vs) & 1, a.status);
-          ph_v ^= 1u << vs;
-        } else {
-          wait_tile(vs);
-        }
-        if (j + 1 < blocks) wait_tile((vi + 1) % NS);
+      for (int64_t group = group_of; group * kRows < rows; group += groups_hint) {
+        const Group<TILES, KEYS> w(a, group, rows, pos0, cap, split);
+        const int blocks = w.blocks();
+        if (elect_one()) {
+          auto wait_tile = [&](int st) {
+            wait_bar(kv_full + st, (ph_full >> st) & 1, a.status);
+            ph_full ^= 1u << st;
+          };
+          auto qk = [&](int t, int st) {
+            const uint64_t qd = q_desc + (uint64_t)(t * (S::kQ >> 4)), kd = k_desc + (uint64_t)(st * (S::kStage >> 4));
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j >= w.count[t]) continue;
-          wait_bar(p_ready + t, ph_p[t], a.status);
-          ph_p[t] ^= 1;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t vb = ring + vs * S::kStage;
-#pragma unroll
-            for (int k = 0; k < kTileKeys / 16; ++k)
-              umma_ts(tmem + 2 * kTileKeys + t * D, tmem + t * kTileKeys + k * 8, desc_v(vb + k * 2048), id_o, j > 0 || k > 0);
-          }
-          if (j + 1 < w.count[t])
-            qk(t, j + 1);
-          else if (lane == 0)
+            for (int k = 0; k < D / 16; ++k)
+              umma_bf16(tmem + t * KEYS, qd + (((k >> 2) * (kTileRows * 128) + (k & 3) * 32) >> 4),
+                        kd + (((k >> 2) * (KEYS * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
             umma_commit(s_full + t);
-          __syncwarp();
+          };
+          auto pv = [&](int t, uint64_t vd, int from, int to, bool fresh) {
+#pragma unroll
+            for (int k = from; k < to; ++k)
+              umma_ts(tmem + TILES * KEYS + t * D, tmem + t * KEYS + k * 8, vd + k * 128, id_o, !fresh || k > 0);
+          };
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) {
+            if (t >= w.tiles) continue;
+            wait_bar(q_full + t, ph_q[t], a.status);
+            ph_q[t] ^= 1;
+          }
+          int ks = loads % NS;  // stage of the next K tile
+          if (blocks > 0) {
+            wait_tile(ks);
+            tc_fence_after();
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+              if (w.count[t] > 0) qk(t, ks);
+            umma_commit(kv_empty + ks);
+          }
+#pragma unroll 1
+          for (int j = 0; j < blocks; ++j) {
+            const int vs = ks + 1 == NS ? 0 : ks + 1;
+            ks = vs + 1 == NS ? 0 : vs + 1;
+            if (w.guarded(w.b0 + j)) {
+              wait_bar(v_ok + vs, (ph_v >> vs) & 1, a.status);
+              ph_v ^= 1u << vs;
+            } else {
+              wait_tile(vs);
+            }
+            if (j + 1 < blocks) wait_tile(ks);
+            const uint64_t vd = v_desc + (uint64_t)(vs * (S::kStage >> 4));
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+              if (j >= w.count[t]) continue;
+              wait_bar(p_early + t, ph_p[t], a.status);
+              tc_fence_after();
+              pv(t, vd, 0, S::kEarly / 16, j == 0);
+              wait_bar(p_late + t, ph_p[t], a.status);
+              ph_p[t] ^= 1;
+              tc_fence_after();
+              pv(t, vd, S::kEarly / 16, KEYS / 16, false);
+              if (j + 1 < w.count[t])
+                qk(t, ks);
+              else
+                umma_commit(s_full + t);
+            }
+            umma_commit(kv_empty + vs);
+            if (j + 1 < blocks) umma_commit(kv_empty + ks);
+          }
         }
-        if (lane == 0) {
-          umma_commit(kv_empty + vs);
-          if (j + 1 < blocks) umma_commit(kv_empty + (vi + 1) % NS);
-        }
+        __syncwarp();
+        loads += 2 * blocks;
+        next_group(group);
       }
-    } else if (warp == 9) {
+    } else if (warp == SW + 1) {
       // ------------------------------------------------------------ loads
       const int shift = a.pages.page_shift;
       const int32_t* table = a.seqs.table + b * a.seqs.table_stride;
-      const int boxes = kTileKeys / box_rows;  // pages of a block, 1 to 8
+      const int boxes = KEYS / box_rows;  // boxes of a block, 1 to 8
 #pragma unroll 1
-      for (int j = 0; j < blocks; ++j) {
-        const int key0 = (w.b0 + j) * kTileKeys;
-        const int here = min(boxes, (w.keys - key0 + box_rows - 1) / box_rows);  // boxes with keys
+      for (int64_t group = group_of; group * kRows < rows; group += groups_hint) {
+        const Group<TILES, KEYS> w(a, group, rows, pos0, cap, split);
+        const int blocks = w.blocks();
         const int box = lane % 8, half = lane / 8;  // lane -> box and 64-column half
-        const bool mine = box < here && half < D / 64;
-        int page = 0;
-        if (mine) {
-          page = __ldg(table + ((key0 + box * box_rows) >> shift));
-          if ((uint32_t)page >= (uint32_t)a.pages.num_pages) {
+        auto page_id = [&](int j) {
+          const int key = (w.b0 + j) * KEYS + box * box_rows;
+          return j < blocks && box < boxes && half < D / 64 && key < w.keys ? __ldg(table + (key >> shift)) : 0;
+        };
+        int next = page_id(0);
+#pragma unroll 1
+        for (int j = 0; j < blocks; ++j) {
+          const int key0 = (w.b0 + j) * KEYS;
+          const int here = min(boxes, (w.keys - key0 + box_rows - 1) / box_rows);  // boxes with keys
+          const bool mine = box < here && half < D / 64;
+          int page = next;
+          next = page_id(j + 1);
+          if (mine && (uint32_t)page >= (uint32_t)a.pages.num_pages) {
             atomicOr(a.status, DEVERR_PAGE);
             page = a.pages.num_pages;  // out of bounds: filled with zeros
           }
-        }
-        const int in_page = (key0 + box * box_rows) & ((1 << shift) - 1);
+          const int in_page = (key0 + box * box_rows) & ((1 << shift) - 1);
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int i = loads + 2 * j + kv, st = i % NS;
-          wait_bar(kv_empty + st, ((i / NS) & 1) ^ 1, a.status);
-          uint64_t* full = (kv && w.guarded(w.b0 + j) ? g_full : kv_full) + st;
-          if (lane == 0) mbar_arrive_expect_tx(full, here * box_rows * 128 * (D / 64));
-          __syncwarp();
-          if (mine)
-            tma_load_4d(ring + st * S::kStage + half * (kTileKeys * 128) + box * box_rows * 128, kv ? &map_v : &map_k,
-                        half * 64, in_page, kvh, page, full);
-          __syncwarp();
-        }
-      }
-      // every tile has been read before the CTA may end
-      const int n = 2 * blocks;
-      for (int i = max(0, n - NS); i < n; ++i)
-        wait_bar(kv_empty + (loads + i) % NS, ((loads + i) / NS) & 1, a.status);
-    } else {
-      // ------------------------------------------------------------ guards
-      const int g = tid - 320;
-#pragma unroll 1
-      for (int j = 0; j < blocks; ++j) {
-        const int block = w.b0 + j;
-        if (!w.guarded(block)) continue;
-        const int vi = loads + 2 * j + 1, vs = vi % NS;
-        wait_bar(g_full + vs, (ph_v >> vs) & 1, a.status);
-        ph_v ^= 1u << vs;
-        uint8_t* v = smem + 2 * S::kQ + vs * S::kStage;
-        const int key0 = block * kTileKeys, here = min(kTileKeys, w.keys - key0);
-        constexpr int CH = D / 8;
-        uint32_t bad = 0;
-#pragma unroll 4
-        for (int i = g; i < kTileKeys * CH; i += 64) {  // 16-byte chunk i of the tile, as it lies
-          const int key = (i >> 3) & (kTileKeys - 1);
-          uint4* p = reinterpret_cast<uint4*>(v) + i;
-          if (key >= here) {
-            *p = make_uint4(0, 0, 0, 0);
-          } else {
-            const uint4 u = *p;
-            bad |= not_finite2<T>(u.x) | not_finite2<T>(u.y) | not_finite2<T>(u.z) | not_finite2<T>(u.w);
+          for (int kv = 0; kv < 2; ++kv) {
+            const int i = loads + 2 * j + kv, st = i % NS;
+            wait_bar(kv_empty + st, ((i / NS) & 1) ^ 1, a.status);
+            uint64_t* full = (kv && w.guarded(w.b0 + j) ? g_full : kv_full) + st;
+            if (lane == 0) mbar_arrive_expect_tx(full, here * box_rows * 128 * (D / 64));
+            __syncwarp();
+            if (mine)
+              tma_load_4d(ring + st * S::kStage + half * (KEYS * 128) + box * box_rows * 128, kv ? &map_v : &map_k,
+                          half * 64, in_page, kvh, page, full);
+            __syncwarp();
           }
         }
-        if (bad) {
-          *any_odd = 1;
+        // every tile has been read before the CTA may end
+        const int n = 2 * blocks;
+        for (int i = max(0, n - NS); i < n; ++i)
+          wait_bar(kv_empty + (loads + i) % NS, ((loads + i) / NS) & 1, a.status);
+        loads += n;
+        next_group(group);
+      }
+    } else {
+      // ------------------------------------------------------------ guards
+      const int g = tid - 32 * (SW + 2);
+      uint32_t ph_v = 0;
 #pragma unroll 1
-          for (int i = g; i < here * 8; i += 64) {
+      for (int64_t group = group_of; group * kRows < rows; group += groups_hint) {
+        const Group<TILES, KEYS> w(a, group, rows, pos0, cap, split);
+        const int blocks = w.blocks();
 #pragma unroll 1
-            for (int half = 0; half < D / 64; ++half) {
-              const int key = i >> 3, chunk = (i & 7) ^ (key & 7);
-              uint16_t* p = reinterpret_cast<uint16_t*>(v + half * (kTileKeys * 128) + i * 16);
+        for (int j = 0; j < blocks; ++j) {
+          const int block = w.b0 + j;
+          if (!w.guarded(block)) continue;
+          const int vs = (loads + 2 * j + 1) % NS;
+          wait_bar(g_full + vs, (ph_v >> vs) & 1, a.status);
+          ph_v ^= 1u << vs;
+          uint8_t* v = smem + TILES * S::kQ + vs * S::kStage;
+          const int key0 = block * KEYS, here = min(KEYS, w.keys - key0);
+          constexpr int CH = D / 8;
+          uint32_t bad = 0;
+#pragma unroll 8
+          for (int i = g; i < KEYS * CH; i += 64) {  // 16-byte chunk i of the tile, as it lies
+            const int key = (i >> 3) & (KEYS - 1);
+            uint4* p = reinterpret_cast<uint4*>(v) + i;
+            if (key >= here) {
+              *p = make_uint4(0, 0, 0, 0);
+            } else {
+              const uint4 u = *p;
+              bad |= not_finite2<T>(u.x) | not_finite2<T>(u.y) | not_finite2<T>(u.z) | not_finite2<T>(u.w);
+            }
+          }
+          if (bad) {
+            *any_odd = 1;
+#pragma unroll 1
+            for (int i = g; i < KEYS * CH; i += 64) {
+              const int key = (i >> 3) & (KEYS - 1), col = i / (8 * KEYS) * 64 + (((i & 7) ^ (key & 7)) * 8);
+              uint16_t* p = reinterpret_cast<uint16_t*>(v + i * 16);
 #pragma unroll 1
               for (int e = 0; e < 8; ++e) {
-                if (!not_finite16<T>(p[e])) continue;
                 const uint16_t bits = p[e];
+                if (!not_finite16<T>(bits)) continue;
                 const float f = to_f32<T>(*reinterpret_cast<const T*>(&bits));
-                atomicMin(odd + (f != f ? 0 : f > 0.f ? 1 : 2) * D + half * 64 + chunk * 8 + e, key0 + key);
+                atomicMin(odd + (f != f ? 0 : f > 0.f ? 1 : 2) * D + col + e, key0 + key);
                 p[e] = 0;
               }
             }
           }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_ok + vs);
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(v_ok + vs);
+        loads += 2 * blocks;
+        next_group(group);
       }
     }
-    loads += 2 * blocks;
-    __syncthreads();
-    if ((pair + pairs_hint) * (2 * kTileRows) < rows) {
-      if (*any_odd) {
-        __syncthreads();
-        for (int i = tid; i < 3 * D; i += kTilesThreads) odd[i] = INT_MAX;
-        if (tid == 0) *any_odd = 0;
-      }
-      __syncthreads();
-      tc_fence_after();
-    }
   }
-  if (warp == 8) {
-    tc_fence_after();
-    tmem_dealloc(tmem, 512);
-  }
+  if (warp == SW) tmem_dealloc(tmem, S::kTmem);
 }
 
 // ======================================================================== host
@@ -516,7 +654,7 @@ typedef CUresult (*TiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*
                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 static int map_pages(CUtensorMap* m, const void* base, int head_dim, int page_size, int kv_heads, int num_pages,
-                     int64_t row, int64_t head, int64_t page, bool half) {
+                     int64_t row, int64_t head, int64_t page, int box_rows, bool half) {
   static TiledFn fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -532,7 +670,7 @@ static int map_pages(CUtensorMap* m, const void* base, int head_dim, int page_si
   }
   const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)kv_heads, (cuuint64_t)num_pages};
   const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)std::min(page_size, kTileKeys), 1, 1}, es[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, es[4] = {1, 1, 1, 1};
   const CUresult r = fn(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                         const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -544,27 +682,33 @@ static int map_pages(CUtensorMap* m, const void* base, int head_dim, int page_si
   return PPMOE_OK;
 }
 
-template <typename T, int D>
-static int launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttendArgs& a, int page_size, int pairs,
-                  cudaStream_t st) {
-  auto fn = attend_tiles_kernel<T, D>;
-  PPMOE_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, TilesSmem<D>::kBytes));
-  const int64_t ctas = (int64_t)pairs * a.nsplit * a.pages.kv_heads * a.seqs.batch;
-  fn<<<(unsigned)ctas, kTilesThreads, TilesSmem<D>::kBytes, st>>>(mk, mv, a, std::min(page_size, kTileKeys), pairs);
+template <typename T, int D, int TILES, int KEYS>
+static int launch(const AttendArgs& a, int page_size, int groups, cudaStream_t st) {
+  using S = TilesShape<D, TILES, KEYS>;
+  constexpr bool half = std::is_same<T, __half>::value;
+  const Pages& p = a.pages;
+  const int box = std::min(page_size, KEYS);
+  CUtensorMap mk, mv;
+  if (int rc = map_pages(&mk, p.k, D, page_size, p.kv_heads, p.num_pages, p.k_row, p.k_head, p.k_page, box, half)) return rc;
+  if (int rc = map_pages(&mv, p.v, D, page_size, p.kv_heads, p.num_pages, p.v_row, p.v_head, p.v_page, box, half)) return rc;
+  auto fn = attend_tiles_kernel<T, D, TILES, KEYS>;
+  PPMOE_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+  const int64_t ctas = (int64_t)groups * a.nsplit * p.kv_heads * a.seqs.batch;
+  fn<<<(unsigned)ctas, S::kThreads, S::kBytes, st>>>(mk, mv, a, box, groups);
   PPMOE_CHECK_CUDA(cudaGetLastError());
   return PPMOE_OK;
 }
 
-int attend_tiles_launch(AttendArgs& a, int head_dim, int page_size, bool half, int pairs, cudaStream_t st) {
-  CUtensorMap mk, mv;
-  const Pages& p = a.pages;
-  if (int rc = map_pages(&mk, p.k, head_dim, page_size, p.kv_heads, p.num_pages, p.k_row, p.k_head, p.k_page, half)) return rc;
-  if (int rc = map_pages(&mv, p.v, head_dim, page_size, p.kv_heads, p.num_pages, p.v_row, p.v_head, p.v_page, half)) return rc;
-  if (half)
-    return head_dim == 128 ? launch<__half, 128>(mk, mv, a, page_size, pairs, st)
-                           : launch<__half, 64>(mk, mv, a, page_size, pairs, st);
-  return head_dim == 128 ? launch<__nv_bfloat16, 128>(mk, mv, a, page_size, pairs, st)
-                         : launch<__nv_bfloat16, 64>(mk, mv, a, page_size, pairs, st);
+int attend_tiles_launch(AttendArgs& a, int head_dim, int page_size, bool half, int tiles, int groups, cudaStream_t st) {
+  auto go = [&](auto type, auto dim) {
+    using T = decltype(type);
+    constexpr int D = decltype(dim)::value;
+    return tiles == 2 ? launch<T, D, 2, 128>(a, page_size, groups, st) : launch<T, D, 1, 64>(a, page_size, groups, st);
+  };
+  std::integral_constant<int, 128> d128;
+  std::integral_constant<int, 64> d64;
+  if (half) return head_dim == 128 ? go(__half{}, d128) : go(__half{}, d64);
+  return head_dim == 128 ? go(__nv_bfloat16{}, d128) : go(__nv_bfloat16{}, d64);
 }
 
 }  // namespace ppmoe
