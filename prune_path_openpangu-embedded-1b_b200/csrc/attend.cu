@@ -55,11 +55,6 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// 16 bytes global -> shared, or 16 zero bytes (the source is then not read).
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const __grid_constant__ AttendArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];

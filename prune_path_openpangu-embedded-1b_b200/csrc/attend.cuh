@@ -71,6 +71,11 @@ __device__ __forceinline__ void store_row(T* out, const float (&v)[C], float inv
   }
 }
 
+// 16 bytes global -> shared, or 16 zero bytes (the source is then not read).
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
 // What q is multiplied by (-1, 0 or 1), on a packed pair.
 __device__ __forceinline__ uint32_t q_pair(uint32_t v, int sign) {
   return sign > 0 ? v : sign < 0 ? v ^ 0x80008000u : 0u;

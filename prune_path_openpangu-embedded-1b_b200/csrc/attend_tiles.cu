@@ -213,6 +213,21 @@ struct Group {
   __device__ bool guarded(int block) const { return (block + 1) * KEYS > clear; }
 };
 
+// Token and head (of the group) of a row, and of the rows `step` further on, without a division each.
+struct RowWalk {
+  int64_t tok;
+  int head, d_tok, d_head, group;
+  __device__ RowWalk(int row, int step, int g) : tok(row / g), head(row % g), d_tok(step / g), d_head(step % g), group(g) {}
+  __device__ void step() {
+    tok += d_tok;
+    head += d_head;
+    if (head >= group) {
+      head -= group;
+      ++tok;
+    }
+  }
+};
+
 template <typename T, int D, int TILES, int KEYS>
 __global__ void __launch_bounds__(TilesShape<D, TILES, KEYS>::kThreads, TilesShape<D, TILES, KEYS>::kCtas)
 attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -297,25 +312,34 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       const Group<TILES, KEYS> w(a, group, rows, pos0, cap, split);
       if (t < w.tiles) {
         const int base = w.r0 + t * kTileRows, r = base + row;
-        constexpr int CH = D / 8;
-#pragma unroll 4
-        for (int i = row; i < kTileRows * CH; i += kTileRows) {
-          const int rr = i / CH, ch = i % CH, q_row = base + rr;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (q_row < rows) {
-            const int tok = q_row / a.group;
-            const T* p = static_cast<const T*>(a.q) + (int64_t)(sq.first + tok) * a.q_t +
-                         (int64_t)(kvh * a.group + q_row - tok * a.group) * a.q_h + ch * 8;
-            if (a.q_wide16) {
-              v = __ldg(reinterpret_cast<const uint4*>(p));
-            } else {
-              const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-              v = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
-                             h[6] | (uint32_t)h[7] << 16);
+        constexpr int CH = D / 8, STEP = kTileRows / CH;  // 16-byte chunks of a row, rows the 128 threads take at once
+        const int ch = row % CH;
+        {
+          uint8_t* q_s = smem + t * S::kQ + (ch >> 3) * (kTileRows * 128);
+          RowWalk at(base + row / CH, STEP, a.group);
+          const T* q = static_cast<const T*>(a.q) + sq.first * a.q_t + (int64_t)kvh * a.group * a.q_h + ch * 8;
+          if (a.q_wide16 && a.q_sign > 0) {  // all in flight at once: 1.5 us; by way of registers it took 10
+#pragma unroll
+            for (int i = 0; i < CH; ++i, at.step()) {
+              const int rr = row / CH + i * STEP;
+              const bool real = base + rr < rows;
+              cp_async16_or_zero(smem_u32(q_s + sw128_offset(rr, ch & 7)), q + (real ? at.tok * a.q_t + at.head * a.q_h : 0), real);
             }
-            v = make_uint4(q_pair(v.x, a.q_sign), q_pair(v.y, a.q_sign), q_pair(v.z, a.q_sign), q_pair(v.w, a.q_sign));
+            cp_async_commit();
+            cp_async_wait<0>();
+          } else {
+#pragma unroll 1
+            for (int i = 0; i < CH; ++i, at.step()) {
+              const int rr = row / CH + i * STEP;
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (base + rr < rows) {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(q + at.tok * a.q_t + at.head * a.q_h);
+                v = make_uint4(q_pair(h[0] | (uint32_t)h[1] << 16, a.q_sign), q_pair(h[2] | (uint32_t)h[3] << 16, a.q_sign),
+                               q_pair(h[4] | (uint32_t)h[5] << 16, a.q_sign), q_pair(h[6] | (uint32_t)h[7] << 16, a.q_sign));
+              }
+              *reinterpret_cast<uint4*>(q_s + sw128_offset(rr, ch & 7)) = v;
+            }
           }
-          *reinterpret_cast<uint4*>(smem + t * S::kQ + (ch >> 3) * (kTileRows * 128) + sw128_offset(rr, ch & 7)) = v;
         }
         fence_proxy_async();
         mbar_arrive(q_full + t);
@@ -422,44 +446,79 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         const bool listed = *reinterpret_cast<volatile int*>(any_odd) != 0;
         const float inv = a.nsplit > 1 ? 1.f : l > 0.f ? 1.f / l : l == l ? 0.f : l;
-        const int64_t token = sq.first + tok;
-        const int h = kvh * a.group + r - tok * a.group;
-        const int64_t at = ((int64_t)split * a.tokens + token) * a.q_heads + h;
+        // Through the q tile's place (no product reads it any more) to whole rows in memory: results in one go,
+        // parts in two halves of the columns.
+        uint8_t* stage = smem + t * S::kQ;
+        const int per = a.nsplit > 1 ? D / 2 : D;  // columns of one go
 #pragma unroll 1
-        for (int i = 0; i < D; i += 32) {
-          float o[32];
-          if (count > 0) {
-            tmem_ld32_async(t_o + i, o);
-            tmem_ld_wait();
-            tmem_ld_bind(o);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0.f;
-          }
-          if (listed) {
+        for (int c0 = 0; c0 < D; c0 += per) {
 #pragma unroll 1
-            for (int e = 0; e < 32; ++e) {
-              float add = 0.f;
-              if (odd[D + i + e] <= lim) add += CUDART_INF_F;
-              if (odd[2 * D + i + e] <= lim) add -= CUDART_INF_F;
-              if (odd[i + e] <= lim) add = CUDART_NAN_F;
-              if (!(add == 0.f)) {
+          for (int i = c0; i < c0 + per; i += 32) {
+            float o[32];
+            if (count > 0) {
+              tmem_ld32_async(t_o + i, o);
+              tmem_ld_wait();
+              tmem_ld_bind(o);
+            } else {
 #pragma unroll
-                for (int z = 0; z < 32; ++z) o[z] = z == e ? o[z] + add : o[z];
+              for (int e = 0; e < 32; ++e) o[e] = 0.f;
+            }
+            if (listed) {
+#pragma unroll 1
+              for (int e = 0; e < 32; ++e) {
+                float add = 0.f;
+                if (odd[D + i + e] <= lim) add += CUDART_INF_F;
+                if (odd[2 * D + i + e] <= lim) add -= CUDART_INF_F;
+                if (odd[i + e] <= lim) add = CUDART_NAN_F;
+                if (!(add == 0.f)) {
+#pragma unroll
+                  for (int z = 0; z < 32; ++z) o[z] = z == e ? o[z] + add : o[z];
+                }
               }
             }
-          }
-          if (r < rows) {
+            uint8_t* line = stage + row * (D * 2);
             if (a.nsplit == 1) {
-              store_row<T, 32>(static_cast<T*>(a.out) + token * a.o_t + h * a.o_h + i, o, inv, a.o_wide);
+#pragma unroll
+              for (int e = 0; e < 32; e += 8)
+                *reinterpret_cast<uint4*>(line + ((((i + e) / 8) ^ (row & 7)) << 4)) =
+                    make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv),
+                               pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
             } else {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<float4*>(a.part_o + at * D + i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                *reinterpret_cast<float4*>(line + ((((i - c0 + e) / 4) ^ (row & 7)) << 4)) =
+                    make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
+          named_bar_sync(1 + t, kTileRows);
+          RowWalk at(base + row / CH, STEP, a.group);
+#pragma unroll 4
+          for (int i = 0; i < CH; ++i, at.step()) {
+            const int rr = row / CH + i * STEP;
+            if (base + rr >= rows) break;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((ch ^ (rr & 7)) << 4));
+            const int64_t token = sq.first + at.tok;
+            const int h = kvh * a.group + at.head;
+            if (a.nsplit > 1) {
+              float* part = a.part_o + (((int64_t)split * a.tokens + token) * a.q_heads + h) * D;
+              *reinterpret_cast<uint4*>(part + c0 + ch * 4) = v;
+            } else {
+              T* out = static_cast<T*>(a.out) + token * a.o_t + h * a.o_h + ch * 8;
+              if (a.o_wide) {
+                *reinterpret_cast<uint4*>(out) = v;
+              } else {
+                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(out)[e] = (uint16_t)(u[e / 2] >> (16 * (e & 1)));
+              }
+            }
+          }
+          if (c0 + per < D) named_bar_sync(1 + t, kTileRows);
         }
-        if (a.nsplit > 1 && r < rows) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m * c, l);
+        if (a.nsplit > 1 && r < rows) {
+          const int64_t at = ((int64_t)split * a.tokens + sq.first + tok) * a.q_heads + kvh * a.group + r - tok * a.group;
+          *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m * c, l);
+        }
       }
       next_group(group);
     }
@@ -518,7 +577,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             } else {
               wait_tile(vs);
             }
-            if (j + 1 < blocks) wait_tile(ks);
+            bool next = j + 1 < blocks;  // its K tile has not been waited for yet
             const uint64_t vd = v_desc + (uint64_t)(vs * (S::kStage >> 4));
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
@@ -526,6 +585,10 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               wait_bar(p_early + t, ph_p[t], a.status);
               tc_fence_after();
               pv(t, vd, 0, S::kEarly / 16, j == 0);
+              if (next) {
+                wait_tile(ks);
+                next = false;
+              }
               wait_bar(p_late + t, ph_p[t], a.status);
               ph_p[t] ^= 1;
               tc_fence_after();
@@ -536,6 +599,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 umma_commit(s_full + t);
             }
             umma_commit(kv_empty + vs);
+            if (next) wait_tile(ks);
             if (j + 1 < blocks) umma_commit(kv_empty + ks);
           }
         }
