@@ -258,26 +258,43 @@ PPMOE_API int ppmoe_decode_noalloc_status(void* stream);
  * The attention half of a decoder layer around a paged key/value cache.
  *
  * dtype: PPMOE_BF16, PPMOE_F16 (and PPMOE_F32 for ppmoe_rotary) of every value tensor of the
- * call.  Strides are in elements; the values of one head are contiguous.
+ * call.  Strides are in elements; the values of one head are contiguous.  The two structures are
+ * read during the call and not kept: a captured graph holds what they said then.
  * ------------------------------------------------------------------------------------- */
 #define PPMOE_BF16 0
 #define PPMOE_F16 1
 #define PPMOE_F32 2
 
+/* A rotation: the first rotary_dim values of a head are rotary_dim / 2 pairs (i, i + rotary_dim / 2),
+ * or (2i, 2i + 1) with interleaved != 0; pair i at position p turns by 2 pi p turns[i] and is
+ * multiplied by gain; the other values are copied.  The angle is reduced in fp64. */
+typedef struct ppmoe_rotation {
+  int rotary_dim, interleaved;
+  double gain;
+  double turns[128];
+} ppmoe_rotation;
+
 /* Rotary position embedding of queries [batch][length][q_heads][head_dim] and keys (k_heads; 0:
- * none) in one launch.  The first rotary_dim values of a head are rotary_dim / 2 pairs (i, i +
- * rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0; pair i at position p turns by
- * 2 pi p turns[i] and is multiplied by gain; the other values are copied.  turns: rotary_dim / 2
- * doubles in HOST memory, copied into the launch (a captured graph keeps them).  The angle is
- * reduced in fp64.  inverse != 0 turns the other way: the gradient.  positions: int64 or int32,
+ * none) in one launch.  inverse != 0 turns the other way: the gradient.  positions: int64 or int32,
  * element (b, t) at b * pos_b + t * pos_t.  q_out may be q with the same strides (in place), likewise
  * k_out; otherwise outputs overlap nothing.  head_dim even, 2 .. 256. */
-PPMOE_API int ppmoe_rotary(const void* q, int64_t q_b, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_b,
-                           int64_t qo_t, int64_t qo_h, int q_heads, const void* k, int64_t k_b, int64_t k_t,
-                           int64_t k_h, void* k_out, int64_t ko_b, int64_t ko_t, int64_t ko_h, int k_heads, int batch,
-                           int64_t length, int head_dim, int rotary_dim, int interleaved, const double* turns,
-                           float gain, int inverse, const void* positions, int positions64, int64_t pos_b,
-                           int64_t pos_t, int dtype, void* stream);
+PPMOE_API int ppmoe_rotary(const ppmoe_rotation* rotation, int inverse, const void* q, int64_t q_b, int64_t q_t,
+                           int64_t q_h, void* q_out, int64_t qo_b, int64_t qo_t, int64_t qo_h, int q_heads,
+                           const void* k, int64_t k_b, int64_t k_t, int64_t k_h, void* k_out, int64_t ko_b,
+                           int64_t ko_t, int64_t ko_h, int k_heads, int batch, int64_t length, int head_dim,
+                           const void* positions, int positions64, int64_t pos_b, int64_t pos_t, int dtype,
+                           void* stream);
+
+/* A paged cache: k and v with strides (page, head, row), 16-byte aligned, every stride whole 16
+ * bytes; page_size 16, 32, 64, 128 or 256; head_dim 64 or 128; bf16 or fp16.
+ * status: device memory, >= 256 bytes, zeroed once (ppmoe_workspace_init); a position whose page the
+ * table or the cache does not have is recorded there and reported by ppmoe_workspace_status. */
+typedef struct ppmoe_kv_cache {
+  void *k, *v;
+  int64_t k_page, k_head, k_row, v_page, v_head, v_row;
+  int num_pages, page_size, kv_heads, head_dim, dtype;
+  void* status;
+} ppmoe_kv_cache;
 
 /* A ragged batch over a paged cache, as the two calls below take it: sequence b owns the packed
  * rows [starts[b], starts[b+1]), its newest tokens; lengths[b] counts its positions, these rows
@@ -286,22 +303,15 @@ PPMOE_API int ppmoe_rotary(const void* q, int64_t q_b, int64_t q_t, int64_t q_h,
  * lengths [batch], table [batch][max_pages] (rows table_stride apart): int32, device memory, read
  * by the kernels, so a captured graph follows their contents.  Rows outside every sequence are
  * left alone.  Page ids of positions that a sequence does not reach are not read.
- * Cache: k_pages and v_pages with strides (page, head, row), 16-byte aligned, every stride whole
- * 16 bytes; page_size 16, 32, 64, 128 or 256; head_dim 64 or 128; num_pages pages.
- * status: >= 256 bytes, zeroed once (ppmoe_workspace_init); a position whose page the table or
- * the cache does not have is recorded there and reported by ppmoe_workspace_status.
  *
- * Append: rows of k are rotated (as by ppmoe_rotary, at their positions; rotary_dim 0: not) and
- * written to the cache with the rows of v; rows of q (q_heads 0: none) are rotated into q_out (which
- * may be q).  A row without a page is not stored.  Two rows of a call must not share a place. */
-PPMOE_API int ppmoe_kv_append(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h,
-                              int q_heads, const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t,
-                              int64_t v_h, int tokens, void* k_pages, int64_t kp_page, int64_t kp_head,
-                              int64_t kp_row, void* v_pages, int64_t vp_page, int64_t vp_head, int64_t vp_row,
-                              int num_pages, int page_size, int kv_heads, int head_dim, const int32_t* starts,
-                              const int32_t* lengths, const int32_t* table, int64_t table_stride, int batch,
-                              int max_pages, int rotary_dim, int interleaved, const double* turns, float gain,
-                              int dtype, void* status, void* stream);
+ * Append: rows of k are rotated to their positions (rotation NULL: not) and written to the cache with
+ * the rows of v; rows of q (q_heads 0: none) are rotated into q_out (which may be q).  A row without a
+ * page is not stored.  Two rows of a call must not share a place. */
+PPMOE_API int ppmoe_kv_append(const ppmoe_kv_cache* cache, const ppmoe_rotation* rotation, const void* q, int64_t q_t,
+                              int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h, int q_heads, const void* k,
+                              int64_t k_t, int64_t k_h, const void* v, int64_t v_t, int64_t v_h, int tokens,
+                              const int32_t* starts, const int32_t* lengths, const int32_t* table,
+                              int64_t table_stride, int batch, int max_pages, void* stream);
 
 /* Attention: out[t][h] = sum over positions j <= p(t) of softmax_j(scale q[t][h] . k_j) v_j over
  * the cache of t's sequence, with query head h reading kv head h / (q_heads / kv_heads); 0 where no
@@ -311,12 +321,10 @@ PPMOE_API int ppmoe_kv_append(const void* q, int64_t q_t, int64_t q_h, void* q_o
  * numbers, 16-byte aligned, contents of no importance before or after the call. */
 PPMOE_API size_t ppmoe_attend_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim, int batch,
                                               int max_new, int64_t max_length);
-PPMOE_API int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads, int tokens, const void* k_pages,
-                           int64_t kp_page, int64_t kp_head, int64_t kp_row, const void* v_pages, int64_t vp_page,
-                           int64_t vp_head, int64_t vp_row, int num_pages, int page_size, int kv_heads, int head_dim,
-                           const int32_t* starts, const int32_t* lengths, const int32_t* table, int64_t table_stride,
-                           int batch, int max_pages, float scale, int max_new, int64_t max_length, void* out,
-                           int64_t o_t, int64_t o_h, int dtype, void* status, void* ws, size_t ws_bytes,
+PPMOE_API int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t q_t, int64_t q_h, int q_heads,
+                           int tokens, const int32_t* starts, const int32_t* lengths, const int32_t* table,
+                           int64_t table_stride, int batch, int max_pages, float scale, int max_new,
+                           int64_t max_length, void* out, int64_t o_t, int64_t o_h, void* ws, size_t ws_bytes,
                            void* stream);
 
 /* Diagnostics: when `buf` (device, >= 32 * 8 bytes per CTA of the decode grid) is non-NULL,

@@ -25,6 +25,21 @@ _c_int64 = ctypes.c_int64
 
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 
+
+class Rotation(ctypes.Structure):
+    """``ppmoe_rotation``"""
+    _fields_ = [("rotary_dim", _c_int), ("interleaved", _c_int), ("gain", ctypes.c_double),
+                ("turns", ctypes.c_double * 128)]
+
+
+class KVCache(ctypes.Structure):
+    """``ppmoe_kv_cache``"""
+    _fields_ = ([("k", _c_void_p), ("v", _c_void_p)]
+                + [(n, _c_int64) for n in ("k_page", "k_head", "k_row", "v_page", "v_head", "v_row")]
+                + [(n, _c_int) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "dtype")]
+                + [("status", _c_void_p)])
+
+
 # name -> (restype, argtypes); mirrors include/ppmoe.h
 SIGNATURES = {
     "ppmoe_version": (_c_int, []),
@@ -68,20 +83,17 @@ SIGNATURES = {
     "ppmoe_decode_host": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_float,
                                    _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size_t,
                                    _c_void_p]),
-    "ppmoe_rotary": (_c_int, [_c_void_p, _c_int64, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_int64,
-                              _c_int, _c_void_p, _c_int64, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64,
-                              _c_int64, _c_int, _c_int, _c_int64, _c_int, _c_int, _c_int, _c_void_p, _c_float,
-                              _c_int, _c_void_p, _c_int, _c_int64, _c_int64, _c_int, _c_void_p]),
-    "ppmoe_kv_append": (_c_int, [_c_void_p, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_int, _c_void_p,
-                                 _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_int, _c_void_p, _c_int64,
-                                 _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_int64, _c_int, _c_int,
-                                 _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int, _c_int, _c_int,
-                                 _c_int, _c_void_p, _c_float, _c_int, _c_void_p, _c_void_p]),
+    "ppmoe_rotary": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_int64, _c_int64, _c_int64, _c_void_p, _c_int64,
+                              _c_int64, _c_int64, _c_int, _c_void_p, _c_int64, _c_int64, _c_int64, _c_void_p, _c_int64,
+                              _c_int64, _c_int64, _c_int, _c_int, _c_int64, _c_int, _c_void_p, _c_int, _c_int64,
+                              _c_int64, _c_int, _c_void_p]),
+    "ppmoe_kv_append": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64,
+                                 _c_int, _c_void_p, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int64, _c_int,
+                                 _c_void_p, _c_void_p, _c_void_p, _c_int64, _c_int, _c_int, _c_void_p]),
     "ppmoe_attend_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int64]),
-    "ppmoe_attend": (_c_int, [_c_void_p, _c_int64, _c_int64, _c_int, _c_int, _c_void_p, _c_int64, _c_int64, _c_int64,
-                              _c_void_p, _c_int64, _c_int64, _c_int64, _c_int, _c_int, _c_int, _c_int, _c_void_p,
-                              _c_void_p, _c_void_p, _c_int64, _c_int, _c_int, _c_float, _c_int, _c_int64, _c_void_p,
-                              _c_int64, _c_int64, _c_int, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    "ppmoe_attend": (_c_int, [_c_void_p, _c_void_p, _c_int64, _c_int64, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p,
+                              _c_int64, _c_int, _c_int, _c_float, _c_int, _c_int64, _c_void_p, _c_int64, _c_int64,
+                              _c_void_p, _c_size_t, _c_void_p]),
 }
 
 _lib = None

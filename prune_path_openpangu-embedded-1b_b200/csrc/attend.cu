@@ -479,24 +479,17 @@ extern "C" size_t ppmoe_attend_workspace_bytes(int tokens, int q_heads, int kv_h
   return plan_bytes(plan_of(tokens, q_heads, kv_heads, batch, max_new, max_length), tokens, q_heads, head_dim);
 }
 
-extern "C" int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads, int tokens, const void* k_pages,
-                            int64_t kp_page, int64_t kp_head, int64_t kp_row, const void* v_pages, int64_t vp_page,
-                            int64_t vp_head, int64_t vp_row, int num_pages, int page_size, int kv_heads, int head_dim,
-                            const int32_t* starts, const int32_t* lengths, const int32_t* table, int64_t table_stride,
-                            int batch, int max_pages, float scale, int max_new, int64_t max_length, void* out,
-                            int64_t o_t, int64_t o_h, int dtype, void* status, void* ws, size_t ws_bytes,
+extern "C" int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t q_t, int64_t q_h, int q_heads,
+                            int tokens, const int32_t* starts, const int32_t* lengths, const int32_t* table,
+                            int64_t table_stride, int batch, int max_pages, float scale, int max_new,
+                            int64_t max_length, void* out, int64_t o_t, int64_t o_h, void* ws, size_t ws_bytes,
                             void* stream) {
   clear_error();
   AttendArgs a{};
-  a.pages = {const_cast<void*>(k_pages), const_cast<void*>(v_pages), kp_page, kp_head, kp_row, vp_page, vp_head,
-             vp_row, num_pages, 0, kv_heads};
   a.seqs = {starts, lengths, table, table_stride, batch, max_pages};
-  if (int rc = check_pages("ppmoe_attend", a.pages, page_size, head_dim)) return rc;
+  if (int rc = check_cache("ppmoe_attend", cache, a.pages)) return rc;
   if (int rc = check_seqs("ppmoe_attend", a.seqs)) return rc;
-  if (dtype != PPMOE_BF16 && dtype != PPMOE_F16) {
-    set_error("ppmoe_attend: dtype=%d (0 bf16, 1 fp16)", dtype);
-    return PPMOE_ERR_UNSUPPORTED;
-  }
+  const int kv_heads = cache->kv_heads, head_dim = cache->head_dim;
   if (tokens < 0 || q_heads < 1 || q_heads % kv_heads) {
     set_error("ppmoe_attend: tokens=%d, q_heads=%d must be a positive multiple of kv_heads=%d", tokens, q_heads,
               kv_heads);
@@ -508,7 +501,7 @@ extern "C" int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads
               (long long)batch * kv_heads, (long long)tokens * q_heads);
     return PPMOE_ERR_UNSUPPORTED;
   }
-  if (!q || !out || !status) {
+  if (!q || !out) {
     set_error("ppmoe_attend: null pointer");
     return PPMOE_ERR_INVALID_ARG;
   }
@@ -522,7 +515,6 @@ extern "C" int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads
     set_error("ppmoe_attend: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, ws ? ws_bytes : 0);
     return PPMOE_ERR_WORKSPACE;
   }
-  while ((1 << a.pages.page_shift) < page_size) ++a.pages.page_shift;
   a.q = q;
   a.q_t = q_t;
   a.q_h = q_h;
@@ -543,9 +535,9 @@ extern "C" int ppmoe_attend(const void* q, int64_t q_t, int64_t q_h, int q_heads
   a.nsplit = p.nsplit;
   a.part_o = static_cast<float*>(ws);
   a.part_ml = a.part_o + (size_t)p.nsplit * tokens * q_heads * head_dim;
-  a.status = static_cast<uint32_t*>(status);
+  a.status = static_cast<uint32_t*>(cache->status);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == PPMOE_BF16)
+  if (cache->dtype == PPMOE_BF16)
     return head_dim == 128 ? launch<__nv_bfloat16, 128>(a, p, st) : launch<__nv_bfloat16, 64>(a, p, st);
   return head_dim == 128 ? launch<__half, 128>(a, p, st) : launch<__half, 64>(a, p, st);
 }

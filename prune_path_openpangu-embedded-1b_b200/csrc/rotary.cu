@@ -211,41 +211,49 @@ static bool wide_view(const void* p, int64_t sb, int64_t st, int64_t sh, int siz
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && sb % v == 0 && st % v == 0 && sh % v == 0;
 }
 
-static int check_rotation(const char* fn, int head_dim, int rotary_dim, const double* turns, RotaryArgs& a) {
+static int check_rotation(const char* fn, int head_dim, const ppmoe_rotation* r, RotaryArgs& a) {
+  const int rotary_dim = r ? r->rotary_dim : 0;
   if (head_dim < 2 || head_dim > 2 * kMaxPairs || head_dim % 2 || rotary_dim < 0 || rotary_dim > head_dim ||
       rotary_dim % 2) {
     set_error("%s: head_dim=%d must be even and in [2, %d], rotary_dim=%d even and in [0, head_dim]", fn, head_dim,
               2 * kMaxPairs, rotary_dim);
     return PPMOE_ERR_UNSUPPORTED;
   }
-  if (rotary_dim && !turns) {
-    set_error("%s: null turns", fn);
-    return PPMOE_ERR_INVALID_ARG;
-  }
   a.head_dim = head_dim;
   a.pairs = rotary_dim / 2;
-  for (int i = 0; i < a.pairs; ++i) a.turns[i] = turns[i];
+  a.gain = r ? (float)r->gain : 1.f;
+  for (int i = 0; i < a.pairs; ++i) a.turns[i] = r->turns[i];
   return PPMOE_OK;
 }
 
-int check_pages(const char* fn, const Pages& p, int page_size, int head_dim) {
-  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) {
-    set_error("%s: page_size=%d must be 16, 32, 64, 128 or 256", fn, page_size);
-    return PPMOE_ERR_UNSUPPORTED;
-  }
-  if (head_dim != 64 && head_dim != 128) {
-    set_error("%s: head_dim=%d must be 64 or 128", fn, head_dim);
-    return PPMOE_ERR_UNSUPPORTED;
-  }
-  if (p.num_pages < 1 || p.kv_heads < 1) {
-    set_error("%s: num_pages=%d and kv_heads=%d must be positive", fn, p.num_pages, p.kv_heads);
+int check_cache(const char* fn, const ppmoe_kv_cache* c, Pages& p) {
+  if (!c) {
+    set_error("%s: null cache", fn);
     return PPMOE_ERR_INVALID_ARG;
   }
-  if (!p.k || !p.v || !wide_view(p.k, p.k_page, p.k_head, p.k_row, 2) ||
-      !wide_view(p.v, p.v_page, p.v_head, p.v_row, 2)) {
+  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) {
+    set_error("%s: page_size=%d must be 16, 32, 64, 128 or 256", fn, c->page_size);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
+  if (c->head_dim != 64 && c->head_dim != 128) {
+    set_error("%s: head_dim=%d must be 64 or 128", fn, c->head_dim);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
+  if (c->dtype != PPMOE_BF16 && c->dtype != PPMOE_F16) {
+    set_error("%s: dtype=%d (0 bf16, 1 fp16)", fn, c->dtype);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
+  if (c->num_pages < 1 || c->kv_heads < 1) {
+    set_error("%s: num_pages=%d and kv_heads=%d must be positive", fn, c->num_pages, c->kv_heads);
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  if (!c->k || !c->v || !c->status || !wide_view(c->k, c->k_page, c->k_head, c->k_row, 2) ||
+      !wide_view(c->v, c->v_page, c->v_head, c->v_row, 2)) {
     set_error("%s: cache tensors must be non-null, 16-byte aligned, with strides of whole 16 bytes", fn);
     return PPMOE_ERR_INVALID_ARG;
   }
+  p = {c->k, c->v, c->k_page, c->k_head, c->k_row, c->v_page, c->v_head, c->v_row, c->num_pages, 0, c->kv_heads};
+  while ((1 << p.page_shift) < c->page_size) ++p.page_shift;
   return PPMOE_OK;
 }
 
@@ -265,15 +273,19 @@ int check_seqs(const char* fn, const Seqs& s) {
 
 using namespace ppmoe;
 
-extern "C" int ppmoe_rotary(const void* q, int64_t q_b, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_b,
-                            int64_t qo_t, int64_t qo_h, int q_heads, const void* k, int64_t k_b, int64_t k_t,
-                            int64_t k_h, void* k_out, int64_t ko_b, int64_t ko_t, int64_t ko_h, int k_heads, int batch,
-                            int64_t length, int head_dim, int rotary_dim, int interleaved, const double* turns,
-                            float gain, int inverse, const void* positions, int positions64, int64_t pos_b,
-                            int64_t pos_t, int dtype, void* stream) {
+extern "C" int ppmoe_rotary(const ppmoe_rotation* rotation, int inverse, const void* q, int64_t q_b, int64_t q_t,
+                            int64_t q_h, void* q_out, int64_t qo_b, int64_t qo_t, int64_t qo_h, int q_heads,
+                            const void* k, int64_t k_b, int64_t k_t, int64_t k_h, void* k_out, int64_t ko_b,
+                            int64_t ko_t, int64_t ko_h, int k_heads, int batch, int64_t length, int head_dim,
+                            const void* positions, int positions64, int64_t pos_b, int64_t pos_t, int dtype,
+                            void* stream) {
   clear_error();
   RotaryArgs a{};
-  if (int rc = check_rotation("ppmoe_rotary", head_dim, rotary_dim, turns, a)) return rc;
+  if (!rotation) {
+    set_error("ppmoe_rotary: null rotation");
+    return PPMOE_ERR_INVALID_ARG;
+  }
+  if (int rc = check_rotation("ppmoe_rotary", head_dim, rotation, a)) return rc;
   if (dtype != PPMOE_BF16 && dtype != PPMOE_F16 && dtype != PPMOE_F32) {
     set_error("ppmoe_rotary: dtype=%d (0 bf16, 1 fp16, 2 fp32)", dtype);
     return PPMOE_ERR_UNSUPPORTED;
@@ -302,52 +314,42 @@ extern "C" int ppmoe_rotary(const void* q, int64_t q_b, int64_t q_t, int64_t q_h
   a.pos_t = pos_t;
   a.batch = batch;
   a.length = length;
-  a.gain = gain;
   a.sign = inverse ? -1.f : 1.f;
-  const bool wide = head_dim % (2 * v) == 0 && rotary_dim % (2 * v) == 0 &&
+  const bool wide = head_dim % (2 * v) == 0 && rotation->rotary_dim % (2 * v) == 0 &&
                     (!q_heads || (wide_view(q, q_b, q_t, q_h, size) && wide_view(q_out, qo_b, qo_t, qo_h, size))) &&
                     (!k_heads || (wide_view(k, k_b, k_t, k_h, size) && wide_view(k_out, ko_b, ko_t, ko_h, size)));
-  return launch<false>(a, interleaved != 0, dtype, wide, static_cast<cudaStream_t>(stream));
+  return launch<false>(a, rotation->interleaved != 0, dtype, wide, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int ppmoe_kv_append(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h,
-                               int q_heads, const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t,
-                               int64_t v_h, int tokens, void* k_pages, int64_t kp_page, int64_t kp_head,
-                               int64_t kp_row, void* v_pages, int64_t vp_page, int64_t vp_head, int64_t vp_row,
-                               int num_pages, int page_size, int kv_heads, int head_dim, const int32_t* starts,
-                               const int32_t* lengths, const int32_t* table, int64_t table_stride, int batch,
-                               int max_pages, int rotary_dim, int interleaved, const double* turns, float gain,
-                               int dtype, void* status, void* stream) {
+extern "C" int ppmoe_kv_append(const ppmoe_kv_cache* cache, const ppmoe_rotation* rotation, const void* q, int64_t q_t,
+                               int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h, int q_heads, const void* k,
+                               int64_t k_t, int64_t k_h, const void* v, int64_t v_t, int64_t v_h, int tokens,
+                               const int32_t* starts, const int32_t* lengths, const int32_t* table,
+                               int64_t table_stride, int batch, int max_pages, void* stream) {
   clear_error();
   RotaryArgs a{};
-  a.pages = {k_pages, v_pages, kp_page, kp_head, kp_row, vp_page, vp_head, vp_row, num_pages, 0, kv_heads};
   a.seqs = {starts, lengths, table, table_stride, batch, max_pages};
-  if (int rc = check_rotation("ppmoe_kv_append", head_dim, rotary_dim, turns, a)) return rc;
-  if (int rc = check_pages("ppmoe_kv_append", a.pages, page_size, head_dim)) return rc;
+  if (int rc = check_cache("ppmoe_kv_append", cache, a.pages)) return rc;
+  if (int rc = check_rotation("ppmoe_kv_append", cache->head_dim, rotation, a)) return rc;
   if (int rc = check_seqs("ppmoe_kv_append", a.seqs)) return rc;
-  if (dtype != PPMOE_BF16 && dtype != PPMOE_F16) {
-    set_error("ppmoe_kv_append: dtype=%d (0 bf16, 1 fp16)", dtype);
-    return PPMOE_ERR_UNSUPPORTED;
-  }
+  const int kv_heads = cache->kv_heads, head_dim = cache->head_dim;
   if (tokens < 0 || q_heads < 0 || (int64_t)(q_heads + 2ll * kv_heads) * head_dim > (1 << 24)) {
     set_error("ppmoe_kv_append: tokens=%d, q_heads=%d, kv_heads=%d", tokens, q_heads, kv_heads);
     return PPMOE_ERR_INVALID_ARG;
   }
   if (tokens == 0) return PPMOE_OK;
-  if (!k || !v || !status || (q_heads && (!q || !q_out))) {
+  if (!k || !v || (q_heads && (!q || !q_out))) {
     set_error("ppmoe_kv_append: null pointer");
     return PPMOE_ERR_INVALID_ARG;
   }
-  while ((1 << a.pages.page_shift) < page_size) ++a.pages.page_shift;
   a.q = {q, q_out, 0, q_t, q_h, 0, qo_t, qo_h, q_heads};
   a.k = {k, nullptr, 0, k_t, k_h, 0, 0, 0, kv_heads};
   a.v = {v, nullptr, 0, v_t, v_h, 0, 0, 0, kv_heads};
   a.batch = 1;
   a.length = a.tokens = tokens;
-  a.gain = gain;
   a.sign = 1.f;
-  a.status = static_cast<uint32_t*>(status);
-  const bool wide = rotary_dim % 16 == 0 && wide_view(k, 0, k_t, k_h, 2) && wide_view(v, 0, v_t, v_h, 2) &&
+  a.status = static_cast<uint32_t*>(cache->status);
+  const bool wide = a.pairs % 8 == 0 && wide_view(k, 0, k_t, k_h, 2) && wide_view(v, 0, v_t, v_h, 2) &&
                     (!q_heads || (wide_view(q, 0, q_t, q_h, 2) && wide_view(q_out, 0, qo_t, qo_h, 2)));
-  return launch<true>(a, interleaved != 0, dtype, wide, static_cast<cudaStream_t>(stream));
+  return launch<true>(a, rotation && rotation->interleaved, cache->dtype, wide, static_cast<cudaStream_t>(stream));
 }

@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
 }
 
 // Host-side checks common to the entry points of both files (kvcache layout and batch tables).
-int check_pages(const char* fn, const Pages& p, int page_size, int head_dim);
+int check_cache(const char* fn, const ppmoe_kv_cache* c, Pages& p);
 int check_seqs(const char* fn, const Seqs& s);
 
 }  // namespace ppmoe

@@ -11,13 +11,13 @@ sequence (padding behind ``starts[batch]``) are not read and their outputs not w
 """
 from __future__ import annotations
 
-import math
+import ctypes
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .rotary import RotaryEmbedding, _on, _stream
+from .rotary import _NONE, RotaryEmbedding, _enter, _stream
 
 __all__ = ["PagedKVCache"]
 
@@ -73,38 +73,45 @@ class PagedKVCache:
         self.k, self.v = k, v
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype, self.device = k.dtype, k.device
-        self._code = _DTYPES[k.dtype]
         self._status = torch.zeros(256, dtype=torch.uint8, device=k.device)
 
         def strides(t):  # a size of one has any stride: give it a harmless one
             return tuple(s if n > 1 else 8 for n, s in zip(t.shape[:3], t.stride()))
 
-        self._pages = (k.data_ptr(), *strides(k), v.data_ptr(), *strides(v), self.num_pages, self.page_size,
-                       self.kv_heads, self.head_dim)
+        self._c = _lib.KVCache(k.data_ptr(), v.data_ptr(), *strides(k), *strides(v), *k.shape[:1], self.page_size,
+                               self.kv_heads, self.head_dim, _DTYPES[k.dtype], self._status.data_ptr())
+        self._ptr = ctypes.addressof(self._c)
 
     # ------------------------------------------------------------------ checks
     def _rows(self, name, x, heads=None):
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
-            raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {self.head_dim}], got {list(x.shape)}")
+        """x and its strides, checked."""
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
+            raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {self.head_dim}], got {list(shape)}")
         if x.dtype is not self.dtype or x.device != self.device:
             raise ValueError(f"{name} must be {self.dtype} on {self.device}, got {x.dtype} on {x.device}")
-        return x if x.stride(2) == 1 else x.contiguous()
+        s = x.stride()
+        if s[2] != 1:
+            x = x.contiguous()
+            s = x.stride()
+        return x, s
 
     def _batch(self, starts, lengths, table):
-        for name, t, dim in (("starts", starts, 1), ("lengths", lengths, 1), ("table", table, 2)):
-            if t.dtype is not torch.int32 or t.device != self.device or t.dim() != dim:
-                raise ValueError(f"{name} must be int32 of {dim} dimension(s) on {self.device}, "
-                                 f"got {t.dtype} {list(t.shape)} on {t.device}")
-        B = lengths.shape[0]
-        if starts.shape[0] != B + 1 or table.shape[0] != B or B < 1 or table.shape[1] < 1:
-            raise ValueError(f"starts {list(starts.shape)}, lengths {list(lengths.shape)} and table {list(table.shape)} "
+        i32, dev, ts = torch.int32, self.device, table.shape
+        if (starts.dtype is not i32 or lengths.dtype is not i32 or table.dtype is not i32 or starts.device != dev
+                or lengths.device != dev or table.device != dev or len(ts) != 2):
+            raise ValueError(f"starts, lengths and table [batch, max_pages] must be int32 on {dev}, got "
+                             + ", ".join(f"{t.dtype} {list(t.shape)} on {t.device}" for t in (starts, lengths, table)))
+        B, pages = ts
+        if starts.shape != (B + 1,) or lengths.shape != (B,) or B < 1 or pages < 1:
+            raise ValueError(f"starts {list(starts.shape)}, lengths {list(lengths.shape)} and table {list(ts)} "
                              "must be [batch + 1], [batch] and [batch, max_pages]")
-        if starts.stride(0) != 1 or (B > 1 and lengths.stride(0) != 1) or (table.shape[1] > 1 and table.stride(1) != 1):
+        s = table.stride()
+        if not starts.is_contiguous() or not lengths.is_contiguous() or (pages > 1 and s[1] != 1):
             raise ValueError("starts, lengths and the rows of table must be contiguous")
-        return (starts.data_ptr(), lengths.data_ptr(), table.data_ptr(), table.stride(0), B, table.shape[1])
+        return starts.data_ptr(), lengths.data_ptr(), table.data_ptr(), s[0], B, pages
 
     # ------------------------------------------------------------------ calls
-    @torch.no_grad()
     def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
                lengths: torch.Tensor, table: torch.Tensor, *, rotary: Optional[RotaryEmbedding] = None,
                out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
@@ -113,34 +120,36 @@ class PagedKVCache:
         rotated likewise: a new tensor, or ``out`` (which may be ``q``).  ``q`` None returns None.  Rows
         outside every sequence are not written, in ``out`` neither.  The rows of one call must go to
         different places.  Records no gradients."""
-        k, v = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
+        k, sk = self._rows("k", k, self.kv_heads)
+        v, sv = self._rows("v", v, self.kv_heads)
         T = k.shape[0]
         if v.shape[0] != T or (q is not None and q.shape[0] != T):
             raise ValueError("q, k and v must have the same number of rows")
         if rotary is not None and rotary.head_dim != self.head_dim:
             raise ValueError(f"rotary has head_dim={rotary.head_dim}, the cache {self.head_dim}")
         batch = self._batch(starts, lengths, table)
+        Hq, qp, op, sq, so = 0, None, None, _NONE, _NONE
         if q is not None:
-            q = self._rows("q", q)
+            q, sq = self._rows("q", q)
+            Hq = q.shape[1]
             if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                so = (Hq * self.head_dim, self.head_dim)
             else:
-                self._out(out, q)
+                so = self._out(out, q)
+            qp, op = q.data_ptr(), out.data_ptr()
         elif out is not None:
             raise ValueError("out without q")
-        qa = (None, 0, 0, None, 0, 0, 0) if q is None else (
-            q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), q.shape[1])
-        rot = (0, 0, None, 1.0) if rotary is None else (
-            rotary.rotary_dim, rotary.layout == "interleaved", rotary._turns_ptr, rotary.gain)
-        with _on(self.device):
-            rc = _lib.load().ppmoe_kv_append(
-                *qa, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), T, *self._pages,
-                *batch, *rot, self._code, self._status.data_ptr(), _stream(self.device))
+        back = _enter(self.device)
+        rc = _lib.load().ppmoe_kv_append(
+            self._ptr, None if rotary is None else rotary._ptr, qp, sq[0], sq[1], op, so[0], so[1], Hq, k.data_ptr(),
+            sk[0], sk[1], v.data_ptr(), sv[0], sv[1], T, *batch, _stream(self.device))
+        if back is not None:
+            torch.cuda.set_device(back)
         if rc:
             raise _lib.PPMoEError("ppmoe_kv_append", rc, _lib.load().ppmoe_last_error().decode())
         return out
 
-    @torch.no_grad()
     def attend(self, q: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, *,
                max_new: Optional[int] = None, max_length: Optional[int] = None, scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -150,38 +159,46 @@ class PagedKVCache:
         sequence are not written.  ``max_new`` / ``max_length``: the most new rows and the greatest length of
         a sequence as far as the host knows (default: the largest possible); they choose how the work is
         laid out, never what is computed.  ``scale`` defaults to ``head_dim ** -0.5``.  Records no gradients."""
-        q = self._rows("q", q)
+        q, sq = self._rows("q", q)
         T, Hq, D = q.shape
         if Hq < 1 or Hq % self.kv_heads:
             raise ValueError(f"q has {Hq} heads: not a multiple of the cache's {self.kv_heads}")
         batch = self._batch(starts, lengths, table)
-        B, cap = batch[4], batch[5] * self.page_size
+        cap = batch[5] * self.page_size
         new = T if max_new is None else max(1, min(int(max_new), T))
         length = cap if max_length is None else max(1, min(int(max_length), cap))
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            so = (Hq * D, D)
         else:
-            self._out(out, q)
+            so = self._out(out, q)
         lib = _lib.load()
-        with _on(self.device):
-            n = lib.ppmoe_attend_workspace_bytes(T, Hq, self.kv_heads, D, B, new, length)
-            ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-            rc = lib.ppmoe_attend(
-                q.data_ptr(), q.stride(0), q.stride(1), Hq, T, *self._pages, *batch,
-                D ** -0.5 if scale is None else float(scale), new, length, out.data_ptr(), out.stride(0), out.stride(1),
-                self._code, self._status.data_ptr(), _lib.ptr(ws), n, _stream(self.device))
+        back = _enter(self.device)
+        n = lib.ppmoe_attend_workspace_bytes(T, Hq, self.kv_heads, D, batch[4], new, length)
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        rc = lib.ppmoe_attend(self._ptr, q.data_ptr(), sq[0], sq[1], Hq, T, *batch, D ** -0.5 if scale is None else scale,
+                              new, length, out.data_ptr(), so[0], so[1], None if ws is None else ws.data_ptr(), n,
+                              _stream(self.device))
+        if back is not None:
+            torch.cuda.set_device(back)
         if rc:
             raise _lib.PPMoEError("ppmoe_attend", rc, lib.ppmoe_last_error().decode())
         return out
 
     def _out(self, out, q):
-        if out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or (out.numel() and out.stride(2) != 1):
+        s = out.stride()
+        if out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or (out.numel() and s[2] != 1):
             raise ValueError(f"out must be {list(q.shape)} {q.dtype} on {q.device} with contiguous heads")
-        if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        if any(n > 1 and x == 0 for n, x in zip(out.shape, s)):
             raise ValueError("out repeats elements")
+        return s
 
     def check_device_status(self) -> None:
         """Synchronise and raise if a call met a position without a page (its row was not stored, or what
         it gave is not defined); clears the status."""
-        with _on(self.device):
+        back = _enter(self.device)
+        try:
             _lib.call("ppmoe_workspace_status", self._status.data_ptr(), _stream(self.device))
+        finally:
+            if back is not None:
+                torch.cuda.set_device(back)

@@ -24,20 +24,16 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-class _on:
-    """Makes ``device`` current for a launch where it is not (a launch goes to the current device)."""
+_NONE = (0, 0, 0, 0)
 
-    def __init__(self, device: torch.device):
-        self.device = device
 
-    def __enter__(self):
-        self.back = torch.cuda.current_device()
-        if self.back != self.device.index:
-            torch.cuda.set_device(self.device)
-
-    def __exit__(self, *exc):
-        if self.back != self.device.index:
-            torch.cuda.set_device(self.back)
+def _enter(device: torch.device):
+    """Makes ``device`` current (a launch goes to the current device); the device to go back to, or None."""
+    now = torch.cuda.current_device()
+    if now == device.index:
+        return None
+    torch.cuda.set_device(device)
+    return now
 
 
 class _Rotate(torch.autograd.Function):
@@ -127,8 +123,9 @@ class RotaryEmbedding:
         if sc:
             raise ValueError(f"unknown scaling entries {sorted(sc)}")
         self.turns = freq / (2.0 * math.pi)
-        self._turns_c = (ctypes.c_double * (rotary_dim // 2))(*self.turns.tolist())
-        self._turns_ptr = ctypes.addressof(self._turns_c)
+        self._c = _lib.Rotation(rotary_dim, layout == "interleaved", self.gain)
+        self._c.turns[:rotary_dim // 2] = self.turns.tolist()
+        self._ptr = ctypes.addressof(self._c)
 
     # ------------------------------------------------------------------ calls
     def __call__(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor
@@ -152,49 +149,60 @@ class RotaryEmbedding:
         self._launch(q, k, positions, False, (q, k))
 
     def _launch(self, q, k, positions, inverse, out=None):
-        dev = q.device
+        dev, shape, dt = q.device, q.shape, q.dtype
         if dev.type != "cuda":
             raise RuntimeError("RotaryEmbedding runs on CUDA only; got a tensor on " + str(dev))
-        shape = q.shape
-        if len(shape) not in (3, 4) or shape[-1] != self.head_dim:
+        n = len(shape)
+        if n not in (3, 4) or shape[-1] != self.head_dim:
             raise ValueError(f"q must be [(batch,) tokens, heads, {self.head_dim}], got {list(shape)}")
-        code = _DTYPES.get(q.dtype)
+        code = _DTYPES.get(dt)
         if code is None:
-            raise TypeError(f"RotaryEmbedding takes bf16, fp16 or fp32, got {q.dtype}")
-        if k is not None and (k.dtype != q.dtype or k.device != dev or k.shape[:-2] != shape[:-2]
-                              or k.shape[-1] != self.head_dim):
-            raise ValueError(f"k {list(k.shape)} {k.dtype} on {k.device} does not go with q {list(shape)} {q.dtype} on {dev}")
+            raise TypeError(f"RotaryEmbedding takes bf16, fp16 or fp32, got {dt}")
+        if k is not None:
+            ks = k.shape
+            if k.dtype is not dt or k.device != dev or ks[:-2] != shape[:-2] or ks[-1] != self.head_dim:
+                raise ValueError(f"k {list(ks)} {k.dtype} on {k.device} does not go with q {list(shape)} {dt} on {dev}")
         if positions.device != dev or positions.dtype not in (torch.int64, torch.int32):
             raise ValueError(f"positions must be int64 or int32 on {dev}, got {positions.dtype} on {positions.device}")
         if positions.shape != shape[:-2] and positions.shape != shape[-3:-2]:
             raise ValueError(f"positions {list(positions.shape)} do not go with q {list(shape)}")
-        if q.stride(-1) != 1:
+        sq = q.stride()
+        if sq[-1] != 1:
             q = q.contiguous()
-        if k is not None and k.stride(-1) != 1:
-            k = k.contiguous()
+            sq = q.stride()
+        B, L, Hq = (shape[0] if n == 4 else 1), shape[-3], shape[-2]
+        sk, Hk, k2, sk2 = _NONE, 0, None, _NONE
+        if k is not None:
+            sk, Hk = k.stride(), ks[-2]
+            if sk[-1] != 1:
+                k = k.contiguous()
+                sk = k.stride()
         if out is None:
-            q2 = torch.empty(shape, dtype=q.dtype, device=dev)
-            k2 = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+            q2 = torch.empty_like(q, memory_format=torch.contiguous_format)
+            sq2 = (L * Hq * self.head_dim, Hq * self.head_dim, self.head_dim, 1)
+            if k is not None:
+                k2 = torch.empty_like(k, memory_format=torch.contiguous_format)
+                sk2 = (L * Hk * self.head_dim, Hk * self.head_dim, self.head_dim, 1)
         else:
             q2, k2 = out
+            sq2 = sq if n == 4 else (0, *sq)
+            if k2 is not None:
+                sk2 = sk if n == 4 else (0, *sk)
             if q2.data_ptr() != q.data_ptr() or (k is not None and k2.data_ptr() != k.data_ptr()):
                 raise ValueError("rotate_ needs contiguous heads")
-        four = len(shape) == 4
-        B, L, Hq = (shape[0] if four else 1), shape[-3], shape[-2]
-
-        def strides(t):
-            if t is None:
-                return 0, 0, 0
-            s = t.stride()
-            return (s[0], s[1], s[2]) if four else (0, s[0], s[1])
-
+        if n == 3:
+            sq = (0, *sq)
+            if k is not None:
+                sk = (0, *sk)
         pb, pt = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
-        with _on(dev):
-            rc = _lib.load().ppmoe_rotary(
-                q.data_ptr(), *strides(q), q2.data_ptr(), *strides(q2), Hq,
-                _lib.ptr(k), *strides(k), _lib.ptr(k2), *strides(k2), 0 if k is None else k.shape[-2],
-                B, L, self.head_dim, self.rotary_dim, self.layout == "interleaved", self._turns_ptr, self.gain,
-                inverse, positions.data_ptr(), positions.dtype is torch.int64, pb, pt, code, _stream(dev))
+        back = _enter(dev)
+        rc = _lib.load().ppmoe_rotary(
+            self._ptr, inverse, q.data_ptr(), sq[0], sq[1], sq[2], q2.data_ptr(), sq2[0], sq2[1], sq2[2], Hq,
+            None if k is None else k.data_ptr(), sk[0], sk[1], sk[2], None if k is None else k2.data_ptr(),
+            sk2[0], sk2[1], sk2[2], Hk, B, L, self.head_dim, positions.data_ptr(),
+            positions.dtype is torch.int64, pb, pt, code, _stream(dev))
+        if back is not None:
+            torch.cuda.set_device(back)
         if rc:
             raise _lib.PPMoEError("ppmoe_rotary", rc, _lib.load().ppmoe_last_error().decode())
         return q2, k2

@@ -1,4 +1,5 @@
 """Paged key/value cache: append and attention against fp64, alone and as a decoder uses them; refusals."""
+import ctypes
 import math
 
 import pytest
@@ -34,25 +35,37 @@ def test_constructor_refusals():
 def test_host_validation_without_gpu():
     lib = pkg()._lib.load()
 
-    def append(tokens=1, page=16, dim=64, num=4, kvh=2, kp=1024, batch=1, mp=4, rot=0, dtype=0, k=16, status=256, starts=16):
-        return lib.ppmoe_kv_append(None, 0, 0, None, 0, 0, 0, k, 128, 64, 16, 128, 64, tokens, kp, 2048, 1024, 64, 1024, 2048,
-                                   1024, 64, num, page, kvh, dim, starts, 16, 16, mp, batch, mp, rot, 0, None, 1.0, dtype,
-                                   status, None)
+    def cache(page=16, dim=64, num=4, kvh=2, k=1024, dtype=0, status=256):
+        return ctypes.byref(pkg()._lib.KVCache(k, 1024, 2048, 1024, 64, 2048, 1024, 64, num, page, kvh, dim, dtype, status))
 
-    assert append(tokens=0) == 0
-    assert append(page=8) == -2 and append(page=24) == -2 and append(page=512) == -2 and append(dim=96) == -2
-    assert append(num=0) == -1 and append(kvh=0) == -1 and append(kp=1032) == -1 and append(kp=None) == -1
-    assert append(batch=0) == -1 and append(mp=0) == -1 and append(starts=None) == -1
-    assert append(rot=64) == -1 and append(rot=3) == -2 and append(dtype=2) == -2
-    assert append(k=None) == -1 and append(status=None) == -1 and append(tokens=-1) == -1
+    rotation = pkg()._lib.Rotation(64, 0, 1.0)
 
-    def attend(tokens=1, hq=4, page=16, dim=64, kvh=2, dtype=0, q=16, ws=None, n=0, batch=1, new=1, length=64, q_t=256):
-        return lib.ppmoe_attend(q, q_t, 64, hq, tokens, 1024, 2048, 1024, 64, 1024, 2048, 1024, 64, 4, page, kvh, dim, 16, 16,
-                                16, 4, batch, 4, 0.125, new, length, 16, 256, 64, dtype, 256, ws, n, None)
+    def append(tokens=1, batch=1, mp=4, rot=None, k=16, starts=16, null=False, **c):
+        rotation.rotary_dim = rot or 0
+        return lib.ppmoe_kv_append(None if null else cache(**c), None if rot is None else ctypes.byref(rotation), None, 0, 0, None,
+                                   0, 0, 0, k, 128, 64, 16, 128, 64, tokens, starts, 16, 16, mp, batch, mp, None)
 
-    assert attend(tokens=0) == 0
-    assert attend(hq=3) == -1 and attend(hq=0) == -1 and attend(page=40) == -2 and attend(dim=32) == -2
-    assert attend(dtype=2) == -2 and attend(q=None) == -1 and attend(tokens=-1) == -1 and attend(batch=0) == -1
+    def attend(tokens=1, hq=4, q=16, batch=1, new=1, length=64, scale=0.125, ws=None, n=0, null=False, **c):
+        return lib.ppmoe_attend(None if null else cache(**c), q, 256, 64, hq, tokens, 16, 16, 16, 4, batch, 4, scale, new, length,
+                                16, 256, 64, ws, n, None)
+
+    for call in (append, attend):
+        assert call(tokens=0) == 0  # nothing to do: no launch
+        assert call(null=True) == -1 and call(page=8) == -2 and call(page=24) == -2 and call(page=512) == -2
+        assert call(dim=96) == -2 and call(dtype=2) == -2 and call(num=0) == -1 and call(kvh=0) == -1
+        assert call(k=1032) == -1 or call is append  # (append's k are the new rows)
+        assert call(status=None) == -1 and call(batch=0) == -1 and call(tokens=-1) == -1
+    assert append(mp=0) == -1 and append(starts=None) == -1 and append(k=None) == -1
+    assert append(rot=66) == -2 and append(rot=3) == -2
+    assert attend(hq=3) == -1 and attend(hq=0) == -1 and attend(q=None) == -1
+    assert attend(scale=math.inf) == -1 and attend(scale=math.nan) == -1
+    assert attend(batch=1 << 20) == -2 and attend(tokens=1 << 30) == -2
+    n = lib.ppmoe_attend_workspace_bytes(1, 4, 2, 64, 1, 1, 64 * 1024)
+    assert n > 0 and attend(length=64 * 1024) == -5 and attend(length=64 * 1024, ws=1024, n=n - 1) == -5
+    assert attend(length=64 * 1024, ws=1032, n=n) == -5 and b"workspace" in lib.ppmoe_last_error()
+    for odd in [(0, 4, 2, 64, 1, 1, 64), (1, 4, 0, 64, 1, 1, 64), (1, 1, 2, 64, 1, 1, 64), (1, 4, 2, 64, 0, 1, 64)]:
+        assert lib.ppmoe_attend_workspace_bytes(*odd) == 0
+    assert lib.ppmoe_attend_workspace_bytes(1, 4, 2, 64, 1, -5, -7) == lib.ppmoe_attend_workspace_bytes(1, 4, 2, 64, 1, 1, 1)
 
 
 # ------------------------------------------------------------------ GPU: append

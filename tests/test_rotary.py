@@ -56,13 +56,14 @@ def test_host_validation_without_gpu():
     lib = pkg()._lib.load()
     e = emb(64)
 
-    def call(heads=1, batch=1, length=2, head_dim=64, rot=64, turns=e._turns_ptr, dtype=0, q=16, pos=16):
-        return lib.ppmoe_rotary(q, 0, 64, 64, q, 0, 64, 64, heads, None, 0, 0, 0, None, 0, 0, 0, 0, batch, length,
-                                head_dim, rot, 0, turns, 1.0, 0, pos, 1, 0, 1, dtype, None)
+    def call(heads=1, batch=1, length=2, head_dim=64, rot=64, dtype=0, q=16, pos=16, ptr=None):
+        e._c.rotary_dim = rot
+        return lib.ppmoe_rotary(e._ptr if ptr is None else ptr, 0, q, 0, 64, 64, q, 0, 64, 64, heads, None, 0, 0, 0, None, 0, 0, 0,
+                                0, batch, length, head_dim, pos, 1, 0, 1, dtype, None)
 
     assert call(length=0) == 0 and call(heads=0) == 0  # nothing to do: no launch
     assert call(head_dim=63) == -2 and call(head_dim=258) == -2 and call(rot=66) == -2 and call(rot=3) == -2
-    assert call(turns=None) == -1 and call(dtype=3) == -2 and call(q=None) == -1 and call(pos=None) == -1
+    assert call(ptr=0) == -1 and call(dtype=3) == -2 and call(q=None) == -1 and call(pos=None) == -1
     assert call(batch=-1) == -1 and call(batch=2, length=2**31) == -1 and call(heads=1 << 20) == -2
     assert b"heads" in lib.ppmoe_last_error()
 
