@@ -17,20 +17,25 @@
 namespace ppmoe {
 
 // ======================================================================== few rows
-// Up to 16 rows at a time per (sequence, kv head): one token per sequence up to a few.  Bound by
-// the cache's bytes.  Each warp takes 32 keys at a time through a ring of its own (cp.async, no block
+// Up to 16 or 32 rows at a time per (sequence, kv head): one token per sequence up to a few.  Bound by
+// the cache's bytes.  Each warp takes 32 (or 16) keys at a time through a ring of its own (cp.async, no block
 // barrier), m16n8k16 products (rows padded to 16: the tensor pipe has room, it is the loads that
 // count), and the warps' and then the parts' (m, l, sum) are joined at the end.
-constexpr int kThinWarps = 4;
-constexpr int kThinKeys = 32;
-constexpr int kThinStages = 3;
+// Small CTAs, several to an SM, so that one's start and end hide behind the others' loads: 64 ragged
+// sequences of up to 8192 keys, 32 query and 8 kv heads of 128, in us: 2 warps x 2 stages (3 CTAs an SM) 196,
+// 2 x 3 (2) 220, 4 x 3 (1) 235, 1 x 2 (6) 229.
+constexpr int kThinWarps = 2;
 
-template <int D>
-struct ThinSmem {
-  static constexpr int kTile = kThinKeys * D * 2;         // bytes of K (or V) of one stage
-  static constexpr int kWarp = kThinStages * 2 * kTile;   // bytes of one warp's ring
-  static constexpr int kJoin = kThinWarps * (16 * (D + 4) + 32) * 4;
-  static constexpr int kBytes = kThinWarps * kWarp > kJoin ? kThinWarps * kWarp : kJoin;
+template <int D, int MT>  // MT: row tiles of 16
+struct ThinShape {
+  static constexpr int kKeys = MT == 2 && D == 128 ? 16 : 32;  // (registers: 128 for the sums alone)
+  static constexpr int kStages = MT == 1 && D == 128 ? 2 : 3;
+  static constexpr int kCtas = 3;  // per SM
+  static constexpr int kTile = kKeys * D * 2;          // bytes of K (or V) of one stage
+  static constexpr int kWarp = kStages * 2 * kTile;    // bytes of one warp's ring
+  static constexpr int kQ = MT == 2 ? 32 * D * 2 : 0;  // q of two row tiles (of one: registers)
+  static constexpr int kJoin = kThinWarps * MT * 16 * (D + 4 + 2) * 4;
+  static constexpr int kBytes = kQ + (kThinWarps * kWarp > kJoin ? kThinWarps * kWarp : kJoin);
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -55,10 +60,13 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T, int D>
-__global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const __grid_constant__ AttendArgs a) {
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kThinWarps * 32, ThinShape<D, MT>::kCtas)
+attend_thin_kernel(const __grid_constant__ AttendArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  using S = ThinSmem<D>;
+  using S = ThinShape<D, MT>;
+  constexpr int KEYS = S::kKeys, STAGES = S::kStages, R = 16 * MT;
+  constexpr int KN = KEYS / 8;   // n-tiles of the scores
   constexpr int KS = D / 16;     // k-steps of q.k
   constexpr int NT = D / 8;      // n-tiles of the output
   constexpr int CH = D / 8;      // 16-byte chunks of a row
@@ -76,36 +84,44 @@ __global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const _
   const int rows = sq.rows * a.group;
   const int32_t* table = a.seqs.table + b * a.seqs.table_stride;
   const int shift = a.pages.page_shift;
-  const uint32_t ring = smem_u32(smem) + warp * S::kWarp;
-  float* j_o = reinterpret_cast<float*>(smem);              // [warps][16][D + 4]
-  float* j_ml = j_o + kThinWarps * 16 * (D + 4);            // [warps][16][2]
+  const uint32_t q_s = smem_u32(smem), ring = q_s + S::kQ + warp * S::kWarp;
+  float* j_o = reinterpret_cast<float*>(smem + S::kQ);  // [warps][R][D + 4]
+  float* j_ml = j_o + kThinWarps * R * (D + 4);         // [warps][R][2]
 
-  for (int r0 = 0; r0 < rows; r0 += 16) {
-    const int last = r0 + 15 < rows ? r0 + 15 : rows - 1;
+  for (int r0 = 0; r0 < rows; r0 += R) {
+    const int last = r0 + R - 1 < rows ? r0 + R - 1 : rows - 1;
     const int pos_lo = pos0 + r0 / a.group, pos_hi = pos0 + last / a.group;
     const int keys = pos_hi + 1 < cap ? pos_hi + 1 : cap;  // keys some row sees
-    const int blocks = keys > 0 ? (keys + kThinKeys - 1) / kThinKeys : 0;
+    const int blocks = keys > 0 ? (keys + KEYS - 1) / KEYS : 0;
     const int per = (blocks + a.nsplit - 1) / a.nsplit;
     const int blk_end = min(blocks, (split + 1) * per);
     int blk = split * per + warp;
 
-    // this thread's two rows: how far they see (-1: nothing), their q fragments
-    const int ra = r0 + (lane >> 2), rb = ra + 8;
-    const int lim_a = ra < rows ? pos0 + ra / a.group : -1, lim_b = rb < rows ? pos0 + rb / a.group : -1;
-    uint32_t qf[KS][4];
-    {
-      const T* qa = nullptr;
-      const T* qb = nullptr;
-      if (ra < rows)
-        qa = static_cast<const T*>(a.q) + (int64_t)(sq.first + ra / a.group) * a.q_t + (int64_t)(kvh * a.group + ra % a.group) * a.q_h;
-      if (rb < rows)
-        qb = static_cast<const T*>(a.q) + (int64_t)(sq.first + rb / a.group) * a.q_t + (int64_t)(kvh * a.group + rb % a.group) * a.q_h;
-      auto pair = [&](const T* p, int e) -> uint32_t {
-        if (!p) return 0u;
-        if (a.q_wide) return q_pair(__ldg(reinterpret_cast<const uint32_t*>(p + e)), a.q_sign);
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(p + e);
-        return q_pair(h[0] | (uint32_t)h[1] << 16, a.q_sign);
-      };
+    // row r of this sequence and kv head in q (null past the last)
+    auto q_row = [&](int r) -> const T* {
+      if (r >= rows) return nullptr;
+      const int tok = r / a.group;
+      return static_cast<const T*>(a.q) + (int64_t)(sq.first + tok) * a.q_t + (int64_t)(kvh * a.group + r - tok * a.group) * a.q_h;
+    };
+    auto pair = [&](const T* p, int e) -> uint32_t {
+      if (!p) return 0u;
+      if (a.q_wide) return q_pair(__ldg(reinterpret_cast<const uint32_t*>(p + e)), a.q_sign);
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p + e);
+      return q_pair(h[0] | (uint32_t)h[1] << 16, a.q_sign);
+    };
+    // this thread's rows (lane / 4 and that + 8 of each tile): how far they see (-1: nothing), their q fragments
+    int lim[MT][2];
+    uint32_t qf[MT == 1 ? KS : 1][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = r0 + t * 16 + (lane >> 2) + 8 * i;
+        lim[t][i] = r < rows ? min(pos0 + r / a.group, cap - 1) : -1;
+      }
+    }
+    if constexpr (MT == 1) {
+      const T *qa = q_row(r0 + (lane >> 2)), *qb = q_row(r0 + (lane >> 2) + 8);
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int e = k * 16 + (lane & 3) * 2;
@@ -114,21 +130,38 @@ __global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const _
         qf[k][2] = pair(qa, e + 8);
         qf[k][3] = pair(qb, e + 8);
       }
+    } else {
+#pragma unroll 4
+      for (int i = tid; i < R * CH; i += kThinWarps * 32) {
+        const int row = i / CH, c = i % CH;
+        const T* p = q_row(r0 + row);
+        const uint32_t d = q_s + row * (D * 2) + ((c ^ (row & 7)) << 4);
+        if (a.q_wide16 && a.q_sign > 0) {
+          cp_async16_or_zero(d, p ? p + c * 8 : static_cast<const T*>(a.q), p != nullptr);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(d + e * 4), "r"(pair(p, c * 8 + e * 2)) : "memory");
+        }
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      __syncthreads();
     }
 
-    // pages of a block's two halves of 16 keys (one page, or two of 16 rows)
+    // pages of a block's halves of 16 keys (one page, or two of 16 rows)
     auto ids = [&](int bk, int& p0, int& p1) {
-      const int key = bk * kThinKeys;
+      const int key = bk * KEYS;
       p0 = bk < blk_end ? __ldg(table + (key >> shift)) : -1;
-      p1 = bk < blk_end && key + 16 < keys ? __ldg(table + ((key + 16) >> shift)) : -1;
+      p1 = KEYS > 16 && bk < blk_end && key + 16 < keys ? __ldg(table + ((key + 16) >> shift)) : -1;
     };
     auto fetch = [&](int bk, int stage, int p0, int p1) {
       if (bk < blk_end) {
-        const int key = bk * kThinKeys;
+        const int key = bk * KEYS;
         const uint32_t kd = ring + stage * 2 * S::kTile, vd = kd + S::kTile;
         const bool ok0 = (uint32_t)p0 < (uint32_t)a.pages.num_pages;
         const bool ok1 = (uint32_t)p1 < (uint32_t)a.pages.num_pages;
-        if (lane == 0 && (!ok0 || (!ok1 && key + 16 < keys))) atomicOr(a.status, DEVERR_PAGE);
+        if (lane == 0 && (!ok0 || (KEYS > 16 && !ok1 && key + 16 < keys))) atomicOr(a.status, DEVERR_PAGE);
         const int in = key & ((1 << shift) - 1), in1 = (key + 16) & ((1 << shift) - 1);
         const int c = lane % CH, rr = lane / CH;
         const T* kb0 = static_cast<const T*>(a.pages.k) + kvh * a.pages.k_head + c * 8;
@@ -138,7 +171,7 @@ __global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const _
         kb0 += ok0 ? p0 * a.pages.k_page + (in + rr) * a.pages.k_row : 0;
         vb0 += ok0 ? p0 * a.pages.v_page + (in + rr) * a.pages.v_row : 0;
 #pragma unroll
-        for (int i = 0; i < kThinKeys / RPI; ++i) {
+        for (int i = 0; i < KEYS / RPI; ++i) {
           const int row = i * RPI + rr;
           const bool hi = i * RPI >= 16;
           const bool real = (hi ? ok1 : ok0) && key + row < keys;
@@ -151,107 +184,126 @@ __global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const _
       cp_async_commit();
     };
 
-    float o[NT][4], m_a = -CUDART_INF_F, m_b = -CUDART_INF_F, l_a = 0.f, l_b = 0.f;
+    float o[MT][NT][4], m[MT][2], l[MT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    for (int t = 0; t < MT; ++t) {
+      m[t][0] = m[t][1] = -CUDART_INF_F;
+      l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
+    }
 
     int p0, p1;
 #pragma unroll
-    for (int s = 0; s < kThinStages - 1; ++s) {
+    for (int s = 0; s < STAGES - 1; ++s) {
       ids(blk + s * kThinWarps, p0, p1);
       fetch(blk + s * kThinWarps, s, p0, p1);
     }
-    ids(blk + (kThinStages - 1) * kThinWarps, p0, p1);
+    ids(blk + (STAGES - 1) * kThinWarps, p0, p1);
     int stage = 0;
 #pragma unroll 1
     for (; blk < blk_end; blk += kThinWarps) {
       {
-        const int ahead = blk + (kThinStages - 1) * kThinWarps;
-        int st = stage + kThinStages - 1;
-        if (st >= kThinStages) st -= kThinStages;
+        const int ahead = blk + (STAGES - 1) * kThinWarps;
+        int st = stage + STAGES - 1;
+        if (st >= STAGES) st -= STAGES;
         fetch(ahead, st, p0, p1);
         ids(ahead + kThinWarps, p0, p1);
       }
-      cp_async_wait<kThinStages - 1>();
+      cp_async_wait<STAGES - 1>();
       __syncwarp();
       const uint32_t kd = ring + stage * 2 * S::kTile, vd = kd + S::kTile;
-      const int key = blk * kThinKeys;
+      const int key = blk * KEYS;
 
-      float s[4][4];
+      float s[MT][KN][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int n = 0; n < KN; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.f;
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
+        uint32_t qk[MT][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int t = 0; t < MT; ++t) {
+          if constexpr (MT == 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qk[t][e] = qf[k][e];
+          } else {
+            const int row = t * 16 + (lane & 15), ch = k * 2 + (lane >> 4);
+            ldsm4(qk[t], q_s + row * (D * 2) + ((ch ^ (row & 7)) << 4));
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < KN / 2; ++h) {
           // matrices: keys h*16 + 0..7 (two k halves), then keys + 8
           const int row = h * 16 + (lane & 7) + ((lane >> 4) << 3);
           const int ch = k * 2 + ((lane >> 3) & 1);
           uint32_t f[4];
           ldsm4(f, kd + row * (D * 2) + ((ch ^ (row & 7)) << 4));
-          mma16<T>(s[2 * h], qf[k], f[0], f[1]);
-          mma16<T>(s[2 * h + 1], qf[k], f[2], f[3]);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            mma16<T>(s[t][2 * h], qk[t], f[0], f[1]);
+            mma16<T>(s[t][2 * h + 1], qk[t], f[2], f[3]);
+          }
         }
       }
-      const bool partly = key + kThinKeys > pos_lo + 1 || key + kThinKeys > keys;
-      float mx_a = m_a, mx_b = m_b;
+      const bool partly = key + KEYS > pos_lo + 1 || key + KEYS > keys;
+      uint32_t pf[MT][KN / 2][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+      for (int t = 0; t < MT; ++t) {
+        float mx[2] = {m[t][0], m[t][1]};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] *= a.c;
-        if (partly) {
-          const int j = key + n * 8 + (lane & 3) * 2;
-          if (j > lim_a || j >= cap) s[n][0] = -CUDART_INF_F;
-          if (j + 1 > lim_a || j + 1 >= cap) s[n][1] = -CUDART_INF_F;
-          if (j > lim_b || j >= cap) s[n][2] = -CUDART_INF_F;
-          if (j + 1 > lim_b || j + 1 >= cap) s[n][3] = -CUDART_INF_F;
+        for (int n = 0; n < KN; ++n) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[t][n][i] *= a.c;
+            if (partly && key + n * 8 + (lane & 3) * 2 + (i & 1) > lim[t][i >> 1]) s[t][n][i] = -CUDART_INF_F;
+            mx[i >> 1] = fmaxf(mx[i >> 1], s[t][n][i]);
+          }
         }
-        mx_a = fmaxf(mx_a, fmaxf(s[n][0], s[n][1]));
-        mx_b = fmaxf(mx_b, fmaxf(s[n][2], s[n][3]));
-      }
 #pragma unroll
-      for (int x = 1; x < 4; x <<= 1) {
-        mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, x));
-        mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, x));
-      }
-      if (__any_sync(0xffffffffu, mx_a > m_a || mx_b > m_b)) {
-        // old sums to the new maxima (a row without keys so far has sums of 0)
-        const float f_a = m_a == -CUDART_INF_F ? 0.f : exp2_ftz(m_a - mx_a);
-        const float f_b = m_b == -CUDART_INF_F ? 0.f : exp2_ftz(m_b - mx_b);
-        l_a *= f_a;
-        l_b *= f_b;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          o[n][0] *= f_a;
-          o[n][1] *= f_a;
-          o[n][2] *= f_b;
-          o[n][3] *= f_b;
+        for (int x = 1; x < 4; x <<= 1) {
+          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], x));
+          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], x));
         }
-        m_a = mx_a;
-        m_b = mx_b;
-      }
-      const float sub_a = (m_a == -CUDART_INF_F ? 0.f : m_a) - kLift<T>;
-      const float sub_b = (m_b == -CUDART_INF_F ? 0.f : m_b) - kLift<T>;
-      uint32_t pf[2][4];
+        if (__any_sync(0xffffffffu, mx[0] > m[t][0] || mx[1] > m[t][1])) {
+          // old sums to the new maxima (a row without keys so far has sums of 0)
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float e0 = exp2_ftz(s[n][0] - sub_a), e1 = exp2_ftz(s[n][1] - sub_a);
-        const float e2 = exp2_ftz(s[n][2] - sub_b), e3 = exp2_ftz(s[n][3] - sub_b);
-        l_a += e0 + e1;
-        l_b += e2 + e3;
-        pf[n >> 1][(n & 1) * 2] = pack2<T>(e0, e1);
-        pf[n >> 1][(n & 1) * 2 + 1] = pack2<T>(e2, e3);
+          for (int i = 0; i < 2; ++i) {
+            const float f = m[t][i] == -CUDART_INF_F ? 0.f : exp2_ftz(m[t][i] - mx[i]);
+            l[t][i] *= f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              o[t][n][2 * i] *= f;
+              o[t][n][2 * i + 1] *= f;
+            }
+            m[t][i] = mx[i];
+          }
+        }
+        const float sub[2] = {(m[t][0] == -CUDART_INF_F ? 0.f : m[t][0]) - kLift<T>,
+                              (m[t][1] == -CUDART_INF_F ? 0.f : m[t][1]) - kLift<T>};
+#pragma unroll
+        for (int n = 0; n < KN; ++n) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float e0 = exp2_ftz(s[t][n][2 * i] - sub[i]), e1 = exp2_ftz(s[t][n][2 * i + 1] - sub[i]);
+            l[t][i] += e0 + e1;
+            pf[t][n >> 1][(n & 1) * 2 + i] = pack2<T>(e0, e1);
+          }
+        }
       }
       if (partly) {  // values that are not finite, of keys that some row does not see
-        bool bad = false;
+        uint32_t bad = 0;
 #pragma unroll 4
-        for (int i = lane; i < kThinKeys * D / 2; i += 32) {
-          uint32_t v;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(vd + i * 4) : "memory");
-          bad |= not_finite2<T>(v) != 0;
+        for (int i = lane; i < KEYS * CH; i += 32) {
+          uint4 v;
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(vd + i * 16) : "memory");
+          bad |= not_finite2<T>(v.x) | not_finite2<T>(v.y) | not_finite2<T>(v.z) | not_finite2<T>(v.w);
         }
-        if (__any_sync(0xffffffffu, bad)) {
-          for (int j = 0; j < kThinKeys; ++j) {
+        if (__any_sync(0xffffffffu, bad != 0)) {
+#pragma unroll 1
+          for (int j = 0; j < KEYS; ++j) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint32_t at = vd + j * (D * 2) + ((n ^ (j & 7)) << 4) + (lane & 3) * 4;
@@ -264,8 +316,11 @@ __global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const _
                 const uint16_t bits = (uint16_t)(v >> (16 * e));
                 if (not_finite16<T>(bits)) {
                   const float f = to_f32<T>(*reinterpret_cast<const T*>(&bits));
-                  if (key + j <= lim_a) o[n][e] += f;
-                  if (key + j <= lim_b) o[n][2 + e] += f;
+#pragma unroll
+                  for (int t = 0; t < MT; ++t) {
+                    if (key + j <= lim[t][0]) o[t][n][e] += f;
+                    if (key + j <= lim[t][1]) o[t][n][2 + e] += f;
+                  }
                   keep &= e ? 0xffffu : 0xffff0000u;
                 }
               }
@@ -276,74 +331,75 @@ __global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const _
         }
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < KN / 2; ++h) {
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
           // matrices: keys h*16 + 0..7 and + 8 of columns n, then of columns n + 1
           const int row = h * 16 + (lane & 15), ch = n + (lane >> 4);
           uint32_t f[4];
           ldsm4_t(f, vd + row * (D * 2) + ((ch ^ (row & 7)) << 4));
-          mma16<T>(o[n], pf[h], f[0], f[1]);
-          mma16<T>(o[n + 1], pf[h], f[2], f[3]);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            mma16<T>(o[t][n], pf[t][h], f[0], f[1]);
+            mma16<T>(o[t][n + 1], pf[t][h], f[2], f[3]);
+          }
         }
       }
       __syncwarp();
-      stage = stage + 1 == kThinStages ? 0 : stage + 1;
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
     cp_async_wait<0>();
-#pragma unroll
-    for (int x = 1; x < 4; x <<= 1) {
-      l_a += __shfl_xor_sync(0xffffffffu, l_a, x);
-      l_b += __shfl_xor_sync(0xffffffffu, l_b, x);
-    }
     __syncthreads();  // every warp is through with its ring
-    {
-      float* oa = j_o + (warp * 16 + (lane >> 2)) * (D + 4) + (lane & 3) * 2;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        *reinterpret_cast<float2*>(oa + n * 8) = make_float2(o[n][0], o[n][1]);
-        *reinterpret_cast<float2*>(oa + 8 * (D + 4) + n * 8) = make_float2(o[n][2], o[n][3]);
-      }
-      if ((lane & 3) == 0) {
-        float* ml = j_ml + (warp * 16 + (lane >> 2)) * 2;
-        ml[0] = m_a;
-        ml[1] = l_a;
-        ml[16] = m_b;
-        ml[17] = l_b;
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float sum = l[t][i];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const int row = warp * R + t * 16 + (lane >> 2) + 8 * i;
+        float* to = j_o + row * (D + 4) + (lane & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(to + n * 8) = make_float2(o[t][n][2 * i], o[t][n][2 * i + 1]);
+        if ((lane & 3) == 0) *reinterpret_cast<float2*>(j_ml + row * 2) = make_float2(m[t][i], sum);
       }
     }
     __syncthreads();
     {
-      constexpr int C = D / 8;  // columns of one thread
-      const int row = tid >> 3, col = (tid & 7) * C, r = r0 + row;
+      constexpr int TPR = kThinWarps * 32 / R, C = D / TPR;  // threads of a row, columns of one thread
+      const int row = tid / TPR, col = (tid % TPR) * C, r = r0 + row;
       if (r < rows) {
-        float m = -CUDART_INF_F, l = 0.f, f[kThinWarps], acc[C];
+        float top = -CUDART_INF_F, sum = 0.f, f[kThinWarps];
 #pragma unroll
-        for (int w = 0; w < kThinWarps; ++w) m = fmaxf(m, j_ml[(w * 16 + row) * 2]);
+        for (int w = 0; w < kThinWarps; ++w) top = fmaxf(top, j_ml[(w * R + row) * 2]);
 #pragma unroll
         for (int w = 0; w < kThinWarps; ++w) {
-          const float mw = j_ml[(w * 16 + row) * 2];
-          f[w] = mw == -CUDART_INF_F ? 0.f : exp2_ftz(mw - m);
-          l += f[w] * j_ml[(w * 16 + row) * 2 + 1];
+          const float mw = j_ml[(w * R + row) * 2];
+          f[w] = mw == -CUDART_INF_F ? 0.f : exp2_ftz(mw - top);
+          sum += f[w] * j_ml[(w * R + row) * 2 + 1];
         }
+        const int tok = r / a.group;
+        const int64_t t = sq.first + tok;
+        const int h = kvh * a.group + r - tok * a.group;
+        const int64_t at = ((int64_t)split * a.tokens + t) * a.q_heads + h;
+        const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+#pragma unroll 1
+        for (int c = col; c < col + C; c += 8) {
+          float acc[8];
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-          acc[i] = 0.f;
+          for (int i = 0; i < 8; ++i) {
+            acc[i] = 0.f;
 #pragma unroll
-          for (int w = 0; w < kThinWarps; ++w) acc[i] += f[w] * j_o[(w * 16 + row) * (D + 4) + col + i];
+            for (int w = 0; w < kThinWarps; ++w) acc[i] += f[w] * j_o[(w * R + row) * (D + 4) + c + i];
+          }
+          if (a.nsplit == 1) {
+            store_row<T, 8>(static_cast<T*>(a.out) + t * a.o_t + h * a.o_h + c, acc, inv, a.o_wide);
+          } else {
+            *reinterpret_cast<float4*>(a.part_o + at * D + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            *reinterpret_cast<float4*>(a.part_o + at * D + c + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+          }
         }
-        const int64_t t = sq.first + r / a.group;
-        const int h = kvh * a.group + r % a.group;
-        if (a.nsplit == 1) {
-          store_row<T, C>(static_cast<T*>(a.out) + t * a.o_t + h * a.o_h + col, acc, l > 0.f ? 1.f / l : l == l ? 0.f : l,
-                          a.o_wide);
-        } else {
-          const int64_t at = ((int64_t)split * a.tokens + t) * a.q_heads + h;
-#pragma unroll
-          for (int i = 0; i < C; i += 4)
-            *reinterpret_cast<float4*>(a.part_o + at * D + col + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-          if (col == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
-        }
+        if (a.nsplit > 1 && col == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, sum);
       }
     }
     __syncthreads();  // before the next rows' copies
@@ -351,38 +407,42 @@ __global__ void __launch_bounds__(kThinWarps * 32, 2) attend_thin_kernel(const _
 }
 
 // ======================================================================== joining the parts
-// One warp per (token, head): out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, in part order.
+// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s: a CTA per (token, head), its warps taking the parts in
+// turn and meeting in warp order, so the order of every sum is fixed.
+constexpr int kJoinWarps = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int C = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int64_t items = (int64_t)a.tokens * a.q_heads;
-  if (item >= items) return;
-  const int t = (int)(item / a.q_heads), h = (int)(item % a.q_heads);
+  __shared__ float s_o[kJoinWarps][D], s_l[kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t item = blockIdx.x, items = gridDim.x;
+  const int t = (int)(item / a.q_heads), h = (int)(item - (int64_t)t * a.q_heads);
   const int first = a.seqs.starts[0], end = a.seqs.starts[a.seqs.batch];
   pdl_wait();  // the parts are complete and visible
   if (t < first || t >= end) return;
-  float m = -CUDART_INF_F;
-  for (int s = lane; s < a.nsplit; s += 32) m = fmaxf(m, a.part_ml[(s * items + item) * 2]);
+  float m = -CUDART_INF_F, mine[4], ls[4];  // this lane's parts: lane, lane + 32, ... (128 at most)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = lane + 32 * i;
+    const float2 v = s < a.nsplit ? *reinterpret_cast<const float2*>(a.part_ml + (s * items + item) * 2)
+                                  : make_float2(-CUDART_INF_F, 0.f);
+    mine[i] = v.x;
+    ls[i] = v.y;
+    m = fmaxf(m, v.x);
+  }
   m = warp_max(m);
   float l = 0.f, acc[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) acc[i] = 0.f;
-  for (int s0 = 0; s0 < a.nsplit; s0 += 32) {
-    float ms = -CUDART_INF_F, ls = 0.f;
-    if (s0 + lane < a.nsplit) {
-      const float2 v = *reinterpret_cast<const float2*>(a.part_ml + ((s0 + lane) * items + item) * 2);
-      ms = v.x;
-      ls = v.y;
-    }
-    const float fs = ms == -CUDART_INF_F ? 0.f : exp2_ftz(ms - m);
-    const int n = min(32, a.nsplit - s0);
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float f = __shfl_sync(0xffffffffu, fs, s), ll = __shfl_sync(0xffffffffu, ls, s);
-      l += f * ll;
-      const float* p = a.part_o + ((s0 + s) * items + item) * D + lane * C;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    mine[i] = mine[i] == -CUDART_INF_F ? 0.f : exp2_ftz(mine[i] - m);  // the part's factor
+    const int n = min(32, a.nsplit - 32 * i);
+#pragma unroll 4
+    for (int s = warp; s < n; s += kJoinWarps) {
+      const float f = __shfl_sync(0xffffffffu, mine[i], s);
+      l += f * __shfl_sync(0xffffffffu, ls[i], s);
+      const float* p = a.part_o + ((s + 32 * i) * items + item) * D + lane * C;
       if constexpr (C == 4) {
         const float4 v = *reinterpret_cast<const float4*>(p);
         acc[0] += f * v.x;
@@ -396,16 +456,27 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant_
       }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
-  T* out = static_cast<T*>(a.out) + t * a.o_t + h * a.o_h + lane * C;
 #pragma unroll
-  for (int i = 0; i < C; ++i) out[i] = from_f32<T>(acc[i] * inv);
+  for (int i = 0; i < C; ++i) s_o[warp][lane * C + i] = acc[i];
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) l += s_l[w];
+  const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
+  T* out = static_cast<T*>(a.out) + t * a.o_t + h * a.o_h;
+  for (int c = threadIdx.x; c < D; c += kJoinWarps * 32) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) v += s_o[w][c];
+    out[c] = from_f32<T>(v * inv);
+  }
 }
 
 // ======================================================================== host
 struct Plan {
-  int tiles;   // 0: the kernel for few rows; else 128-row tiles of a CTA (1 or 2)
-  int groups;  // CTAs' worth of row tiles of the longest sequence
+  int tiles;   // 128-row tiles of a CTA (1 or 2); 0: the kernel for few rows
+  int groups;  // CTAs' worth of row tiles of the longest sequence; few rows: 16-row tiles taken at once (1 or 2)
   int nsplit;  // parts the keys of a (sequence, kv head) are cut into
 };
 
@@ -413,10 +484,11 @@ static Plan make_plan(int q_heads, int kv_heads, int batch, int max_new, int64_t
   auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
   const int64_t rows = (int64_t)max_new * (q_heads / kv_heads), base = (int64_t)batch * kv_heads;
   Plan p;
-  if (rows <= 16) {
+  if (rows <= 32) {
     // Up to two CTAs an SM a part may be as short as 128 keys (one block of each warp): there latency
     // counts; beyond, parts of 512 keys or more, up to 1184 CTAs, so that ragged lengths even out.
-    p.tiles = p.groups = 0;
+    p.tiles = 0;
+    p.groups = rows <= 16 ? 1 : 2;
     const int64_t n1 = std::min(up(max_length, 128), up(296, base));
     const int64_t n2 = std::min(up(max_length, 512), up(1184, base));
     p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(128, std::max(n1, n2)));
@@ -436,21 +508,29 @@ static size_t plan_bytes(const Plan& p, int tokens, int q_heads, int head_dim) {
   return p.nsplit > 1 ? (size_t)p.nsplit * tokens * q_heads * (head_dim + 2) * 4 : 0;
 }
 
+template <typename T, int D, int MT>
+static int launch_thin(const AttendArgs& a, cudaStream_t st) {
+  constexpr int bytes = ThinShape<D, MT>::kBytes;
+  auto fn = attend_thin_kernel<T, D, MT>;
+  PPMOE_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  const int64_t ctas = (int64_t)a.nsplit * a.pages.kv_heads * a.seqs.batch;
+  fn<<<(unsigned)ctas, kThinWarps * 32, bytes, st>>>(a);
+  PPMOE_CHECK_CUDA(cudaGetLastError());
+  return PPMOE_OK;
+}
+
 template <typename T, int D>
 static int launch(AttendArgs& a, const Plan& p, cudaStream_t st) {
   if (p.tiles) {
     if (int rc = attend_tiles_launch(a, D, 1 << a.pages.page_shift, std::is_same<T, __half>::value, p.tiles, p.groups, st)) return rc;
   } else {
-    auto fn = attend_thin_kernel<T, D>;
-    PPMOE_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, ThinSmem<D>::kBytes));
-    const int64_t ctas = (int64_t)a.nsplit * a.pages.kv_heads * a.seqs.batch;
-    fn<<<(unsigned)ctas, kThinWarps * 32, ThinSmem<D>::kBytes, st>>>(a);
-    PPMOE_CHECK_CUDA(cudaGetLastError());
+    const int rc = p.groups == 1 ? launch_thin<T, D, 1>(a, st) : launch_thin<T, D, 2>(a, st);
+    if (rc) return rc;
   }
   if (a.nsplit > 1) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(((int64_t)a.tokens * a.q_heads + 3) / 4));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3((unsigned)((int64_t)a.tokens * a.q_heads));
+    cfg.blockDim = dim3(kJoinWarps * 32);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
