@@ -33,8 +33,8 @@ struct ThinShape {
   static constexpr int kCtas = 3;  // per SM
   static constexpr int kTile = kKeys * D * 2;          // bytes of K (or V) of one stage
   static constexpr int kWarp = kStages * 2 * kTile;    // bytes of one warp's ring
-  static constexpr int kQ = MT == 2 ? 32 * D * 2 : 0;  // q of two row tiles (of one: registers)
-  static constexpr int kJoin = kThinWarps * MT * 16 * (D + 4 + 2) * 4;
+  static constexpr int kQ = MT * 16 * D * 2;
+  static constexpr int kJoin = (kThinWarps * (D + 4 + 2) + 2) * MT * 16 * 4;
   static constexpr int kBytes = kQ + (kThinWarps * kWarp > kJoin ? kThinWarps * kWarp : kJoin);
 };
 
@@ -60,6 +60,23 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Parts of a (sequence, kv head) that are one cluster (2 to 8) meet in shared memory: no workspace, no
+// second launch.
+constexpr int kMaxCluster = 8;
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kThinWarps * 32, ThinShape<D, MT>::kCtas)
 attend_thin_kernel(const __grid_constant__ AttendArgs a) {
@@ -87,6 +104,7 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
   const uint32_t q_s = smem_u32(smem), ring = q_s + S::kQ + warp * S::kWarp;
   float* j_o = reinterpret_cast<float*>(smem + S::kQ);  // [warps][R][D + 4]
   float* j_ml = j_o + kThinWarps * R * (D + 4);         // [warps][R][2]
+  float* c_ml = j_ml + kThinWarps * R * 2;              // [R][2]: of all warps, for the cluster
 
   for (int r0 = 0; r0 < rows; r0 += R) {
     const int last = r0 + R - 1 < rows ? r0 + R - 1 : rows - 1;
@@ -97,21 +115,8 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
     const int blk_end = min(blocks, (split + 1) * per);
     int blk = split * per + warp;
 
-    // row r of this sequence and kv head in q (null past the last)
-    auto q_row = [&](int r) -> const T* {
-      if (r >= rows) return nullptr;
-      const int tok = r / a.group;
-      return static_cast<const T*>(a.q) + (int64_t)(sq.first + tok) * a.q_t + (int64_t)(kvh * a.group + r - tok * a.group) * a.q_h;
-    };
-    auto pair = [&](const T* p, int e) -> uint32_t {
-      if (!p) return 0u;
-      if (a.q_wide) return q_pair(__ldg(reinterpret_cast<const uint32_t*>(p + e)), a.q_sign);
-      const uint16_t* h = reinterpret_cast<const uint16_t*>(p + e);
-      return q_pair(h[0] | (uint32_t)h[1] << 16, a.q_sign);
-    };
-    // this thread's rows (lane / 4 and that + 8 of each tile): how far they see (-1: nothing), their q fragments
+    // this thread's rows (lane / 4 and that + 8 of each tile): how far they see (-1: nothing)
     int lim[MT][2];
-    uint32_t qf[MT == 1 ? KS : 1][4];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
 #pragma unroll
@@ -120,34 +125,27 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
         lim[t][i] = r < rows ? min(pos0 + r / a.group, cap - 1) : -1;
       }
     }
-    if constexpr (MT == 1) {
-      const T *qa = q_row(r0 + (lane >> 2)), *qb = q_row(r0 + (lane >> 2) + 8);
+    // q to shared memory, behind the first keys' page numbers
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const int e = k * 16 + (lane & 3) * 2;
-        qf[k][0] = pair(qa, e);
-        qf[k][1] = pair(qb, e);
-        qf[k][2] = pair(qa, e + 8);
-        qf[k][3] = pair(qb, e + 8);
-      }
-    } else {
-#pragma unroll 4
-      for (int i = tid; i < R * CH; i += kThinWarps * 32) {
-        const int row = i / CH, c = i % CH;
-        const T* p = q_row(r0 + row);
-        const uint32_t d = q_s + row * (D * 2) + ((c ^ (row & 7)) << 4);
-        if (a.q_wide16 && a.q_sign > 0) {
-          cp_async16_or_zero(d, p ? p + c * 8 : static_cast<const T*>(a.q), p != nullptr);
-        } else {
+    for (int i = tid; i < R * CH; i += kThinWarps * 32) {
+      const int row = i / CH, c = i % CH, r = r0 + row, tok = r / a.group;
+      const bool real = r < rows;
+      const T* p = static_cast<const T*>(a.q);
+      if (real) p += (int64_t)(sq.first + tok) * a.q_t + (int64_t)(kvh * a.group + r - tok * a.group) * a.q_h + c * 8;
+      const uint32_t d = q_s + row * (D * 2) + ((c ^ (row & 7)) << 4);
+      if (a.q_wide16 && a.q_sign > 0) {
+        cp_async16_or_zero(d, p, real);
+      } else {
+        uint32_t v[4] = {0, 0, 0, 0};
+        if (real) {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(d + e * 4), "r"(pair(p, c * 8 + e * 2)) : "memory");
+          for (int e = 0; e < 4; ++e) v[e] = q_pair(h[2 * e] | (uint32_t)h[2 * e + 1] << 16, a.q_sign);
         }
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(d), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
       }
-      cp_async_commit();
-      cp_async_wait<0>();
-      __syncthreads();
     }
+    cp_async_commit();
 
     // pages of a block's halves of 16 keys (one page, or two of 16 rows)
     auto ids = [&](int bk, int& p0, int& p1) {
@@ -200,6 +198,17 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
       fetch(blk + s * kThinWarps, s, p0, p1);
     }
     ids(blk + (STAGES - 1) * kThinWarps, p0, p1);
+    cp_async_wait<STAGES - 1>();  // q
+    __syncthreads();
+    uint32_t qf[MT == 1 ? KS : 1][4];
+    auto load_q = [&](uint32_t (&f)[4], int t, int k) {
+      const int row = t * 16 + (lane & 15), ch = k * 2 + (lane >> 4);
+      ldsm4(f, q_s + row * (D * 2) + ((ch ^ (row & 7)) << 4));
+    };
+    if constexpr (MT == 1) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k) load_q(qf[k], 0, k);
+    }
     int stage = 0;
 #pragma unroll 1
     for (; blk < blk_end; blk += kThinWarps) {
@@ -230,8 +239,7 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) qk[t][e] = qf[k][e];
           } else {
-            const int row = t * 16 + (lane & 15), ch = k * 2 + (lane >> 4);
-            ldsm4(qk[t], q_s + row * (D * 2) + ((ch ^ (row & 7)) << 4));
+            load_q(qk[t], t, k);
           }
         }
 #pragma unroll
@@ -394,13 +402,58 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
           }
           if (a.nsplit == 1) {
             store_row<T, 8>(static_cast<T*>(a.out) + t * a.o_t + h * a.o_h + c, acc, inv, a.o_wide);
+          } else if (a.nsplit <= kMaxCluster) {  // (over what this thread alone has read)
+            *reinterpret_cast<float4*>(j_o + row * (D + 4) + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            *reinterpret_cast<float4*>(j_o + row * (D + 4) + c + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
           } else {
             *reinterpret_cast<float4*>(a.part_o + at * D + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
             *reinterpret_cast<float4*>(a.part_o + at * D + c + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
           }
         }
-        if (a.nsplit > 1 && col == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, sum);
+        if (a.nsplit > 1 && col == 0)
+          *reinterpret_cast<float2*>(a.nsplit <= kMaxCluster ? c_ml + row * 2 : a.part_ml + at * 2) = make_float2(top, sum);
       }
+    }
+    if (a.nsplit > 1 && a.nsplit <= kMaxCluster) {
+      cluster_sync();
+      const int n = min(R, rows - r0) * (D / 8);  // pieces of 8 columns, shared out over the cluster's threads
+      for (int i = tid + split * kThinWarps * 32; i < n; i += a.nsplit * kThinWarps * 32) {
+        const int row = i / (D / 8), c = i % (D / 8) * 8, r = r0 + row;
+        // (parts past the last read the last again and count nothing: all loads are in flight at once)
+        float2 ml[kMaxCluster];
+        float4 x[kMaxCluster], y[kMaxCluster];
+#pragma unroll
+        for (int w = 0; w < kMaxCluster; ++w) {
+          const int from = min(w, a.nsplit - 1);
+          ml[w] = ld_cluster2(mapa_u32(c_ml + row * 2, from));
+          const uint32_t at = mapa_u32(j_o + row * (D + 4) + c, from);
+          x[w] = ld_cluster4(at);
+          y[w] = ld_cluster4(at + 16);
+        }
+        float top = -CUDART_INF_F, sum = 0.f, acc[8] = {};
+#pragma unroll
+        for (int w = 0; w < kMaxCluster; ++w) top = fmaxf(top, ml[w].x);
+#pragma unroll
+        for (int w = 0; w < kMaxCluster; ++w) {
+          const bool real = w < a.nsplit && ml[w].x != -CUDART_INF_F;
+          const float f = real ? exp2_ftz(ml[w].x - top) : 0.f;
+          if (real) {  // (a part without keys holds sums of 0; one past the last may hold inf or NaN)
+            sum += f * ml[w].y;
+            acc[0] += f * x[w].x;
+            acc[1] += f * x[w].y;
+            acc[2] += f * x[w].z;
+            acc[3] += f * x[w].w;
+            acc[4] += f * y[w].x;
+            acc[5] += f * y[w].y;
+            acc[6] += f * y[w].z;
+            acc[7] += f * y[w].w;
+          }
+        }
+        const int tok = r / a.group;
+        store_row<T, 8>(static_cast<T*>(a.out) + (sq.first + tok) * a.o_t + (int64_t)(kvh * a.group + r - tok * a.group) * a.o_h + c,
+                        acc, sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum, a.o_wide);
+      }
+      cluster_sync();  // every part has been read
     }
     __syncthreads();  // before the next rows' copies
   }
@@ -486,11 +539,11 @@ static Plan make_plan(int q_heads, int kv_heads, int batch, int max_new, int64_t
   Plan p;
   if (rows <= 32) {
     // Up to two CTAs an SM a part may be as short as 128 keys (one block of each warp): there latency
-    // counts; beyond, parts of 512 keys or more, up to 1184 CTAs, so that ragged lengths even out.
+    // counts; beyond, parts of 768 keys or more, up to 1184 CTAs, so that ragged lengths even out.
     p.tiles = 0;
     p.groups = rows <= 16 ? 1 : 2;
     const int64_t n1 = std::min(up(max_length, 128), up(296, base));
-    const int64_t n2 = std::min(up(max_length, 512), up(1184, base));
+    const int64_t n2 = std::min(up(max_length, 768), up(1184, base));
     p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(128, std::max(n1, n2)));
   } else {
     // (A CTA goes on to further groups where there are fewer CTAs than groups: batches so wide that most
@@ -504,8 +557,11 @@ static Plan make_plan(int q_heads, int kv_heads, int batch, int max_new, int64_t
   return p;
 }
 
+// Whether parts meet by way of the workspace and a second launch.
+static bool joins(const Plan& p) { return p.nsplit > (p.tiles ? 1 : kMaxCluster); }
+
 static size_t plan_bytes(const Plan& p, int tokens, int q_heads, int head_dim) {
-  return p.nsplit > 1 ? (size_t)p.nsplit * tokens * q_heads * (head_dim + 2) * 4 : 0;
+  return joins(p) ? (size_t)p.nsplit * tokens * q_heads * (head_dim + 2) * 4 : 0;
 }
 
 template <typename T, int D, int MT>
@@ -514,8 +570,18 @@ static int launch_thin(const AttendArgs& a, cudaStream_t st) {
   auto fn = attend_thin_kernel<T, D, MT>;
   PPMOE_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   const int64_t ctas = (int64_t)a.nsplit * a.pages.kv_heads * a.seqs.batch;
-  fn<<<(unsigned)ctas, kThinWarps * 32, bytes, st>>>(a);
-  PPMOE_CHECK_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kThinWarps * 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.nsplit <= kMaxCluster ? a.nsplit : 1;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PPMOE_CHECK_CUDA(cudaLaunchKernelEx(&cfg, fn, a));
   return PPMOE_OK;
 }
 
@@ -527,7 +593,7 @@ static int launch(AttendArgs& a, const Plan& p, cudaStream_t st) {
     const int rc = p.groups == 1 ? launch_thin<T, D, 1>(a, st) : launch_thin<T, D, 2>(a, st);
     if (rc) return rc;
   }
-  if (a.nsplit > 1) {
+  if (joins(p)) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)((int64_t)a.tokens * a.q_heads));
     cfg.blockDim = dim3(kJoinWarps * 32);
