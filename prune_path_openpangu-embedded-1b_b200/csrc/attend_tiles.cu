@@ -213,17 +213,25 @@ struct Group {
   __device__ bool guarded(int block) const { return (block + 1) * KEYS > clear; }
 };
 
-// Token and head (of the group) of a row, and of the rows `step` further on, without a division each.
+// Where a row of (token, head of the group) lies in a tensor of these strides, and the rows `step` further on each
+// time, without a division for each.
 struct RowWalk {
-  int64_t tok;
-  int head, d_tok, d_head, group;
-  __device__ RowWalk(int row, int step, int g) : tok(row / g), head(row % g), d_tok(step / g), d_head(step % g), group(g) {}
+  int64_t off, inc, wrap;
+  unsigned head, d_head, group;
+  __device__ RowWalk(unsigned row, unsigned step, unsigned g, int64_t s_tok, int64_t s_head) : group(g) {
+    const unsigned tok = row / g, d_tok = step / g;
+    head = row - tok * g;
+    d_head = step - d_tok * g;
+    off = tok * s_tok + head * s_head;
+    inc = d_tok * s_tok + d_head * s_head;
+    wrap = s_tok - (int64_t)g * s_head;
+  }
   __device__ void step() {
-    tok += d_tok;
+    off += inc;
     head += d_head;
     if (head >= group) {
       head -= group;
-      ++tok;
+      off += wrap;
     }
   }
 };
@@ -263,24 +271,64 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   if (cap < sq.length && tid == 0) atomicOr(a.status, DEVERR_PAGE);
   const int pos0 = sq.length - (a.seqs.starts[b + 1] - a.seqs.starts[b]);
 
-  if (tid == 0) {
-    for (int i = 0; i < NS; ++i) {
-      mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 1);
-      mbar_init(g_full + i, 1);
-      mbar_init(v_ok + i, 2);
+  // q tile of this thread's softmax group, rows from `base`: all copies in flight at once, the first group's
+  // behind the set-up
+  constexpr int CH = D / 8, STEP = kTileRows / CH;  // 16-byte chunks of a row, rows 128 threads take at once
+  auto load_q = [&](int base) {
+    const int row = tid & 127, ch = row % CH;
+    uint8_t* q_s = smem + (warp >> 2) * S::kQ + (ch >> 3) * (kTileRows * 128);
+    RowWalk at(base + row / CH, STEP, a.group, a.q_t, a.q_h);
+    const T* q = static_cast<const T*>(a.q) + sq.first * a.q_t + (int64_t)kvh * a.group * a.q_h + ch * 8;
+    if (a.q_wide16 && a.q_sign > 0) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i, at.step()) {
+        const int rr = row / CH + i * STEP;
+        const bool real = base + rr < rows;
+        cp_async16_or_zero(smem_u32(q_s + sw128_offset(rr, ch & 7)), q + (real ? at.off : 0), real);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < CH; ++i, at.step()) {
+        const int rr = row / CH + i * STEP;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (base + rr < rows) {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(q + at.off);
+          v = make_uint4(q_pair(h[0] | (uint32_t)h[1] << 16, a.q_sign), q_pair(h[2] | (uint32_t)h[3] << 16, a.q_sign),
+                         q_pair(h[4] | (uint32_t)h[5] << 16, a.q_sign), q_pair(h[6] | (uint32_t)h[7] << 16, a.q_sign));
+        }
+        *reinterpret_cast<uint4*>(q_s + sw128_offset(rr, ch & 7)) = v;
+      }
     }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(s_full + t, 1);
-      mbar_init(p_early + t, kTileRows);
-      mbar_init(p_late + t, kTileRows);
-      mbar_init(q_full + t, kTileRows);
+    cp_async_commit();
+  };
+
+  if (warp < SW) {
+    const int base = group_of * kRows + (warp >> 2) * kTileRows;
+    if (base < rows) load_q(base);
+  } else if (warp == SW) {
+    tmem_alloc(tmem_slot, S::kTmem);
+  } else if (warp == SW + 1) {
+    if (lane == 0) {
+      for (int i = 0; i < NS; ++i) {
+        mbar_init(kv_full + i, 1);
+        mbar_init(kv_empty + i, 1);
+        mbar_init(g_full + i, 1);
+        mbar_init(v_ok + i, 2);
+      }
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(s_full + t, 1);
+        mbar_init(p_early + t, kTileRows);
+        mbar_init(p_late + t, kTileRows);
+        mbar_init(q_full + t, kTileRows);
+      }
+      *any_odd = 0;
+      fence_mbar_init();
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
     }
-    *any_odd = 0;
-    fence_mbar_init();
+  } else {
+    for (int i = tid - 32 * (SW + 2); i < 3 * D; i += 64) odd[i] = INT_MAX;
   }
-  for (int i = tid; i < 3 * D; i += S::kThreads) odd[i] = INT_MAX;
-  if (warp == SW) tmem_alloc(tmem_slot, S::kTmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -312,35 +360,8 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       const Group<TILES, KEYS> w(a, group, rows, pos0, cap, split);
       if (t < w.tiles) {
         const int base = w.r0 + t * kTileRows, r = base + row;
-        constexpr int CH = D / 8, STEP = kTileRows / CH;  // 16-byte chunks of a row, rows the 128 threads take at once
-        const int ch = row % CH;
-        {
-          uint8_t* q_s = smem + t * S::kQ + (ch >> 3) * (kTileRows * 128);
-          RowWalk at(base + row / CH, STEP, a.group);
-          const T* q = static_cast<const T*>(a.q) + sq.first * a.q_t + (int64_t)kvh * a.group * a.q_h + ch * 8;
-          if (a.q_wide16 && a.q_sign > 0) {  // all in flight at once: 1.5 us; by way of registers it took 10
-#pragma unroll
-            for (int i = 0; i < CH; ++i, at.step()) {
-              const int rr = row / CH + i * STEP;
-              const bool real = base + rr < rows;
-              cp_async16_or_zero(smem_u32(q_s + sw128_offset(rr, ch & 7)), q + (real ? at.tok * a.q_t + at.head * a.q_h : 0), real);
-            }
-            cp_async_commit();
-            cp_async_wait<0>();
-          } else {
-#pragma unroll 1
-            for (int i = 0; i < CH; ++i, at.step()) {
-              const int rr = row / CH + i * STEP;
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (base + rr < rows) {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(q + at.tok * a.q_t + at.head * a.q_h);
-                v = make_uint4(q_pair(h[0] | (uint32_t)h[1] << 16, a.q_sign), q_pair(h[2] | (uint32_t)h[3] << 16, a.q_sign),
-                               q_pair(h[4] | (uint32_t)h[5] << 16, a.q_sign), q_pair(h[6] | (uint32_t)h[7] << 16, a.q_sign));
-              }
-              *reinterpret_cast<uint4*>(q_s + sw128_offset(rr, ch & 7)) = v;
-            }
-          }
-        }
+        if (group != group_of) load_q(base);
+        cp_async_wait<0>();
         fence_proxy_async();
         mbar_arrive(q_full + t);
         const int tok = r / a.group;
@@ -450,66 +471,77 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         // parts in two halves of the columns.
         uint8_t* stage = smem + t * S::kQ;
         const int per = a.nsplit > 1 ? D / 2 : D;  // columns of one go
+        constexpr int W = D / 2;                   // ... that a thread holds at once
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += per) {
 #pragma unroll 1
-          for (int i = c0; i < c0 + per; i += 32) {
-            float o[32];
+          for (int i = c0; i < c0 + per; i += W) {
+            float o[W];
             if (count > 0) {
-              tmem_ld32_async(t_o + i, o);
+#pragma unroll
+              for (int e = 0; e < W; e += 32) tmem_ld32_async(t_o + i + e, o + e);
               tmem_ld_wait();
-              tmem_ld_bind(o);
+#pragma unroll
+              for (int e = 0; e < W; e += 32) tmem_ld_bind(o + e);
             } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = 0.f;
+              for (int e = 0; e < W; ++e) o[e] = 0.f;
             }
             if (listed) {
 #pragma unroll 1
-              for (int e = 0; e < 32; ++e) {
+              for (int e = 0; e < W; ++e) {
                 float add = 0.f;
                 if (odd[D + i + e] <= lim) add += CUDART_INF_F;
                 if (odd[2 * D + i + e] <= lim) add -= CUDART_INF_F;
                 if (odd[i + e] <= lim) add = CUDART_NAN_F;
                 if (!(add == 0.f)) {
 #pragma unroll
-                  for (int z = 0; z < 32; ++z) o[z] = z == e ? o[z] + add : o[z];
+                  for (int z = 0; z < W; ++z) o[z] = z == e ? o[z] + add : o[z];
                 }
               }
             }
             uint8_t* line = stage + row * (D * 2);
             if (a.nsplit == 1) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 8)
+              for (int e = 0; e < W; e += 8)
                 *reinterpret_cast<uint4*>(line + ((((i + e) / 8) ^ (row & 7)) << 4)) =
                     make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv),
                                pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
             } else {
 #pragma unroll
-              for (int e = 0; e < 32; e += 4)
+              for (int e = 0; e < W; e += 4)
                 *reinterpret_cast<float4*>(line + ((((i - c0 + e) / 4) ^ (row & 7)) << 4)) =
                     make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
           named_bar_sync(1 + t, kTileRows);
-          RowWalk at(base + row / CH, STEP, a.group);
-#pragma unroll 4
-          for (int i = 0; i < CH; ++i, at.step()) {
+          const int ch = row % CH;
+          const uint8_t* from = stage + (row / CH) * (D * 2);
+          auto chunk = [&](int i) {
             const int rr = row / CH + i * STEP;
-            if (base + rr >= rows) break;
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((ch ^ (rr & 7)) << 4));
-            const int64_t token = sq.first + at.tok;
-            const int h = kvh * a.group + at.head;
-            if (a.nsplit > 1) {
-              float* part = a.part_o + (((int64_t)split * a.tokens + token) * a.q_heads + h) * D;
-              *reinterpret_cast<uint4*>(part + c0 + ch * 4) = v;
+            return *reinterpret_cast<const uint4*>(from + i * STEP * (D * 2) + ((ch ^ (rr & 7)) << 4));
+          };
+          if (a.nsplit > 1) {
+            RowWalk to(base + row / CH, STEP, a.group, (int64_t)a.q_heads * D, D);
+            float* part = a.part_o + (((int64_t)split * a.tokens + sq.first) * a.q_heads + kvh * a.group) * D + c0 + ch * 4;
+#pragma unroll 4
+            for (int i = 0; i < CH; ++i, to.step())
+              if (base + row / CH + i * STEP < rows) *reinterpret_cast<uint4*>(part + to.off) = chunk(i);
+          } else {
+            RowWalk to(base + row / CH, STEP, a.group, a.o_t, a.o_h);
+            T* out = static_cast<T*>(a.out) + sq.first * a.o_t + (int64_t)kvh * a.group * a.o_h + ch * 8;
+            if (a.o_wide) {
+#pragma unroll 4
+              for (int i = 0; i < CH; ++i, to.step())
+                if (base + row / CH + i * STEP < rows) *reinterpret_cast<uint4*>(out + to.off) = chunk(i);
             } else {
-              T* out = static_cast<T*>(a.out) + token * a.o_t + h * a.o_h + ch * 8;
-              if (a.o_wide) {
-                *reinterpret_cast<uint4*>(out) = v;
-              } else {
+#pragma unroll 1
+              for (int i = 0; i < CH; ++i, to.step()) {
+                if (base + row / CH + i * STEP >= rows) continue;
+                const uint4 v = chunk(i);
                 const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(out)[e] = (uint16_t)(u[e / 2] >> (16 * (e & 1)));
+                for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(out + to.off)[e] = (uint16_t)(u[e / 2] >> (16 * (e & 1)));
               }
             }
           }
@@ -616,36 +648,45 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       for (int64_t group = group_of; group * kRows < rows; group += groups_hint) {
         const Group<TILES, KEYS> w(a, group, rows, pos0, cap, split);
         const int blocks = w.blocks();
-        const int box = lane % 8, half = lane / 8;  // lane -> box and 64-column half
+        // lane i looks up box i's page; one elected lane issues (see elect_one: 16 lanes with a box each took
+        // 2000 cycles a tile of 16-row pages)
+        constexpr int kMaxBoxes = KEYS / 16;
         auto page_id = [&](int j) {
-          const int key = (w.b0 + j) * KEYS + box * box_rows;
-          return j < blocks && box < boxes && half < D / 64 && key < w.keys ? __ldg(table + (key >> shift)) : 0;
+          const int key = (w.b0 + j) * KEYS + lane * box_rows;
+          return j < blocks && lane < boxes && key < w.keys ? __ldg(table + (key >> shift)) : 0;
         };
         int next = page_id(0);
 #pragma unroll 1
         for (int j = 0; j < blocks; ++j) {
           const int key0 = (w.b0 + j) * KEYS;
           const int here = min(boxes, (w.keys - key0 + box_rows - 1) / box_rows);  // boxes with keys
-          const bool mine = box < here && half < D / 64;
           int page = next;
           next = page_id(j + 1);
-          if (mine && (uint32_t)page >= (uint32_t)a.pages.num_pages) {
+          if (lane < here && (uint32_t)page >= (uint32_t)a.pages.num_pages) {
             atomicOr(a.status, DEVERR_PAGE);
             page = a.pages.num_pages;  // out of bounds: filled with zeros
           }
-          const int in_page = (key0 + box * box_rows) & ((1 << shift) - 1);
+          int pages[kMaxBoxes];
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            const int i = loads + 2 * j + kv, st = i % NS;
-            wait_bar(kv_empty + st, ((i / NS) & 1) ^ 1, a.status);
-            uint64_t* full = (kv && w.guarded(w.b0 + j) ? g_full : kv_full) + st;
-            if (lane == 0) mbar_arrive_expect_tx(full, here * box_rows * 128 * (D / 64));
-            __syncwarp();
-            if (mine)
-              tma_load_4d(ring + st * S::kStage + half * (KEYS * 128) + box * box_rows * 128, kv ? &map_v : &map_k,
-                          half * 64, in_page, kvh, page, full);
-            __syncwarp();
+          for (int i = 0; i < kMaxBoxes; ++i) pages[i] = __shfl_sync(0xffffffffu, page, i);
+          const int in_page = key0 & ((1 << shift) - 1);  // (not 0 only where a page holds more than a block)
+          if (elect_one()) {
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+              const int i = loads + 2 * j + kv, st = i % NS;
+              wait_bar(kv_empty + st, ((i / NS) & 1) ^ 1, a.status);
+              uint64_t* full = (kv && w.guarded(w.b0 + j) ? g_full : kv_full) + st;
+              mbar_arrive_expect_tx(full, here * box_rows * 128 * (D / 64));
+              uint32_t to = ring + st * S::kStage;
+#pragma unroll
+              for (int bx = 0; bx < kMaxBoxes; ++bx, to += box_rows * 128) {
+                if (bx >= here) break;
+                tma_load_4d(to, kv ? &map_v : &map_k, 0, in_page, kvh, pages[bx], full);
+                if constexpr (D == 128) tma_load_4d(to + KEYS * 128, kv ? &map_v : &map_k, 64, in_page, kvh, pages[bx], full);
+              }
+            }
           }
+          __syncwarp();
         }
         // every tile has been read before the CTA may end
         const int n = 2 * blocks;
@@ -671,7 +712,6 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           ph_v ^= 1u << vs;
           uint8_t* v = smem + TILES * S::kQ + vs * S::kStage;
           const int key0 = block * KEYS, here = min(KEYS, w.keys - key0);
-          constexpr int CH = D / 8;
           uint32_t bad = 0;
 #pragma unroll 8
           for (int i = g; i < KEYS * CH; i += 64) {  // 16-byte chunk i of the tile, as it lies
