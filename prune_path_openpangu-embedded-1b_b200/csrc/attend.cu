@@ -533,7 +533,7 @@ struct Plan {
   int nsplit;  // parts the keys of a (sequence, kv head) are cut into
 };
 
-static Plan make_plan(int q_heads, int kv_heads, int batch, int max_new, int64_t max_length) {
+static Plan make_plan(int tokens, int q_heads, int kv_heads, int head_dim, int batch, int max_new, int64_t max_length) {
   auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
   const int64_t rows = (int64_t)max_new * (q_heads / kv_heads), base = (int64_t)batch * kv_heads;
   Plan p;
@@ -548,11 +548,25 @@ static Plan make_plan(int q_heads, int kv_heads, int batch, int max_new, int64_t
   } else {
     // (A CTA goes on to further groups where there are fewer CTAs than groups: batches so wide that most
     // of a larger grid would find nothing to do.)
-    p.tiles = rows <= 128 ? 1 : 2;
+    // One tile to a CTA (two CTAs to an SM) for few rows, and for so few keys that a CTA's start and end weigh more
+    // than its loop: 16 prompts of 256, 12 heads of 128, in us: 20.6 with one, 24.7 with two; of 512: 41 and 41; 4 of
+    // 2048: 83 and 71.
+    p.tiles = rows <= 128 || max_length <= 384 ? 1 : 2;
     p.groups = (int)std::min(up(rows, 128 * p.tiles), std::max<int64_t>(1, (1 << 18) / base));
-    // parts only while they fit in one wave, of 512 keys or more
-    const int64_t slots = p.tiles == 2 ? 148 : 296;
-    p.nsplit = (int)std::max<int64_t>(1, std::min(max_length / 512, slots / (base * p.groups)));
+    // Parts where they fill the last wave better than they cost: measured us of a block of keys and of a CTA's start
+    // and end, and the parts' way through memory at 5 TB/s (2048 rows x 32 heads: 1030 us in one part, 1085 in four,
+    // so a gain of less than a tenth is left alone).
+    const double block = p.tiles == 2 ? 1.65 : 1.32, ends = p.tiles == 2 ? 6. : 5.;
+    const int64_t slots = p.tiles == 2 ? 148 : 296, blocks = up(max_length, 64 * p.tiles);
+    double best = 0.;
+    for (int n = 1; n <= 32 && (n == 1 || n * 512 <= max_length); ++n) {
+      const double t = up(base * p.groups * n, slots) * (up(blocks, n) * block + ends);
+      const double all = n == 1 ? t : 1.1 * t + 4. + n * (tokens * 1e-6 * q_heads * head_dim * 8. / 5.);
+      if (n == 1 || all < best) {
+        best = all;
+        p.nsplit = n;
+      }
+    }
   }
   return p;
 }
@@ -613,16 +627,16 @@ static int launch(AttendArgs& a, const Plan& p, cudaStream_t st) {
 using namespace ppmoe;
 
 // What both entry points make of their hints: max_new and max_length held to what can be.
-static Plan plan_of(int tokens, int q_heads, int kv_heads, int batch, int max_new, int64_t max_length) {
+static Plan plan_of(int tokens, int q_heads, int kv_heads, int head_dim, int batch, int max_new, int64_t max_length) {
   max_new = max_new < 1 ? 1 : max_new > tokens ? tokens : max_new;
   max_length = max_length < 1 ? 1 : max_length > INT32_MAX ? INT32_MAX : max_length;
-  return make_plan(q_heads, kv_heads, batch, max_new, max_length);
+  return make_plan(tokens, q_heads, kv_heads, head_dim, batch, max_new, max_length);
 }
 
 extern "C" size_t ppmoe_attend_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim, int batch,
                                                int max_new, int64_t max_length) {
   if (tokens < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || batch < 1) return 0;
-  return plan_bytes(plan_of(tokens, q_heads, kv_heads, batch, max_new, max_length), tokens, q_heads, head_dim);
+  return plan_bytes(plan_of(tokens, q_heads, kv_heads, head_dim, batch, max_new, max_length), tokens, q_heads, head_dim);
 }
 
 extern "C" int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t q_t, int64_t q_h, int q_heads,
@@ -655,7 +669,7 @@ extern "C" int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t 
     set_error("ppmoe_attend: scale is not finite");
     return PPMOE_ERR_INVALID_ARG;
   }
-  const Plan p = plan_of(tokens, q_heads, kv_heads, batch, max_new, max_length);
+  const Plan p = plan_of(tokens, q_heads, kv_heads, head_dim, batch, max_new, max_length);
   const size_t need = plan_bytes(p, tokens, q_heads, head_dim);
   if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)) {
     set_error("ppmoe_attend: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, ws ? ws_bytes : 0);

@@ -713,16 +713,22 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           uint8_t* v = smem + TILES * S::kQ + vs * S::kStage;
           const int key0 = block * KEYS, here = min(KEYS, w.keys - key0);
           uint32_t bad = 0;
-#pragma unroll 8
-          for (int i = g; i < KEYS * CH; i += 64) {  // 16-byte chunk i of the tile, as it lies
-            const int key = (i >> 3) & (KEYS - 1);
-            uint4* p = reinterpret_cast<uint4*>(v) + i;
-            if (key >= here) {
-              *p = make_uint4(0, 0, 0, 0);
-            } else {
-              const uint4 u = *p;
-              bad |= not_finite2<T>(u.x) | not_finite2<T>(u.y) | not_finite2<T>(u.z) | not_finite2<T>(u.w);
+          // 16-byte chunk i of the tile, as it lies; eight loads in flight
+#pragma unroll 1
+          for (int i0 = g; i0 < KEYS * CH; i0 += 64 * 8) {
+            uint4 u[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = reinterpret_cast<const uint4*>(v)[i0 + 64 * e];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t x = not_finite2<T>(u[e].x) | not_finite2<T>(u[e].y) | not_finite2<T>(u[e].z) | not_finite2<T>(u[e].w);
+              bad |= ((i0 + 64 * e) >> 3 & (KEYS - 1)) < here ? x : 0;
             }
+          }
+          if (here < KEYS) {
+#pragma unroll 4
+            for (int i = g; i < KEYS * CH; i += 64)
+              if ((i >> 3 & (KEYS - 1)) >= here) reinterpret_cast<uint4*>(v)[i] = make_uint4(0, 0, 0, 0);
           }
           if (bad) {
             *any_odd = 1;

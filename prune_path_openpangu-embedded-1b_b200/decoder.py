@@ -9,8 +9,10 @@ SwiGLU MLP it replaces (same weights, all 6144 neurons, cuBLAS GEMMs) for the ba
 
 Prompt prefill runs the prefill path; greedy decode runs one token per step through a CUDA
 graph of the whole 26-layer step (the fused single-launch decode kernel per MoE layer).
-Attention, norms, RoPE and the LM head use PyTorch operators: they are not part of the
-hot path this library rebuilds.
+Norms and the LM head use PyTorch operators.  Attention comes in two forms: ``kv="dense"``
+(PyTorch operators on a dense cache, a rotation table of ``max_seq`` rows) and ``kv="paged"``
+(``rotary.RotaryEmbedding`` and ``kvcache.PagedKVCache``: append with the rotation on the way, paged
+attention; head_dim 64 or 128).
 """
 from __future__ import annotations
 
@@ -19,6 +21,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
+from .kvcache import PagedKVCache
+from .rotary import RotaryEmbedding
 from .tau_moe import TauSparseMoE
 
 __all__ = ["DecoderConfig", "SyntheticDecoder"]
@@ -37,6 +41,8 @@ class DecoderConfig:
     router_scale: float = 1.75
     max_seq: int = 640
     mlp: str = "moe"  # or "dense"
+    kv: str = "dense"  # or "paged"
+    page: int = 16  # rows of a page (paged)
     eps: float = 1e-6
     rope_theta: float = 10000.0
 
@@ -48,6 +54,8 @@ def _rms(x, w, eps):
 
 class SyntheticDecoder:
     def __init__(self, cfg: DecoderConfig, device, seed: int = 0, max_batch: int = 16):
+        if cfg.kv not in ("dense", "paged"):
+            raise ValueError(f"kv={cfg.kv!r} must be 'dense' or 'paged'")
         self.cfg = cfg
         self.dev = torch.device(device)
         g = torch.Generator(device=self.dev).manual_seed(seed)
@@ -77,12 +85,15 @@ class SyntheticDecoder:
                 L["gate_up"] = torch.cat([W_gate.t(), W_up.t()], 0).contiguous()  # [2I, H]
                 L["down"] = W_down.t().contiguous()  # [H, I]
             self.layers.append(L)
+        self.kv = None
+        self.graph = None
+        if cfg.kv == "paged":
+            self.rotary = RotaryEmbedding(cfg.head_dim, base=cfg.rope_theta)
+            return
         half = cfg.head_dim // 2
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(half, device=self.dev, dtype=torch.float32) / half))
         ang = torch.arange(cfg.max_seq, device=self.dev, dtype=torch.float32)[:, None] * inv[None]
         self.cos, self.sin = ang.cos(), ang.sin()
-        self.kv = None
-        self.graph = None
 
     # ------------------------------------------------------------------ pieces
     def _rope(self, x, pos):  # x [B, h, L, d]; pos [L] int64 (device)
@@ -101,6 +112,13 @@ class SyntheticDecoder:
         cfg = self.cfg
         B, T, H = x.shape
         h = _rms(x, L["ln1"], cfg.eps)
+        if cfg.kv == "paged":
+            q, k, v = F.linear(h, L["wqkv"]).view(B * T, 3, cfg.heads, cfg.head_dim).unbind(1)
+            q = self.kv[i].append(q, k, v, *pos, rotary=self.rotary)
+            # prompts: every sequence is its T new tokens; steps: as long as the cache goes
+            o = self.kv[i].attend(q, *pos, max_new=T, max_length=T if prefill else cfg.max_seq)
+            x = x + F.linear(o.view(B, T, H), L["wo"])
+            return x + self._mlp(L, _rms(x, L["ln2"], cfg.eps))
         q, k, v = F.linear(h, L["wqkv"]).view(B, T, 3, cfg.heads, cfg.head_dim).permute(2, 0, 3, 1, 4)
         q, k = self._rope(q, pos), self._rope(k, pos)
         kc, vc = self.kv[i]
@@ -122,6 +140,14 @@ class SyntheticDecoder:
     def prefill(self, ids):
         cfg = self.cfg
         B, T = ids.shape
+        if cfg.kv == "paged":
+            self._pages(B)
+            x = self.embed[ids]
+            i32 = dict(dtype=torch.int32, device=self.dev)
+            batch = (torch.arange(B + 1, **i32) * T, torch.full((B,), T, **i32), self.table)
+            for i, L in enumerate(self.layers):
+                x = self._layer(i, L, x, batch, True)
+            return self._logits_next(x)
         if self.kv is None or self.kv[0][0].shape[0] != B:  # persistent: captured graphs read them
             self.kv = [(torch.zeros(B, cfg.heads, cfg.max_seq, cfg.head_dim, dtype=torch.bfloat16, device=self.dev),
                         torch.zeros(B, cfg.heads, cfg.max_seq, cfg.head_dim, dtype=torch.bfloat16, device=self.dev))
@@ -133,9 +159,23 @@ class SyntheticDecoder:
             x = self._layer(i, L, x, pos, True)
         return self._logits_next(x)
 
+    def _pages(self, B):
+        """Caches and page table for B sequences of max_seq; kept while B stays (captured graphs read them)."""
+        cfg = self.cfg
+        each = -(-cfg.max_seq // cfg.page)
+        if self.kv is None or self.table.shape[0] != B:
+            self.kv = [PagedKVCache(B * each, cfg.page, cfg.heads, cfg.head_dim, device=self.dev)
+                       for _ in range(cfg.layers)]
+            i32 = dict(dtype=torch.int32, device=self.dev)
+            self.table = torch.arange(B * each, **i32).view(B, each)
+            self.one_each = torch.arange(B + 1, **i32)
+            self.graph = None
+
     @torch.no_grad()
     def _step(self, tok, pos):
         x = self.embed[tok][:, None]
+        if self.cfg.kv == "paged":
+            pos = (self.one_each, (pos + 1).to(torch.int32).repeat(tok.shape[0]), self.table)
         for i, L in enumerate(self.layers):
             x = self._layer(i, L, x, pos, False)
         return self._logits_next(x)

@@ -427,3 +427,61 @@ def test_chunks_and_steps_together(cuda, dtype, hq, hk, dim):
         whole = Batch([total[s]], [total[s]], hk, dim, 16, dtype, cuda)
         whole.keys, whole.values = [kr], [v[s]]
         assert_attention(torch.cat(outs[s]), *exact_attention(whole, qr))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 4])
+def test_decoder_on_pages(cuda, batch):
+    """SyntheticDecoder(kv="paged"): captured steps give the eager ones' tokens; every attention it ran agrees
+    with fp64 over the keys and values that its cache held then."""
+    import importlib
+    D = importlib.import_module(pkg().__name__ + ".decoder")
+    cfg = D.DecoderConfig(layers=2, hidden=256, heads=2, head_dim=128, vocab=1000, experts=16, group=32, max_seq=70, kv="paged")
+    d = D.SyntheticDecoder(cfg, cuda, seed=3, max_batch=4)
+    ids = torch.randint(0, 1000, (batch, 20), generator=torch.Generator().manual_seed(1)).to(cuda)
+    t_graph, _, _ = d.generate(ids, 12, use_graph=True)
+    t_again, _, _ = d.generate(ids, 12, use_graph=True)
+    seen, attend = [], pkg().kvcache.PagedKVCache.attend
+
+    def record(cache, q, starts, lengths, table, **hints):
+        out = attend(cache, q, starts, lengths, table, **hints)
+        seen.append((q.clone(), starts, lengths.clone(), table, cache.k.clone(), cache.v.clone(), out.clone()))
+        return out
+
+    pkg().kvcache.PagedKVCache.attend = record
+    try:
+        t_eager, _, _ = d.generate(ids, 12, use_graph=False)
+    finally:
+        pkg().kvcache.PagedKVCache.attend = attend
+    assert torch.equal(t_graph, t_eager) and torch.equal(t_again, t_eager) and t_eager.shape == (batch, 12)
+    assert len(seen) == 2 * 12
+    for q, starts, lengths, table, k, v, out in seen:
+        new = (starts[1:] - starts[:-1]).tolist()
+        b = Batch(new, lengths.tolist(), 2, 128, cfg.page, torch.bfloat16, cuda)
+        b.keys, b.values = ([x[table[s].long()].transpose(1, 2).reshape(-1, 2, 128)[:n] for s, n in enumerate(lengths.tolist())]
+                            for x in (k, v))
+        assert_attention(out, *exact_attention(b, q))
+    for cache in d.kv:
+        cache.check_device_status()
+    with pytest.raises(ValueError):
+        D.SyntheticDecoder(D.DecoderConfig(layers=1, kv="other"), cuda)
+
+
+@pytest.mark.gpu
+def test_decoder_forms_agree(cuda):
+    """Prompt and first step on pages and on the dense cache, in hidden states of one dense-MLP layer.  Both hold
+    q, k, v, weights and outputs in bf16 and differ in a handful of roundings (half a step each, of values
+    that a layer's sums keep at their size): within 16 half steps of the largest value."""
+    import importlib
+    D = importlib.import_module(pkg().__name__ + ".decoder")
+    outs = []
+    for kv in ("dense", "paged"):
+        cfg = D.DecoderConfig(layers=1, hidden=256, heads=4, head_dim=64, vocab=500, experts=8, group=32, max_seq=64, mlp="dense", kv=kv)
+        d = D.SyntheticDecoder(cfg, cuda, seed=5)
+        d._logits_next = lambda x: x
+        ids = torch.randint(0, 500, (3, 21), generator=torch.Generator().manual_seed(2)).to(cuda)
+        x = d.prefill(ids)
+        y = d._step(ids[:, 0], torch.tensor([21], device=cuda))
+        outs.append((x.float(), y.float()))
+    for a, b in zip(*outs):
+        assert (a - b).abs().max() <= 16 * half_step(torch.bfloat16) * a.abs().max()
