@@ -5,14 +5,20 @@
 //   y1 = g (x1 cos - x2 sin),  y2 = g (x2 cos + x1 sin)     (gradient: the same with -angle)
 // The angle is reduced in fp64 (p turns[i] minus the nearest integer), so far positions lose
 // nothing, and its sine and cosine are taken in fp32; values are rounded once, at the store.
+//
+// Bound by memory: every value is read and written once.  Taking the angle from the position costs one
+// fp64 product and one sincospi per pair and token, shared by all heads, and no table that would have
+// to be read or sized.  Measured (bf16, 12 + 12 heads of 128, 16384 tokens, 201 MB): 37.0 us, 5.4 TB/s;
+// (fp16, 32 + 8 heads of 128, half of each turned, 32768 tokens, 671 MB): 104.7 us, 6.4 TB/s.  Streaming
+// loads and stores and CTAs of 2 tokens x 128 threads: 37.0 us; without the hints 41.1; 4 x 256: 38.5.
 #include <cuda_fp16.h>
 #include "seqs.cuh"
 
 namespace ppmoe {
 
 constexpr int kMaxPairs = 128;  // head_dim <= 256
-constexpr int kRotThreads = 256;
-constexpr int kRotTokens = 8;   // most tokens of one CTA
+constexpr int kRotThreads = 128;
+constexpr int kRotTokens = 4;   // most tokens of one CTA
 
 // One tensor of heads: rows of head_dim contiguous values; strides in elements.
 struct HeadsView {
@@ -39,7 +45,7 @@ struct RotaryArgs {
 };
 
 template <typename T, int V>
-struct Chunk {
+struct alignas(V == 1 ? alignof(T) : 16) Chunk {
   T x[V];
 };
 template <typename T, int V>
@@ -49,7 +55,18 @@ __device__ __forceinline__ Chunk<T, V> load_chunk(const T* p) {
     c.x[0] = *p;
   } else {
     static_assert(sizeof(T) * V == 16, "16-byte chunks");
-    *reinterpret_cast<uint4*>(c.x) = *reinterpret_cast<const uint4*>(p);
+    *reinterpret_cast<uint4*>(c.x) = __ldcs(reinterpret_cast<const uint4*>(p));  // read once
+  }
+  return c;
+}
+template <int V>
+__device__ __forceinline__ Chunk<float, V> load_angles(const float* p) {
+  Chunk<float, V> c;
+  if constexpr (V == 1) {
+    c.x[0] = *p;
+  } else {  // (V divides the pairs of a token)
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(c.x + i) = *reinterpret_cast<const float4*>(p + i);
   }
   return c;
 }
@@ -58,57 +75,65 @@ __device__ __forceinline__ void store_chunk(T* p, const Chunk<T, V>& c) {
   if constexpr (V == 1)
     *p = c.x[0];
   else
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(c.x);
+    __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(c.x));
 }
 
 // A unit is V pairs (two 16-byte chunks of a head, or 2 values where alignment allows no
-// more): units [0, pairs / V) of a head are rotated, the rest copied.
+// more): units [0, pairs / V) of a head are rotated, the rest copied.  A CTA takes a few tokens: offsets of
+// their rows, sines and cosines once, into shared memory; then a thread keeps its place in the head and
+// goes through (token, head) in equal steps, so that a unit costs no division.
 template <typename T, int V, bool INTERLEAVED, bool APPEND>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   __shared__ __align__(16) float s_cos[kRotTokens * kMaxPairs], s_sin[kRotTokens * kMaxPairs];
   __shared__ long long s_pos[kRotTokens];
-  __shared__ int64_t s_k[kRotTokens], s_v[kRotTokens];  // append: cache offsets, -1: not stored
-  __shared__ int s_live[kRotTokens];
+  __shared__ int64_t s_in[kRotTokens][3], s_out[kRotTokens][3];  // q, k, v: elements to the token's first head
+  __shared__ bool s_skip[kRotTokens][3];                         // not stored
   const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * a.per_cta;
   const int nt = (int)(a.tokens - t0 < a.per_cta ? a.tokens - t0 : a.per_cta);
 
-  // positions (and, for an append, the place in the cache) of this CTA's tokens
-  if constexpr (APPEND) {
-    const int w = tid >> 5;
-    static_assert(kRotThreads / 32 >= kRotTokens, "a warp a token");
-    if (w < nt) {
-      const int t = (int)(t0 + w);
-      const int b = find_seq_warp(a.seqs.starts, a.seqs.batch, t);
-      if ((tid & 31) == 0) {
+  // a warp a token: its position and (append) its place in the cache
+  static_assert(kRotThreads / 32 >= kRotTokens, "a warp a token");
+  if (const int w = tid >> 5; w < nt) {
+    const unsigned t = (unsigned)(t0 + w);
+    const bool lead = (tid & 31) == 0;
+    if constexpr (APPEND) {
+      const int b = find_seq_warp(a.seqs.starts, a.seqs.batch, (int)t);
+      if (lead) {
         const bool live = b >= 0 && b < a.seqs.batch;
         long long pos = 0;
-        int64_t ko = -1, vo = -1;
+        bool stored = false;
         if (live) {
           pos = (long long)a.seqs.lengths[b] - a.seqs.starts[b + 1] + t;
           const long long pi = pos >> a.pages.page_shift;
           int page = -1;
           if (pos >= 0 && pi < a.seqs.max_pages) page = a.seqs.table[b * a.seqs.table_stride + pi];
-          if (page >= 0 && page < a.pages.num_pages) {
+          stored = page >= 0 && page < a.pages.num_pages;
+          if (stored) {
             const int64_t row = pos & ((1ll << a.pages.page_shift) - 1);
-            ko = page * a.pages.k_page + row * a.pages.k_row;
-            vo = page * a.pages.v_page + row * a.pages.v_row;
+            s_out[w][1] = page * a.pages.k_page + row * a.pages.k_row;
+            s_out[w][2] = page * a.pages.v_page + row * a.pages.v_row;
           } else {
             atomicOr(a.status, DEVERR_PAGE);
           }
         }
-        s_live[w] = live;
         s_pos[w] = pos;
-        s_k[w] = ko;
-        s_v[w] = vo;
+        s_in[w][0] = t * a.q.in_t;
+        s_in[w][1] = t * a.k.in_t;
+        s_in[w][2] = t * a.v.in_t;
+        s_out[w][0] = t * a.q.out_t;
+        s_skip[w][0] = !live;
+        s_skip[w][1] = s_skip[w][2] = !stored;
       }
-    }
-  } else {
-    if (tid < nt) {
-      const int64_t t = t0 + tid;
-      const int64_t i = (t / a.length) * a.pos_b + (t % a.length) * a.pos_t;
-      s_pos[tid] = a.pos64 ? static_cast<const long long*>(a.positions)[i]
-                           : (long long)static_cast<const int32_t*>(a.positions)[i];
+    } else if (lead) {
+      const unsigned b = t / (unsigned)a.length, l = t - b * (unsigned)a.length;
+      const int64_t i = b * a.pos_b + l * a.pos_t;
+      s_pos[w] = a.pos64 ? static_cast<const long long*>(a.positions)[i]
+                         : (long long)static_cast<const int32_t*>(a.positions)[i];
+      s_in[w][0] = b * a.q.in_b + l * a.q.in_t;
+      s_in[w][1] = b * a.k.in_b + l * a.k.in_t;
+      s_out[w][0] = b * a.q.out_b + l * a.q.out_t;
+      s_out[w][1] = b * a.k.out_b + l * a.k.out_t;
     }
   }
   __syncthreads();
@@ -122,56 +147,48 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
   }
   __syncthreads();
 
-  const int units = a.head_dim / (2 * V), turned = a.pairs / V;
+  const int units = a.head_dim / (2 * V);
   const int heads = a.q.heads + a.k.heads + (APPEND ? a.v.heads : 0);
-  const int per_token = heads * units;
-  for (int i = tid; i < nt * per_token; i += kRotThreads) {
-    const int t = i / per_token;
-    const int r = i - t * per_token;
-    int h = r / units;
-    const int u = r - h * units;
-    const int64_t tok = t0 + t;
-    const int64_t b = APPEND ? 0 : tok / a.length, l = APPEND ? tok : tok - b * a.length;
+  const int slots = kRotThreads / units;  // heads taken at once (units <= 128)
+  const int slot = tid / units, u = tid - slot * units;
+  if (slot >= slots) return;
+  const bool turned = u < a.pairs / V;
+  const int step_t = slots / heads, step_h = slots - step_t * heads;
+  int t = slot / heads, h = slot - t * heads;
+  for (; t < nt; t += step_t, h += step_h) {
+    if (h >= heads) {
+      h -= heads;
+      if (++t >= nt) break;
+    }
+    // which tensor
+    const int g = h < a.q.heads ? 0 : !APPEND || h < a.q.heads + a.k.heads ? 1 : 2;
+    if (APPEND && s_skip[t][g]) continue;
     const T* in;
     T* out;
-    bool rotate = u < turned;
-    if (h < a.q.heads) {
-      if (APPEND && !s_live[t]) continue;
-      in = static_cast<const T*>(a.q.in) + b * a.q.in_b + l * a.q.in_t + h * a.q.in_h;
-      out = static_cast<T*>(a.q.out) + b * a.q.out_b + l * a.q.out_t + h * a.q.out_h;
-    } else if (h -= a.q.heads; h < a.k.heads) {
-      in = static_cast<const T*>(a.k.in) + b * a.k.in_b + l * a.k.in_t + h * a.k.in_h;
-      if constexpr (APPEND) {
-        if (s_k[t] < 0) continue;
-        out = static_cast<T*>(a.pages.k) + s_k[t] + h * a.pages.k_head;
-      } else {
-        out = static_cast<T*>(a.k.out) + b * a.k.out_b + l * a.k.out_t + h * a.k.out_h;
-      }
+    if (g == 0) {
+      in = static_cast<const T*>(a.q.in) + s_in[t][0] + h * a.q.in_h;
+      out = static_cast<T*>(a.q.out) + s_out[t][0] + h * a.q.out_h;
+    } else if (!APPEND || g == 1) {
+      const int hh = h - a.q.heads;
+      in = static_cast<const T*>(a.k.in) + s_in[t][1] + hh * a.k.in_h;
+      out = APPEND ? static_cast<T*>(a.pages.k) + s_out[t][1] + hh * a.pages.k_head
+                   : static_cast<T*>(a.k.out) + s_out[t][1] + hh * a.k.out_h;
     } else {
-      h -= a.k.heads;
-      if (s_v[t] < 0) continue;
-      in = static_cast<const T*>(a.v.in) + l * a.v.in_t + h * a.v.in_h;
-      out = static_cast<T*>(a.pages.v) + s_v[t] + h * a.pages.v_head;
-      rotate = false;
+      const int hh = h - a.q.heads - a.k.heads;
+      in = static_cast<const T*>(a.v.in) + s_in[t][2] + hh * a.v.in_h;
+      out = static_cast<T*>(a.pages.v) + s_out[t][2] + hh * a.pages.v_head;
     }
+    const bool rotate = turned && (!APPEND || g < 2);
     // element offsets of the unit's two chunks
-    int e1, e2;
-    if (!INTERLEAVED && u < turned) {
-      e1 = u * V;
-      e2 = a.pairs + u * V;
-    } else {
-      e1 = u * 2 * V;
-      e2 = e1 + V;
-    }
+    const int e1 = !INTERLEAVED && rotate ? u * V : u * 2 * V, e2 = !INTERLEAVED && rotate ? a.pairs + u * V : e1 + V;
     Chunk<T, V> x = load_chunk<T, V>(in + e1), y = load_chunk<T, V>(in + e2);
     if (rotate) {
-      const float* cs = s_cos + t * a.pairs + u * V;
-      const float* sn = s_sin + t * a.pairs + u * V;
+      const Chunk<float, V> cs = load_angles<V>(s_cos + t * a.pairs + u * V), sn = load_angles<V>(s_sin + t * a.pairs + u * V);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         T& p1 = INTERLEAVED ? (2 * j < V ? x.x[2 * j] : y.x[2 * j - V]) : x.x[j];
         T& p2 = INTERLEAVED ? (2 * j + 1 < V ? x.x[2 * j + 1] : y.x[2 * j + 1 - V]) : y.x[j];
-        const float f1 = to_f32<T>(p1), f2 = to_f32<T>(p2), c = cs[j], s = sn[j];
+        const float f1 = to_f32<T>(p1), f2 = to_f32<T>(p2), c = cs.x[j], s = sn.x[j];
         p1 = from_f32<T>(f1 * c - f2 * s);
         p2 = from_f32<T>(f2 * c + f1 * s);
       }
@@ -194,7 +211,7 @@ static int launch_v(RotaryArgs& a, bool interleaved, cudaStream_t st) {
 
 template <bool APPEND>
 static int launch(RotaryArgs& a, bool interleaved, int dtype, bool wide, cudaStream_t st) {
-  a.per_cta = a.tokens <= 1024 ? 1 : 4;
+  a.per_cta = a.tokens <= 1024 ? 1 : 2;  // (few tokens: as many SMs as there are)
   if (dtype == PPMOE_BF16)
     return wide ? launch_v<__nv_bfloat16, 8, APPEND>(a, interleaved, st)
                 : launch_v<__nv_bfloat16, 1, APPEND>(a, interleaved, st);
