@@ -147,36 +147,37 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
     }
     cp_async_commit();
 
-    // pages of a block's halves of 16 keys (one page, or two of 16 rows)
-    auto ids = [&](int bk, int& p0, int& p1) {
-      const int key = bk * KEYS;
-      p0 = bk < blk_end ? __ldg(table + (key >> shift)) : -1;
-      p1 = KEYS > 16 && bk < blk_end && key + 16 < keys ? __ldg(table + ((key + 16) >> shift)) : -1;
+    // pages of a block's sixteens of keys (pages have 16 rows or more)
+    constexpr int NP = KEYS / 16;
+    auto ids = [&](int bk, int (&page)[NP]) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int key = bk * KEYS + i * 16;
+        page[i] = bk < blk_end && key < keys ? __ldg(table + (key >> shift)) : -1;
+      }
     };
-    auto fetch = [&](int bk, int stage, int p0, int p1) {
+    auto fetch = [&](int bk, int stage, const int (&page)[NP]) {
       if (bk < blk_end) {
         const int key = bk * KEYS;
         const uint32_t kd = ring + stage * 2 * S::kTile, vd = kd + S::kTile;
-        const bool ok0 = (uint32_t)p0 < (uint32_t)a.pages.num_pages;
-        const bool ok1 = (uint32_t)p1 < (uint32_t)a.pages.num_pages;
-        if (lane == 0 && (!ok0 || (KEYS > 16 && !ok1 && key + 16 < keys))) atomicOr(a.status, DEVERR_PAGE);
-        const int in = key & ((1 << shift) - 1), in1 = (key + 16) & ((1 << shift) - 1);
         const int c = lane % CH, rr = lane / CH;
-        const T* kb0 = static_cast<const T*>(a.pages.k) + kvh * a.pages.k_head + c * 8;
-        const T* vb0 = static_cast<const T*>(a.pages.v) + kvh * a.pages.v_head + c * 8;
-        const T* kb1 = kb0 + (ok1 ? p1 * a.pages.k_page + (in1 + rr) * a.pages.k_row : 0);
-        const T* vb1 = vb0 + (ok1 ? p1 * a.pages.v_page + (in1 + rr) * a.pages.v_row : 0);
-        kb0 += ok0 ? p0 * a.pages.k_page + (in + rr) * a.pages.k_row : 0;
-        vb0 += ok0 ? p0 * a.pages.v_page + (in + rr) * a.pages.v_row : 0;
+        const T* k0 = static_cast<const T*>(a.pages.k) + kvh * a.pages.k_head + c * 8;
+        const T* v0 = static_cast<const T*>(a.pages.v) + kvh * a.pages.v_head + c * 8;
 #pragma unroll
-        for (int i = 0; i < KEYS / RPI; ++i) {
-          const int row = i * RPI + rr;
-          const bool hi = i * RPI >= 16;
-          const bool real = (hi ? ok1 : ok0) && key + row < keys;
-          const int64_t off = (i * RPI) & 15;
-          const uint32_t d = row * (D * 2) + ((c ^ (row & 7)) << 4);
-          cp_async16_or_zero(kd + d, (hi ? kb1 : kb0) + (real ? off * a.pages.k_row : 0), real);
-          cp_async16_or_zero(vd + d, (hi ? vb1 : vb0) + (real ? off * a.pages.v_row : 0), real);
+        for (int p = 0; p < NP; ++p) {
+          const bool ok = (uint32_t)page[p] < (uint32_t)a.pages.num_pages;
+          if (lane == 0 && !ok && key + p * 16 < keys) atomicOr(a.status, DEVERR_PAGE);
+          const int in = (key + p * 16) & ((1 << shift) - 1);
+          const T* kp = k0 + (ok ? page[p] * a.pages.k_page + (in + rr) * a.pages.k_row : 0);
+          const T* vp = v0 + (ok ? page[p] * a.pages.v_page + (in + rr) * a.pages.v_row : 0);
+#pragma unroll
+          for (int i = 0; i < 16 / RPI; ++i) {
+            const int row = p * 16 + i * RPI + rr;
+            const bool real = ok && key + row < keys;
+            const uint32_t d = row * (D * 2) + ((c ^ (row & 7)) << 4);
+            cp_async16_or_zero(kd + d, kp + (real ? i * RPI * a.pages.k_row : 0), real);
+            cp_async16_or_zero(vd + d, vp + (real ? i * RPI * a.pages.v_row : 0), real);
+          }
         }
       }
       cp_async_commit();
@@ -191,13 +192,13 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
       for (int n = 0; n < NT; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
     }
 
-    int p0, p1;
+    int page[NP];
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
-      ids(blk + s * kThinWarps, p0, p1);
-      fetch(blk + s * kThinWarps, s, p0, p1);
+      ids(blk + s * kThinWarps, page);
+      fetch(blk + s * kThinWarps, s, page);
     }
-    ids(blk + (STAGES - 1) * kThinWarps, p0, p1);
+    ids(blk + (STAGES - 1) * kThinWarps, page);
     cp_async_wait<STAGES - 1>();  // q
     __syncthreads();
     uint32_t qf[MT == 1 ? KS : 1][4];
@@ -216,8 +217,8 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
         const int ahead = blk + (STAGES - 1) * kThinWarps;
         int st = stage + STAGES - 1;
         if (st >= STAGES) st -= STAGES;
-        fetch(ahead, st, p0, p1);
-        ids(ahead + kThinWarps, p0, p1);
+        fetch(ahead, st, page);
+        ids(ahead + kThinWarps, page);
       }
       cp_async_wait<STAGES - 1>();
       __syncwarp();
@@ -435,9 +436,10 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
         for (int w = 0; w < kMaxCluster; ++w) top = fmaxf(top, ml[w].x);
 #pragma unroll
         for (int w = 0; w < kMaxCluster; ++w) {
-          const bool real = w < a.nsplit && ml[w].x != -CUDART_INF_F;
-          const float f = real ? exp2_ftz(ml[w].x - top) : 0.f;
-          if (real) {  // (a part without keys holds sums of 0; one past the last may hold inf or NaN)
+          // a part without keys has a sum of 0 (one whose every score is NaN has a sum of NaN)
+          const bool real = w < a.nsplit && !(ml[w].x == -CUDART_INF_F && ml[w].y == 0.f);
+          const float f = ml[w].x == -CUDART_INF_F ? 1.f : exp2_ftz(ml[w].x - top);
+          if (real) {
             sum += f * ml[w].y;
             acc[0] += f * x[w].x;
             acc[1] += f * x[w].y;

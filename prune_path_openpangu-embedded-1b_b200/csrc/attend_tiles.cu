@@ -417,7 +417,16 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
             if (move) m = mx[0];
           }
-          const float sub = (m == -CUDART_INF_F ? 0.f : m * c) - kLift<T>;
+          float sub = m == -CUDART_INF_F ? 0.f : m * c;
+          // c s - sub carries the rounding of sub, the same factor for every weight of the row: it cancels, but
+          // from |sub| = 2^24 on it could leave the types' range.  Such scores are taken from m first.
+          if (__any_sync(0xffffffffu, fabsf(sub) > 65536.f)) {
+            const float from = m == -CUDART_INF_F ? 0.f : m;
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) s[i] -= from;
+            sub = 0.f;
+          }
+          sub -= kLift<T>;
           const uint64_t c2 = two(c, c), sub2 = two(-sub, -sub);
           uint64_t sum[2] = {0, 0};
           // weights, in eights of pairs: the first three quarters are handed on while the last is computed

@@ -70,7 +70,7 @@ class PagedKVCache:
     def _mount(self, k, v):
         if k.device.type != "cuda":
             raise RuntimeError("PagedKVCache runs on CUDA only; got " + str(k.device))
-        self.k, self.v = k, v
+        self._k, self._v = k, v  # (the structure below holds their addresses)
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype, self.device = k.dtype, k.device
         self._status = torch.zeros(256, dtype=torch.uint8, device=k.device)
@@ -80,11 +80,30 @@ class PagedKVCache:
 
         self._c = _lib.KVCache(k.data_ptr(), v.data_ptr(), *strides(k), *strides(v), *k.shape[:1], self.page_size,
                                self.kv_heads, self.head_dim, _DTYPES[k.dtype], self._status.data_ptr())
-        self._ptr = ctypes.addressof(self._c)
+
+    @property
+    def k(self) -> torch.Tensor:
+        return self._k
+
+    @property
+    def v(self) -> torch.Tensor:
+        return self._v
+
+    @property
+    def _ptr(self) -> int:
+        return ctypes.addressof(self._c)
+
+    def __deepcopy__(self, memo):
+        return PagedKVCache.from_tensors(self._k.clone(), self._v.clone())
+
+    def __reduce__(self):
+        return PagedKVCache.from_tensors, (self._k, self._v)
 
     # ------------------------------------------------------------------ checks
     def _rows(self, name, x, heads=None):
         """x and its strides, checked."""
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires a gradient, and the cache records none: call it under torch.no_grad()")
         shape = x.shape
         if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {self.head_dim}], got {list(shape)}")
@@ -119,7 +138,7 @@ class PagedKVCache:
         ``[tokens, kv_heads, head_dim]`` to their places, and returns ``q [tokens, q_heads, head_dim]``
         rotated likewise: a new tensor, or ``out`` (which may be ``q``).  ``q`` None returns None.  Rows
         outside every sequence are not written, in ``out`` neither.  The rows of one call must go to
-        different places.  Records no gradients."""
+        different places.  Records no gradients, and refuses rows that ask for one."""
         k, sk = self._rows("k", k, self.kv_heads)
         v, sv = self._rows("v", v, self.kv_heads)
         T = k.shape[0]
@@ -158,7 +177,8 @@ class PagedKVCache:
         ``h // (q_heads / kv_heads)``).  A row at a negative position gives zeros; rows outside every
         sequence are not written.  ``max_new`` / ``max_length``: the most new rows and the greatest length of
         a sequence as far as the host knows (default: the largest possible); they choose how the work is
-        laid out, never what is computed.  ``scale`` defaults to ``head_dim ** -0.5``.  Records no gradients."""
+        laid out, never what is computed.  ``scale`` defaults to ``head_dim ** -0.5``.  ``out`` may be ``q``.  Records no gradients, and
+        refuses rows that ask for one."""
         q, sq = self._rows("q", q)
         T, Hq, D = q.shape
         if Hq < 1 or Hq % self.kv_heads:
@@ -176,7 +196,7 @@ class PagedKVCache:
         back = _enter(self.device)
         n = lib.ppmoe_attend_workspace_bytes(T, Hq, self.kv_heads, D, batch[4], new, length)
         ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-        rc = lib.ppmoe_attend(self._ptr, q.data_ptr(), sq[0], sq[1], Hq, T, *batch, D ** -0.5 if scale is None else scale,
+        rc = lib.ppmoe_attend(self._ptr, q.data_ptr(), sq[0], sq[1], Hq, T, *batch, D ** -0.5 if scale is None else float(scale),
                               new, length, out.data_ptr(), so[0], so[1], None if ws is None else ws.data_ptr(), n,
                               _stream(self.device))
         if back is not None:

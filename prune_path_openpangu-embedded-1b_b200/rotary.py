@@ -125,7 +125,10 @@ class RotaryEmbedding:
         self.turns = freq / (2.0 * math.pi)
         self._c = _lib.Rotation(rotary_dim, layout == "interleaved", self.gain)
         self._c.turns[:rotary_dim // 2] = self.turns.tolist()
-        self._ptr = ctypes.addressof(self._c)
+
+    @property
+    def _ptr(self) -> int:  # (of this object's own structure: copies have theirs)
+        return ctypes.addressof(self._c)
 
     # ------------------------------------------------------------------ calls
     def __call__(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor
@@ -138,7 +141,7 @@ class RotaryEmbedding:
         return self._launch(q, k, positions, False)
 
     def rotate_(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor) -> None:
-        """The same in place (no gradients)."""
+        """The same in place (no gradients; ``q`` and ``k`` must not overlap)."""
         for x in (q, k):
             if x is not None and torch.is_grad_enabled() and x.requires_grad:
                 raise RuntimeError("rotate_ records no gradients: call the embedding itself, or use torch.no_grad()")

@@ -281,6 +281,82 @@ def test_values_that_are_not_finite(cuda, dtype, dim, page, new, hint):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new,hint", [(1, 1), (5, 5), (40, 40), (150, 150), (150, 1)])
+def test_a_key_that_is_not_a_number(cuda, new, hint):
+    """NaN in a sequence's first key: every row of it is NaN, also one that sees no other key; the other
+    sequence is as ever."""
+    b = Batch([new, new], [new, 300], 1, 64, 16, torch.float16, cuda, seed=14)
+    b.keys[0][0, 0, 9] = math.nan
+    b.k[b.table[0, 0].long(), 0, 0, 9] = math.nan
+    q = b.normal(3, 2.0)
+    out = b.cache().attend(q, b.starts, b.lens, b.table, max_new=hint)
+    assert out[:new].isnan().all()
+    want = exact_attention(b, q)
+    assert_attention(out[new:], want[0][new:], want[1][new:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new", [1, 20, 200])
+def test_attend_huge_scores(cuda, dtype, new):
+    """Whole-number scores times 2^20: exact in fp32, up to 2^36; each row's weight is shared by its largest."""
+    b = Batch([new], [new + 500], 1, 64, 64, dtype, cuda, seed=15)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    b.keys[0] = torch.randint(-32, 33, (new + 500, 1, 64), generator=g, device=cuda).to(dtype)
+    pos = torch.arange(new + 500, device=cuda)
+    b.k[b.table[0][pos // 64].long(), :, pos % 64] = b.keys[0]
+    q = torch.randint(-32, 33, (new, 2, 64), generator=g, device=cuda).to(dtype)
+    assert_attention(b.cache().attend(q, b.starts, b.lens, b.table, scale=2.0 ** 20, max_new=new), *exact_attention(b, q, 2.0 ** 20))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,length", [(1, 3000), (1, 40000), (20, 3000), (200, 900)])
+def test_attend_in_place_of_q(cuda, new, length):
+    b = Batch([new, 1], [length, 50], 2, 128, 32, torch.bfloat16, cuda, seed=16)
+    q = b.normal(6, 2.0)
+    want = b.cache().attend(q, b.starts, b.lens, b.table, max_new=new)
+    assert b.cache().attend(q, b.starts, b.lens, b.table, max_new=new, out=q) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.gpu
+def test_copies_and_gradients(cuda):
+    import copy
+    import pickle
+    b = Batch([4], [40], 2, 64, 16, torch.bfloat16, cuda, seed=17)
+    cache, q, e = b.cache(), b.normal(4), emb(64)
+    k, v = b.normal(2), b.normal(2)
+    cache2, e2 = copy.deepcopy(cache), copy.deepcopy(e)
+    e3 = pickle.loads(pickle.dumps(e))
+    want = cache.append(q, k, v, b.starts, b.lens, b.table, rotary=e)
+    del e
+    for other in (e2, e3):
+        assert torch.equal(cache2.append(q, k, v, b.starts, b.lens, b.table, rotary=other), want)
+    assert cache2.k.data_ptr() != cache.k.data_ptr() and torch.equal(cache2.k.view(torch.int16), cache.k.view(torch.int16))
+    with pytest.raises(AttributeError):
+        cache.k = cache2.k
+    q.requires_grad_()
+    for call in (lambda: cache.attend(q, b.starts, b.lens, b.table), lambda: cache.append(q, k, v, b.starts, b.lens, b.table)):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call()
+        with torch.no_grad():
+            call()
+
+
+@pytest.mark.gpu
+def test_rows_before_the_first_sequence(cuda):
+    """starts need not begin at 0: rows before it are nobody's."""
+    b = Batch([3, 2], [50, 60], 1, 64, 16, torch.float16, cuda, seed=18, pad=4)
+    q = b.normal(2, 2.0)
+    shifted = torch.cat([q[-2:], q[:-2]])
+    for new in (1, 16, 40):
+        out = torch.full_like(q, 7.0)
+        b.cache().attend(shifted, b.starts + 2, b.lens, b.table, max_new=new, out=out)
+        assert (out[:2] == 7).all() and (out[7:] == 7).all()
+        assert_attention(out[2:7], *(x[:5] for x in exact_attention(b, q)))
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits(cuda):
     """A cache of more than 2^31 values whose used pages lie at its end."""
     pages, page, hk = 140_000, 256, 1
