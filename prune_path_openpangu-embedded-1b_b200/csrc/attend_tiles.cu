@@ -369,6 +369,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const int all_see = min(pos0 + base / a.group, cap - 1);       // ... the tile's first row
         const int count = w.count[t];
         float m = -CUDART_INF_F, l = 0.f;
+        bool far = false;  // some row of the warp has |c m| > 2^16
 #pragma unroll 1
         for (int j = 0; j < count; ++j) {
           float s[KEYS];
@@ -416,29 +417,27 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               tmem_st_wait();
             }
             if (move) m = mx[0];
+            // c s - c m carries the rounding of c m, the same factor for every weight of the row: it cancels, but
+            // from |c m| = 2^24 on it could leave the types' range.  Such scores are taken from m first.
+            far = __any_sync(0xffffffffu, fabsf(m * c) > 65536.f && m != -CUDART_INF_F);
           }
-          float sub = m == -CUDART_INF_F ? 0.f : m * c;
-          // c s - sub carries the rounding of sub, the same factor for every weight of the row: it cancels, but
-          // from |sub| = 2^24 on it could leave the types' range.  Such scores are taken from m first.
-          if (__any_sync(0xffffffffu, fabsf(sub) > 65536.f)) {
-            const float from = m == -CUDART_INF_F ? 0.f : m;
-#pragma unroll
-            for (int i = 0; i < KEYS; ++i) s[i] -= from;
-            sub = 0.f;
-          }
-          sub -= kLift<T>;
-          const uint64_t c2 = two(c, c), sub2 = two(-sub, -sub);
+          const float from = m == -CUDART_INF_F ? 0.f : m;
+          const uint64_t c2 = two(c, c), from2 = two(-from, -from), lift2 = two(kLift<T>, kLift<T>);
+          const uint64_t sub2 = two(kLift<T> - from * c, kLift<T> - from * c);
           uint64_t sum[2] = {0, 0};
           // weights, in eights of pairs: the first three quarters are handed on while the last is computed
-          auto weights = [&](auto some, int from, int to) {
+          // MODE 0: all keys seen, some exponentials by exp2_pair; 1: masked; 2: far scores
+          auto weights = [&](auto mode, int first, int to) {
+            constexpr int MODE = decltype(mode)::value;
 #pragma unroll
-            for (int g = from; g < to; g += 16) {
+            for (int g = first; g < to; g += 16) {
               uint32_t p[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 float x0, x1, e0, e1;
-                untwo(fma2(two(s[g + 2 * i], s[g + 2 * i + 1]), c2, sub2), x0, x1);
-                if (decltype(some)::value && (i & 3) == 3) {
+                const uint64_t s2 = two(s[g + 2 * i], s[g + 2 * i + 1]);
+                untwo(MODE < 2 ? fma2(s2, c2, sub2) : fma2(add2(s2, from2), c2, lift2), x0, x1);
+                if (MODE == 0 && (i & 3) == 3) {
                   exp2_pair<T>(x0, x1, e0, e1);
                 } else {
                   e0 = exp2_ftz(x0);
@@ -450,17 +449,19 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               tmem_st8(t_s + g / 2, p);
             }
           };
-          if (masked)
-            weights(std::false_type{}, 0, S::kEarly);
-          else
-            weights(std::true_type{}, 0, S::kEarly);
+          auto part = [&](int first, int to) {
+            if (far)
+              weights(std::integral_constant<int, 2>{}, first, to);
+            else if (masked)
+              weights(std::integral_constant<int, 1>{}, first, to);
+            else
+              weights(std::integral_constant<int, 0>{}, first, to);
+          };
+          part(0, S::kEarly);
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(p_early + t);
-          if (masked)
-            weights(std::false_type{}, S::kEarly, KEYS);
-          else
-            weights(std::true_type{}, S::kEarly, KEYS);
+          part(S::kEarly, KEYS);
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(p_late + t);
