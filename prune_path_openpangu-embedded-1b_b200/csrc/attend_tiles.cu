@@ -49,6 +49,26 @@ __device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, uint32_
   atomicOr(status, DEVERR_TIMEOUT);
 }
 
+// Which of four barriers have passed a phase (bit i: barrier i), asked all at once.  A question takes the products'
+// warp about 220 cycles whatever the answer (it queues behind the softmax warps' exponentials and TMEM
+// accesses), so it asks for a tile's barriers together and waits only for those that were not ready.
+__device__ __forceinline__ uint32_t test_bars(uint64_t* b0, uint32_t ph0, uint64_t* b1, uint32_t ph1, uint64_t* b2, uint32_t ph2,
+                                              uint64_t* b3, uint32_t ph3) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p0, p1, p2, p3;\n .reg .b32 a, b, c;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p0, [%1], %2;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p1, [%3], %4;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p2, [%5], %6;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p3, [%7], %8;\n"
+      " selp.b32 %0, 1, 0, p0;\n selp.b32 a, 2, 0, p1;\n selp.b32 b, 4, 0, p2;\n selp.b32 c, 8, 0, p3;\n"
+      " or.b32 %0, %0, a;\n or.b32 b, b, c;\n or.b32 %0, %0, b;\n}\n"
+      : "=&r"(r)
+      : "r"(smem_u32(b0)), "r"(ph0), "r"(smem_u32(b1)), "r"(ph1), "r"(smem_u32(b2)), "r"(ph2), "r"(smem_u32(b3)), "r"(ph3)
+      : "memory");
+  return r;
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
@@ -150,36 +170,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-
-// 2^x for pairs of x <= 2^8 on the FMA pipe: x = n + f with n the nearest integer (its bits fall out of adding
-// 1.5 * 2^23) and |f| <= 1/2, a polynomial for 2^f (minimax in relative error, Remez exchange: degree 3
-// 7.5e-5, 3% of bf16's half step; degree 4 2.7e-6, 1% of fp16's half step), n added to its exponent.
-// Below 2^-126: about 2^-126, and so only where no weight may be exactly zero.
-template <typename T>
-__device__ __forceinline__ void exp2_pair(float x0, float x1, float& e0, float& e1) {
-  x0 = fmaxf(x0, -126.f);
-  x1 = fmaxf(x1, -126.f);
-  const uint64_t x = two(x0, x1);
-  const uint64_t t = add2(x, two(12582912.f, 12582912.f));
-  const uint64_t n = add2(t, two(-12582912.f, -12582912.f));
-  const uint64_t f = fma2(n, two(-1.f, -1.f), x);
-  uint64_t p;
-  if constexpr (std::is_same<T, __half>::value) {
-    p = fma2(f, two(0.009570102207362652f, 0.009570102207362652f), two(0.05591785907745361f, 0.05591785907745361f));
-    p = fma2(p, f, two(0.240247443318367f, 0.240247443318367f));
-    p = fma2(p, f, two(0.6931217908859253f, 0.6931217908859253f));
-    p = fma2(p, f, two(0.9999992847442627f, 0.9999992847442627f));
-  } else {
-    p = fma2(f, two(0.0551716685295105f, 0.0551716685295105f), two(0.2426111251115799f, 0.2426111251115799f));
-    p = fma2(p, f, two(0.6932609677314758f, 0.6932609677314758f));
-    p = fma2(p, f, two(0.9999280571937561f, 0.9999280571937561f));
-  }
-  float t0, t1, p0, p1;
-  untwo(t, t0, t1);
-  untwo(p, p0, p1);
-  e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
 // What every warp of a CTA derives alike for one group of TILES row tiles.
@@ -349,7 +339,6 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
   if (warp < SW) {
     // -------------------------------------------------------------- softmax, tile t, one row a thread
-    if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
     const uint32_t t_s = tmem + t * KEYS + lanes, t_o = tmem + TILES * KEYS + t * D + lanes;
@@ -388,13 +377,15 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
             for (int i = 0; i < KEYS; ++i) s[i] = i <= n ? s[i] : -CUDART_INF_F;
           }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
+          float mx[8];
 #pragma unroll
-          for (int i = 4; i < KEYS; i += 8) {
+          for (int e = 0; e < 8; ++e) mx[e] = s[e];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = i + 4 < KEYS ? max3(mx[e], s[i + e], s[i + 4 + e]) : max3(mx[e], s[i + e], s[i + e]);
+          for (int i = 8; i < KEYS; i += 16) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx[e] = i + 8 < KEYS ? max3(mx[e], s[i + e], s[i + 8 + e]) : max3(mx[e], s[i + e], s[i + e]);
           }
-          mx[0] = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
+          mx[0] = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], mx[7]));
           // false where both are -inf; a NaN takes the row for good
           const bool move = (mx[0] - m) * c > 8.f || mx[0] != mx[0];
           if (__any_sync(0xffffffffu, move)) {
@@ -426,23 +417,18 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           const uint64_t sub2 = two(kLift<T> - from * c, kLift<T> - from * c);
           uint64_t sum[2] = {0, 0};
           // weights, in eights of pairs: the first three quarters are handed on while the last is computed
-          // MODE 0: all keys seen, some exponentials by exp2_pair; 1: masked; 2: far scores
-          auto weights = [&](auto mode, int first, int to) {
-            constexpr int MODE = decltype(mode)::value;
+          // (all of them by the special-function pipe: a quarter or half by a polynomial on the FMA pipe took 1 and
+          // 5% longer)
+          auto weights = [&](auto is_far, int first, int to) {
 #pragma unroll
             for (int g = first; g < to; g += 16) {
               uint32_t p[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                float x0, x1, e0, e1;
+                float x0, x1;
                 const uint64_t s2 = two(s[g + 2 * i], s[g + 2 * i + 1]);
-                untwo(MODE < 2 ? fma2(s2, c2, sub2) : fma2(add2(s2, from2), c2, lift2), x0, x1);
-                if (MODE == 0 && (i & 3) == 3) {
-                  exp2_pair<T>(x0, x1, e0, e1);
-                } else {
-                  e0 = exp2_ftz(x0);
-                  e1 = exp2_ftz(x1);
-                }
+                untwo(decltype(is_far)::value ? fma2(add2(s2, from2), c2, lift2) : fma2(s2, c2, sub2), x0, x1);
+                const float e0 = exp2_ftz(x0), e1 = exp2_ftz(x1);
                 sum[i & 1] = add2(sum[i & 1], two(e0, e1));
                 p[i] = pack2<T>(e0, e1);
               }
@@ -451,11 +437,9 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           };
           auto part = [&](int first, int to) {
             if (far)
-              weights(std::integral_constant<int, 2>{}, first, to);
-            else if (masked)
-              weights(std::integral_constant<int, 1>{}, first, to);
+              weights(std::true_type{}, first, to);
             else
-              weights(std::integral_constant<int, 0>{}, first, to);
+              weights(std::false_type{}, first, to);
           };
           part(0, S::kEarly);
           tmem_st_wait();
@@ -565,7 +549,6 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       next_group(group);
     }
   } else {
-    if constexpr (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     int loads = 0;  // K and V tiles so far: use i of the ring is in stage i % NS
     if (warp == SW) {
       // ------------------------------------------------------------ products
@@ -613,25 +596,30 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           for (int j = 0; j < blocks; ++j) {
             const int vs = ks + 1 == NS ? 0 : ks + 1;
             ks = vs + 1 == NS ? 0 : vs + 1;
-            if (w.guarded(w.b0 + j)) {
-              wait_bar(v_ok + vs, (ph_v >> vs) & 1, a.status);
-              ph_v ^= 1u << vs;
-            } else {
-              wait_tile(vs);
-            }
-            bool next = j + 1 < blocks;  // its K tile has not been waited for yet
+            const bool guarded = w.guarded(w.b0 + j);
+            bool v_due = true, next = j + 1 < blocks;  // V's, the next K's tile: not seen to be there yet
             const uint64_t vd = v_desc + (uint64_t)(vs * (S::kStage >> 4));
+            auto take_v = [&](bool ready) {
+              if (!ready) wait_bar(guarded ? v_ok + vs : kv_full + vs, ((guarded ? ph_v : ph_full) >> vs) & 1, a.status);
+              (guarded ? ph_v : ph_full) ^= 1u << vs;
+              v_due = false;
+            };
+            auto take_k = [&](bool ready) {
+              if (!ready) wait_bar(kv_full + ks, (ph_full >> ks) & 1, a.status);
+              ph_full ^= 1u << ks;
+              next = false;
+            };
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
               if (j >= w.count[t]) continue;
-              wait_bar(p_early + t, ph_p[t], a.status);
+              const uint32_t there = test_bars(p_early + t, ph_p[t], p_late + t, ph_p[t], guarded ? v_ok + vs : kv_full + vs,
+                                               ((guarded ? ph_v : ph_full) >> vs) & 1, kv_full + ks, (ph_full >> ks) & 1);
+              if (v_due) take_v(there & 4);
+              if (!(there & 1)) wait_bar(p_early + t, ph_p[t], a.status);
               tc_fence_after();
               pv(t, vd, 0, S::kEarly / 16, j == 0);
-              if (next) {
-                wait_tile(ks);
-                next = false;
-              }
-              wait_bar(p_late + t, ph_p[t], a.status);
+              if (next) take_k(there & 8);
+              if (!(there & 2)) wait_bar(p_late + t, ph_p[t], a.status);
               ph_p[t] ^= 1;
               tc_fence_after();
               pv(t, vd, S::kEarly / 16, KEYS / 16, false);
@@ -640,8 +628,9 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               else
                 umma_commit(s_full + t);
             }
+            if (v_due) take_v(false);
+            if (next) take_k(false);
             umma_commit(kv_empty + vs);
-            if (next) wait_tile(ks);
             if (j + 1 < blocks) umma_commit(kv_empty + ks);
           }
         }
