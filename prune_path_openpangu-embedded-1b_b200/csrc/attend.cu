@@ -673,8 +673,8 @@ extern "C" int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t 
   }
   const Plan p = plan_of(tokens, q_heads, kv_heads, head_dim, batch, max_new, max_length);
   const size_t need = plan_bytes(p, tokens, q_heads, head_dim);
-  if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)) {
-    set_error("ppmoe_attend: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, ws ? ws_bytes : 0);
+  if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 32)) {
+    set_error("ppmoe_attend: workspace of %zu bytes (32-byte aligned) needed, %zu given", need, ws ? ws_bytes : 0);
     return PPMOE_ERR_WORKSPACE;
   }
   a.q = q;
@@ -694,6 +694,7 @@ extern "C" int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t 
   a.q_wide = on(q, q_t, q_h, 2);
   a.q_wide16 = on(q, q_t, q_h, 8);
   a.o_wide = on(out, o_t, o_h, 8);
+  a.o_wide32 = on(out, o_t, o_h, 16);
   a.nsplit = p.nsplit;
   a.part_o = static_cast<float*>(ws);
   a.part_ml = a.part_o + (size_t)p.nsplit * tokens * q_heads * head_dim;

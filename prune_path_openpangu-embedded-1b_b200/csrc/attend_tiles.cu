@@ -226,6 +226,12 @@ struct RowWalk {
   }
 };
 
+// 32 bytes at once.
+__device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
 template <typename T, int D, int TILES, int KEYS>
 __global__ void __launch_bounds__(TilesShape<D, TILES, KEYS>::kThreads, TilesShape<D, TILES, KEYS>::kCtas)
 attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -461,90 +467,61 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         const bool listed = *reinterpret_cast<volatile int*>(any_odd) != 0;
         const float inv = a.nsplit > 1 ? 1.f : l > 0.f ? 1.f / l : l == l ? 0.f : l;
-        // Through the q tile's place (no product reads it any more) to whole rows in memory: results in one go,
-        // parts in two halves of the columns.
-        uint8_t* stage = smem + t * S::kQ;
-        const int per = a.nsplit > 1 ? D / 2 : D;  // columns of one go
-        constexpr int W = D / 2;                   // ... that a thread holds at once
+        const int64_t token = sq.first + tok;
+        const int h = kvh * a.group + r - tok * a.group;
+        const int64_t at = ((int64_t)split * a.tokens + token) * a.q_heads + h;
+        T* out = static_cast<T*>(a.out) + token * a.o_t + h * a.o_h;
+        constexpr int W = D / 2;  // columns held at once
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += per) {
-#pragma unroll 1
-          for (int i = c0; i < c0 + per; i += W) {
-            float o[W];
-            if (count > 0) {
+        for (int i = 0; i < D; i += W) {
+          float o[W];
+          if (count > 0) {
 #pragma unroll
-              for (int e = 0; e < W; e += 32) tmem_ld32_async(t_o + i + e, o + e);
-              tmem_ld_wait();
+            for (int e = 0; e < W; e += 32) tmem_ld32_async(t_o + i + e, o + e);
+            tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < W; e += 32) tmem_ld_bind(o + e);
-            } else {
-#pragma unroll
-              for (int e = 0; e < W; ++e) o[e] = 0.f;
-            }
-            if (listed) {
-#pragma unroll 1
-              for (int e = 0; e < W; ++e) {
-                float add = 0.f;
-                if (odd[D + i + e] <= lim) add += CUDART_INF_F;
-                if (odd[2 * D + i + e] <= lim) add -= CUDART_INF_F;
-                if (odd[i + e] <= lim) add = CUDART_NAN_F;
-                if (!(add == 0.f)) {
-#pragma unroll
-                  for (int z = 0; z < W; ++z) o[z] = z == e ? o[z] + add : o[z];
-                }
-              }
-            }
-            uint8_t* line = stage + row * (D * 2);
-            if (a.nsplit == 1) {
-#pragma unroll
-              for (int e = 0; e < W; e += 8)
-                *reinterpret_cast<uint4*>(line + ((((i + e) / 8) ^ (row & 7)) << 4)) =
-                    make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv),
-                               pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
-            } else {
-#pragma unroll
-              for (int e = 0; e < W; e += 4)
-                *reinterpret_cast<float4*>(line + ((((i - c0 + e) / 4) ^ (row & 7)) << 4)) =
-                    make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            }
-          }
-          named_bar_sync(1 + t, kTileRows);
-          const int ch = row % CH;
-          const uint8_t* from = stage + (row / CH) * (D * 2);
-          auto chunk = [&](int i) {
-            const int rr = row / CH + i * STEP;
-            return *reinterpret_cast<const uint4*>(from + i * STEP * (D * 2) + ((ch ^ (rr & 7)) << 4));
-          };
-          if (a.nsplit > 1) {
-            RowWalk to(base + row / CH, STEP, a.group, (int64_t)a.q_heads * D, D);
-            float* part = a.part_o + (((int64_t)split * a.tokens + sq.first) * a.q_heads + kvh * a.group) * D + c0 + ch * 4;
-#pragma unroll 4
-            for (int i = 0; i < CH; ++i, to.step())
-              if (base + row / CH + i * STEP < rows) *reinterpret_cast<uint4*>(part + to.off) = chunk(i);
+            for (int e = 0; e < W; e += 32) tmem_ld_bind(o + e);
           } else {
-            RowWalk to(base + row / CH, STEP, a.group, a.o_t, a.o_h);
-            T* out = static_cast<T*>(a.out) + sq.first * a.o_t + (int64_t)kvh * a.group * a.o_h + ch * 8;
-            if (a.o_wide) {
-#pragma unroll 4
-              for (int i = 0; i < CH; ++i, to.step())
-                if (base + row / CH + i * STEP < rows) *reinterpret_cast<uint4*>(out + to.off) = chunk(i);
-            } else {
-#pragma unroll 1
-              for (int i = 0; i < CH; ++i, to.step()) {
-                if (base + row / CH + i * STEP >= rows) continue;
-                const uint4 v = chunk(i);
-                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t*>(out + to.off)[e] = (uint16_t)(u[e / 2] >> (16 * (e & 1)));
+            for (int e = 0; e < W; ++e) o[e] = 0.f;
+          }
+          if (listed) {
+#pragma unroll 1
+            for (int e = 0; e < W; ++e) {
+              float add = 0.f;
+              if (odd[D + i + e] <= lim) add += CUDART_INF_F;
+              if (odd[2 * D + i + e] <= lim) add -= CUDART_INF_F;
+              if (odd[i + e] <= lim) add = CUDART_NAN_F;
+              if (!(add == 0.f)) {
+#pragma unroll
+                for (int z = 0; z < W; ++z) o[z] = z == e ? o[z] + add : o[z];
               }
             }
           }
-          if (c0 + per < D) named_bar_sync(1 + t, kTileRows);
+          if (r < rows) {  // whole 32-byte sectors of this thread's row
+            if (a.nsplit > 1) {
+#pragma unroll
+              for (int e = 0; e < W; e += 8) {
+                uint32_t v[8];
+#pragma unroll
+                for (int z = 0; z < 8; ++z) v[z] = __float_as_uint(o[e + z]);
+                st_global32(a.part_o + at * D + i + e, v);
+              }
+            } else if (a.o_wide32) {
+#pragma unroll
+              for (int e = 0; e < W; e += 16) {
+                uint32_t v[8];
+#pragma unroll
+                for (int z = 0; z < 8; ++z) v[z] = pack2<T>(o[e + 2 * z] * inv, o[e + 2 * z + 1] * inv);
+                st_global32(out + i + e, v);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < W; ++e) out[i + e] = from_f32<T>(o[e] * inv);
+            }
+          }
         }
-        if (a.nsplit > 1 && r < rows) {
-          const int64_t at = ((int64_t)split * a.tokens + sq.first + tok) * a.q_heads + kvh * a.group + r - tok * a.group;
-          *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m * c, l);
-        }
+        if (a.nsplit > 1 && r < rows) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m * c, l);
       }
       next_group(group);
     }

@@ -90,7 +90,7 @@ class RotaryEmbedding:
             raise ValueError(f"base={base} must be positive and finite")
         self.head_dim, self.rotary_dim, self.layout = head_dim, rotary_dim, layout
         self.gain = 1.0
-        pair = torch.arange(rotary_dim // 2, dtype=torch.float64)
+        pairs = range(rotary_dim // 2)
         sc = dict(scaling or {})
         kind = sc.pop("type", None)
         if scaling is not None and kind not in ("linear", "ntk", "yarn"):
@@ -102,9 +102,9 @@ class RotaryEmbedding:
             if rotary_dim == 2:
                 raise ValueError("ntk scaling needs rotary_dim > 2")
             base = base * factor ** (rotary_dim / (rotary_dim - 2))
-        freq = base ** (-2.0 * pair / rotary_dim)
+        freq = [base ** (-2.0 * i / rotary_dim) for i in pairs]
         if kind == "linear":
-            freq = freq / factor
+            freq = [f / factor for f in freq]
         elif kind == "yarn":
             if "original_length" not in sc or base == 1.0:
                 raise ValueError("yarn scaling needs original_length, and a base other than 1")
@@ -117,14 +117,15 @@ class RotaryEmbedding:
                 return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
 
             low, high = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rotary_dim - 1)
-            keep = 1.0 - ((pair - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
-            freq = freq * keep + freq / factor * (1.0 - keep)
+            keep = [1.0 - min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0) for i in pairs]
+            freq = [f * k + f / factor * (1.0 - k) for f, k in zip(freq, keep)]
             self.gain = float(sc.pop("gain", 0.1 * math.log(factor) + 1.0))
         if sc:
             raise ValueError(f"unknown scaling entries {sorted(sc)}")
-        self.turns = freq / (2.0 * math.pi)
+        turns = [f / (2.0 * math.pi) for f in freq]
+        self.turns = torch.tensor(turns, dtype=torch.float64)
         self._c = _lib.Rotation(rotary_dim, layout == "interleaved", self.gain)
-        self._c.turns[:rotary_dim // 2] = self.turns.tolist()
+        self._c.turns[:rotary_dim // 2] = turns
 
     @property
     def _ptr(self) -> int:  # (of this object's own structure: copies have theirs)

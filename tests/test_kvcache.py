@@ -62,7 +62,7 @@ def test_host_validation_without_gpu():
     assert attend(batch=1 << 20) == -2 and attend(tokens=1 << 30) == -2
     n = lib.ppmoe_attend_workspace_bytes(1, 4, 2, 64, 1, 1, 64 * 1024)
     assert n > 0 and attend(length=64 * 1024) == -5 and attend(length=64 * 1024, ws=1024, n=n - 1) == -5
-    assert attend(length=64 * 1024, ws=1032, n=n) == -5 and b"workspace" in lib.ppmoe_last_error()
+    assert attend(length=64 * 1024, ws=1040, n=n) == -5 and b"workspace" in lib.ppmoe_last_error()
     for odd in [(0, 4, 2, 64, 1, 1, 64), (1, 4, 0, 64, 1, 1, 64), (1, 1, 2, 64, 1, 1, 64), (1, 4, 2, 64, 0, 1, 64)]:
         assert lib.ppmoe_attend_workspace_bytes(*odd) == 0
     assert lib.ppmoe_attend_workspace_bytes(1, 4, 2, 64, 1, -5, -7) == lib.ppmoe_attend_workspace_bytes(1, 4, 2, 64, 1, 1, 1)
