@@ -37,25 +37,32 @@ def _enter(device: torch.device):
 
 
 class _Rotate(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, emb, q, k, positions):
-        ctx.emb = emb
-        ctx.save_for_backward(positions)
-        ctx.set_materialize_grads(False)
-        q2, k2 = emb._launch(q, k, positions, False)
-        return q2, k2
+    """The rotation by the positions' angles or, inverse, by their negatives; each is the other's gradient."""
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def forward(ctx, emb, q, k, positions, inverse):
+        ctx.emb, ctx.inverse = emb, inverse
+        ctx.save_for_backward(positions)
+        ctx.set_materialize_grads(False)
+        return emb._launch(q, k, positions, inverse)
+
+    @staticmethod
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
-        dq, dk = (g if ctx.needs_input_grad[i] else None for i, g in ((1, dq), (2, dk)))
-        if dq is None and dk is None:
-            return None, None, None, None
-        if dq is None:
-            return None, None, ctx.emb._launch(dk, None, positions, True)[0], None
-        dq, dk = ctx.emb._launch(dq, dk, positions, True)
-        return None, dq, dk, None
+        _, need_q, need_k, _, _ = ctx.needs_input_grad
+        if not need_q:
+            dq = None
+        if not need_k:
+            dk = None
+        first = dk if dq is None else dq
+        if first is None:
+            return None, None, None, None, None
+        rest = None if dq is None else dk
+        if torch.is_grad_enabled():  # a gradient of the gradient is wanted
+            a, b = _Rotate.apply(ctx.emb, first, rest, positions, not ctx.inverse)
+        else:
+            a, b = ctx.emb._launch(first, rest, positions, not ctx.inverse)
+        return (None, None, a, None, None) if dq is None else (None, a, b, None, None)
 
 
 class RotaryEmbedding:
@@ -75,6 +82,8 @@ class RotaryEmbedding:
 
     The object holds numbers only (``turns``: turns per position of each pair, fp64 on the host);
     a captured launch keeps its own copy of them.  bf16, fp16 and fp32; values are rounded once.
+    To capture a backward pass into a CUDA graph, let no eager graph of the same leaves live: autograd would
+    wait for the stream that one was made on, which a capture does not allow.
     """
 
     def __init__(self, head_dim: int, *, rotary_dim: Optional[int] = None, base: float = 10000.0,
@@ -138,7 +147,7 @@ class RotaryEmbedding:
         own number of heads; or None).  ``positions [(batch,) tokens]`` or ``[tokens]``, int64 or int32.
         Any strides with contiguous heads; differentiable in ``q`` and ``k``."""
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-            return _Rotate.apply(self, q, k, positions)
+            return _Rotate.apply(self, q, k, positions, False)
         return self._launch(q, k, positions, False)
 
     def rotate_(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor) -> None:

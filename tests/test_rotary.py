@@ -213,6 +213,48 @@ def test_gradients_of_broadcast_and_partial_use(cuda):
 
 
 @pytest.mark.gpu
+def test_second_gradients(cuda):
+    """The gradient is linear in the incoming one, and its own gradient the rotation again."""
+    e = emb(64, scaling={"type": "yarn", "factor": 4.0, "original_length": 64})
+    pos = torch.arange(7, device=cuda) * 13
+    q = data((7, 2, 64), torch.float32, cuda, 1).requires_grad_()
+    k = data((7, 1, 64), torch.float32, cuda, 2).requires_grad_()
+    wq, wk = (data(s, torch.float32, cuda, i).requires_grad_() for i, s in ((3, (7, 2, 64)), (4, (7, 1, 64))))
+    dq, dk = torch.autograd.grad(e(q, k, pos), (q, k), (wq, wk), create_graph=True)
+    vq, vk = data((7, 2, 64), torch.float32, cuda, 5), data((7, 1, 64), torch.float32, cuda, 6)
+    gq, gk = torch.autograd.grad((dq, dk), (wq, wk), (vq, vk))
+    assert_rotation(gq, *exact_rotation(e, vq, pos))
+    assert_rotation(gk, *exact_rotation(e, vk, pos))
+
+
+@pytest.mark.gpu
+def test_captured_training_step(cuda):
+    """Forward and backward in a captured graph (no eager graph of the same leaves lives meanwhile), and the
+    check that saved positions have not been written to."""
+    e = emb(64)
+    pos = torch.arange(9, device=cuda)
+    q = data((9, 2, 64), torch.bfloat16, cuda, 1).requires_grad_()
+    k = data((9, 1, 64), torch.bfloat16, cuda, 2).requires_grad_()
+    wq, wk = data((9, 2, 64), torch.bfloat16, cuda, 3), data((9, 1, 64), torch.bfloat16, cuda, 4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # warm-up, as a capture of autograd wants it
+        torch.autograd.grad(e(q, k, pos), (q, k), (wq, wk))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(e(q, k, pos), (q, k), (wq, wk))
+    pos += 5
+    graph.replay()
+    for g, w in zip(got, (wq, wk)):
+        assert_rotation(g, *exact_rotation(e, w, pos, inverse=True))
+    out = e(q, k, pos)
+    pos -= 5
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, (q, k), (wq, wk))
+
+
+@pytest.mark.gpu
 def test_streams_and_capture(cuda):
     e = emb(128)
     q, k = data((64, 12, 128), torch.bfloat16, cuda, 1), data((64, 12, 128), torch.bfloat16, cuda, 2)
