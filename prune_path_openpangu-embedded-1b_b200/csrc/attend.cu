@@ -669,8 +669,8 @@ extern "C" int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t 
     set_error("ppmoe_attend: null pointer");
     return PPMOE_ERR_INVALID_ARG;
   }
-  if (!std::isfinite(scale)) {
-    set_error("ppmoe_attend: scale is not finite");
+  if (!std::isfinite(scale * 1.4426950408889634f)) {
+    set_error("ppmoe_attend: scale (times log2 e) is not finite");
     return PPMOE_ERR_INVALID_ARG;
   }
   const Plan p = plan_of(tokens, q_heads, kv_heads, head_dim, batch, max_new, max_length);
@@ -693,7 +693,6 @@ extern "C" int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t 
   auto on = [](const void* x, int64_t s1, int64_t s2, int n) {
     return reinterpret_cast<uintptr_t>(x) % (2 * n) == 0 && s1 % n == 0 && s2 % n == 0;
   };
-  a.q_wide = on(q, q_t, q_h, 2);
   a.q_wide16 = on(q, q_t, q_h, 8);
   a.o_wide = on(out, o_t, o_h, 8);
   a.o_wide32 = on(out, o_t, o_h, 16);

@@ -17,8 +17,7 @@ struct AttendArgs {
   int tokens, q_heads, group;
   float c;         // |scale| log2 e (1 where scale is 0)
   int q_sign;      // -1, 0, 1: what q is multiplied by
-  int q_wide;      // rows of q start on 4-byte boundaries
-  int q_wide16;    // ... on 16-byte boundaries
+  int q_wide16;    // rows of q start on 16-byte boundaries
   int o_wide;      // rows of out start on 16-byte boundaries
   int o_wide32;    // ... on 32-byte boundaries
   int nsplit;      // parts of the keys; above 1 they meet in ws
@@ -35,8 +34,7 @@ __device__ __forceinline__ float exp2_ftz(float x) {
   return y;
 }
 
-// Sequence b as the kernels see it: its first packed row, its new rows, its length held to what the
-// table can name (reported), and to what `tokens` rows can hold.
+// Sequence b as the kernels see it: its first packed row, its new rows (held to the rows there are), its length.
 struct Seq {
   int first, rows, length;
 };
@@ -50,12 +48,11 @@ __device__ __forceinline__ Seq load_seq(const AttendArgs& a, int b) {
   s.rows = end - s.first;
   return s;
 }
-// Position of the sequence's first new row; keys a row at position pos may see.
+// The positions of a sequence that its table can name.
 __device__ __forceinline__ int key_cap(const AttendArgs& a, int length) {
   const int64_t cap = (int64_t)a.seqs.max_pages << a.pages.page_shift;
   return length < cap ? length : (int)cap;
 }
-
 
 // C rounded values of one row piece, scaled by inv.
 template <typename T, int C>

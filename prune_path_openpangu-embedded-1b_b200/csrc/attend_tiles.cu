@@ -10,6 +10,8 @@
 // reach 2^8, which fp32 sums and both 16-bit types hold; m cancels in the end), so the
 // sums are rescaled seldom.  That needs no wait: S_t(j) comes after O_t += W_t(j-1) V(j-1).
 // K and V tiles arrive by TMA, a box per page and 64 columns, in one ring.
+// Two more warps look after V tiles that some row sees in part: rows past the last key become
+// zero (pages end inside a tile), values that are not finite are taken out and listed.
 //
 // Long contexts are bound by the chain score -> softmax -> product of each tile, which the other tile's overlaps:
 // 3000 cycles a block of 128 keys, of which the tensor pipe is busy for 2048 (62% measured, the special
@@ -18,8 +20,6 @@
 // products' warp for each tile (1283 us: the tiles' products interleave and both softmaxes wait at once),
 // persistent CTAs with the next item's loads ahead (1033, and prompts of 512 44-48 us for 41), part of the
 // exponentials as polynomials.  Short prompts are bound by a CTA's start and end (7 + 3 thousand cycles).
-// Two more warps look after V tiles that some row sees in part: rows past the last key become
-// zero (pages end inside a tile), values that are not finite are taken out and listed.
 #include <cuda.h>
 #include <mutex>
 #include "attend.cuh"

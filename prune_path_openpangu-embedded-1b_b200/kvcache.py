@@ -192,13 +192,13 @@ class PagedKVCache:
             so = (Hq * D, D)
         else:
             so = self._out(out, q)
+        scale = D ** -0.5 if scale is None else float(scale)
         lib = _lib.load()
-        back = _enter(self.device)
         n = lib.ppmoe_attend_workspace_bytes(T, Hq, self.kv_heads, D, batch[4], new, length)
         ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-        rc = lib.ppmoe_attend(self._ptr, q.data_ptr(), sq[0], sq[1], Hq, T, *batch, D ** -0.5 if scale is None else float(scale),
-                              new, length, out.data_ptr(), so[0], so[1], None if ws is None else ws.data_ptr(), n,
-                              _stream(self.device))
+        back = _enter(self.device)
+        rc = lib.ppmoe_attend(self._ptr, q.data_ptr(), sq[0], sq[1], Hq, T, *batch, scale, new, length, out.data_ptr(),
+                              so[0], so[1], None if ws is None else ws.data_ptr(), n, _stream(self.device))
         if back is not None:
             torch.cuda.set_device(back)
         if rc:

@@ -58,7 +58,7 @@ def test_host_validation_without_gpu():
     assert append(mp=0) == -1 and append(starts=None) == -1 and append(k=None) == -1
     assert append(rot=66) == -2 and append(rot=3) == -2
     assert attend(hq=3) == -1 and attend(hq=0) == -1 and attend(q=None) == -1
-    assert attend(scale=math.inf) == -1 and attend(scale=math.nan) == -1
+    assert attend(scale=math.inf) == -1 and attend(scale=math.nan) == -1 and attend(scale=3e38) == -1
     assert attend(batch=1 << 20) == -2 and attend(tokens=1 << 30) == -2
     n = lib.ppmoe_attend_workspace_bytes(1, 4, 2, 64, 1, 1, 64 * 1024)
     assert n > 0 and attend(length=64 * 1024) == -5 and attend(length=64 * 1024, ws=1024, n=n - 1) == -5
