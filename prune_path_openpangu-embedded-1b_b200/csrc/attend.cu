@@ -17,8 +17,8 @@
 namespace ppmoe {
 
 // ======================================================================== few rows
-// Up to 16 or 32 rows at a time per (sequence, kv head): one token per sequence up to a few.  Bound by
-// the cache's bytes.  Each warp takes 32 (or 16) keys at a time through a ring of its own (cp.async, no block
+// Up to 16 rows at a time per (sequence, kv head), or 32 of 64 values: one token per sequence up to a few.  Bound by
+// the cache's bytes.  Each warp takes 32 keys at a time through a ring of its own (cp.async, no block
 // barrier), m16n8k16 products (rows padded to 16: the tensor pipe has room, it is the loads that
 // count), and the warps' and then the parts' (m, l, sum) are joined at the end.
 // 64 ragged sequences of up to 8192 keys move 1.144 GB (counted: 1.143 read) in 190 us, 6.0 TB/s; two of 131071
@@ -28,10 +28,11 @@ namespace ppmoe {
 // 2 x 3 (2) 220, 4 x 3 (1) 235, 1 x 2 (6) 229 (before the clusters).
 constexpr int kThinWarps = 2;
 
-template <int D, int MT>  // MT: row tiles of 16
+template <int D, int MT>  // MT: row tiles of 16 (two of 64 values: with 128 the sums alone fill the registers)
 struct ThinShape {
-  static constexpr int kKeys = MT == 2 && D == 128 ? 16 : 32;  // (registers: 128 for the sums alone)
-  static constexpr int kStages = MT == 1 && D == 128 ? 2 : 3;
+  static_assert(MT == 1 || D == 64, "one row tile of 128 values");
+  static constexpr int kKeys = 32;
+  static constexpr int kStages = D == 128 ? 2 : 3;
   static constexpr int kCtas = 3;  // per SM
   static constexpr int kTile = kKeys * D * 2;          // bytes of K (or V) of one stage
   static constexpr int kWarp = kStages * 2 * kTile;    // bytes of one warp's ring
@@ -541,7 +542,10 @@ static Plan make_plan(int tokens, int q_heads, int kv_heads, int head_dim, int b
   auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
   const int64_t rows = (int64_t)max_new * (q_heads / kv_heads), base = (int64_t)batch * kv_heads;
   Plan p;
-  if (rows <= 32) {
+  // Few rows, where the other kernel's tiles would be empty for the most part: 24 ragged sequences x 5 tokens over up to
+  // 4000 keys, in us, here and there: 20 rows of 64 values 23 and 39; of 128 (8 kv heads) 65 (two row
+  // tiles at once, 16 keys at a time) and 57.
+  if (rows <= (head_dim == 64 ? 32 : 16)) {
     // Up to two CTAs an SM a part may be as short as 128 keys (one block of each warp): there latency
     // counts; beyond, parts of 768 keys or more, up to 1184 CTAs, so that ragged lengths even out.
     p.tiles = 0;
@@ -608,7 +612,11 @@ static int launch(AttendArgs& a, const Plan& p, cudaStream_t st) {
   if (p.tiles) {
     if (int rc = attend_tiles_launch(a, D, 1 << a.pages.page_shift, std::is_same<T, __half>::value, p.tiles, p.groups, st)) return rc;
   } else {
-    const int rc = p.groups == 1 ? launch_thin<T, D, 1>(a, st) : launch_thin<T, D, 2>(a, st);
+    int rc;
+    if constexpr (D == 64)
+      rc = p.groups == 1 ? launch_thin<T, D, 1>(a, st) : launch_thin<T, D, 2>(a, st);
+    else
+      rc = launch_thin<T, D, 1>(a, st);
     if (rc) return rc;
   }
   if (joins(p)) {
