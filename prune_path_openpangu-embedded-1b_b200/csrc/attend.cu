@@ -557,14 +557,14 @@ static Plan make_plan(int tokens, int q_heads, int kv_heads, int head_dim, int b
     // (A CTA goes on to further groups where there are fewer CTAs than groups: batches so wide that most
     // of a larger grid would find nothing to do.)
     // One tile to a CTA (two CTAs to an SM) for few rows, and for so few keys that a CTA's start and end weigh more
-    // than its loop: 16 prompts of 256, 12 heads of 128, in us: 20.6 with one, 24.7 with two; of 512: 41 and 41; 4 of
-    // 2048: 83 and 71.
-    p.tiles = rows <= 128 || max_length <= 384 ? 1 : 2;
+    // than its loop: prompts of 12 heads of 128, in us, with one and with two: 16 of 256 20.7 and 24.7, 16 of 512 39 and
+    // 41 (of 64: 31 and 35), 8 of 1024 50.5 and 49.9, 4 of 2048 72.8 and 69.2; 2048 rows over 34816 keys 1134 and 999.
+    p.tiles = rows <= 128 || max_length <= 768 ? 1 : 2;
     p.groups = (int)std::min(up(rows, 128 * p.tiles), std::max<int64_t>(1, (1 << 18) / base));
     // Parts where they fill the last wave better than they cost: measured us of a block of keys and of a CTA's start
     // and end, and the parts' way through memory at 5 TB/s (2048 rows x 32 heads: 1030 us in one part, 1085 in four,
     // so a gain of less than a tenth is left alone).
-    const double block = p.tiles == 2 ? 1.65 : 1.32, ends = p.tiles == 2 ? 6. : 5.;
+    const double block = p.tiles == 2 ? 1.65 : 1.07, ends = p.tiles == 2 ? 6. : 5.;
     const int64_t slots = p.tiles == 2 ? 148 : 296, blocks = up(max_length, 64 * p.tiles);
     double best = 0.;
     for (int n = 1; n <= 32 && (n == 1 || n * 512 <= max_length); ++n) {

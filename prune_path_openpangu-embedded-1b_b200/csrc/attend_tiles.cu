@@ -9,6 +9,8 @@
 // reference maximum m of a row moves only when a tile's maximum exceeds it by 2^8 (weights then
 // reach 2^8, which fp32 sums and both 16-bit types hold; m cancels in the end), so the
 // sums are rescaled seldom.  That needs no wait: S_t(j) comes after O_t += W_t(j-1) V(j-1).
+// CTAs of one row tile (few rows, short prompts; two CTAs to an SM) take 64 keys at a time and have two S tiles in turn:
+// the next scores are computed while the softmax is at the last ones.
 // K and V tiles arrive by TMA, a box per page and 64 columns, in one ring.
 // Two more warps look after V tiles that some row sees in part: rows past the last key become
 // zero (pages end inside a tile), values that are not finite are taken out and listed.
@@ -16,9 +18,9 @@
 // Long contexts are bound by the chain score -> softmax -> product of each tile, which the other tile's overlaps:
 // 3000 cycles a block of 128 keys, of which the tensor pipe is busy for 2048 (62% measured, the special
 // function pipe 62%); over seconds the power limit takes another tenth.  2048 rows over 34816 keys, 32 query
-// and 8 kv heads of 128, bf16: 945 us cold, 1025 us sustained (1.2 and 1.1 PFLOP/s).  Tried and slower: a
+// and 8 kv heads of 128, bf16: 945 us cold, 1000-1025 us sustained (1.2 and 1.1 PFLOP/s).  Tried and slower: a
 // products' warp for each tile (1283 us: the tiles' products interleave and both softmaxes wait at once),
-// persistent CTAs with the next item's loads ahead (1033, and prompts of 512 44-48 us for 41), part of the
+// persistent CTAs with the next item's loads ahead (1033; prompts of 512 44-48 us for 41), part of the
 // exponentials as polynomials.  Short prompts are bound by a CTA's start and end (7 + 3 thousand cycles).
 #include <cuda.h>
 #include <mutex>
@@ -38,10 +40,12 @@ struct TilesShape {
   static constexpr int kStage = KEYS * D * 2;   // a K or V tile, the same way
   static constexpr int kStages = D == 128 ? (TILES == 2 ? 5 : 4) : (TILES == 2 ? 8 : 10);
   static constexpr int kBars = TILES * kQ + kStages * kStage;
-  static constexpr int kNumBars = 4 * kStages + 8;
+  static constexpr int kNumBars = 4 * kStages + 10;
   static constexpr int kList = kBars + ((kNumBars * 8 + 16 + 15) / 16) * 16;  // [3][D] ints
   static constexpr int kBytes = kList + 3 * D * 4 + 1024;
-  static constexpr int kTmem = TILES * (KEYS + D) > 256 ? 512 : 256;  // columns: S tiles, then O tiles
+  static constexpr int kO = 2 * KEYS;           // TMEM columns: two S tiles (of both row tiles; of one, in turn), then O tiles
+  static constexpr int kTmem = TILES == 2 ? 512 : 256;
+  static_assert(kO + TILES * D <= kTmem, "TMEM");
   static constexpr int kEarly = KEYS / 4 * 3;  // keys whose weights are handed on first
 };
 
@@ -253,6 +257,8 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // for a barrier waits for every phase of it.
   uint64_t *kv_full = bars, *kv_empty = bars + NS, *g_full = bars + 2 * NS, *v_ok = bars + 3 * NS;
   uint64_t *s_full = bars + 4 * NS, *p_early = s_full + 2, *p_late = s_full + 4, *q_full = s_full + 6;
+  // one tile: after each product with V (waited for only by whoever must, see there), and after the last
+  uint64_t *pv_done = s_full + 8, *o_full = s_full + 9;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::kNumBars);
   int* any_odd = reinterpret_cast<int*>(tmem_slot + 1);
   int* odd = reinterpret_cast<int*>(smem + S::kList);  // [nan, +inf, -inf][D]: first key with one in that column
@@ -325,6 +331,8 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         mbar_init(p_late + t, kTileRows);
         mbar_init(q_full + t, kTileRows);
       }
+      mbar_init(pv_done, 1);
+      mbar_init(o_full, 1);
       *any_odd = 0;
       fence_mbar_init();
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
@@ -355,9 +363,11 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     // -------------------------------------------------------------- softmax, tile t, one row a thread
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
-    const uint32_t t_s = tmem + t * KEYS + lanes, t_o = tmem + TILES * KEYS + t * D + lanes;
+    const uint32_t t_s0 = tmem + t * KEYS + lanes, t_o = tmem + S::kO + t * D + lanes;
     const float c = a.c;
-    uint32_t ph_s = 0;
+    uint32_t ph_s = 0;  // two tiles: the phase of s_full
+    uint32_t ph_o = 0;
+    int done = 0;       // one tile: blocks so far; block n has S tile n % 2
 #pragma unroll 1
     for (int64_t group = group_of; group * kRows < rows; group += groups_hint) {
       const Group<TILES, KEYS> w(a, group, rows, pos0, cap, split);
@@ -376,8 +386,11 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll 1
         for (int j = 0; j < count; ++j) {
           float s[KEYS];
-          wait_bar(s_full + t, ph_s, a.status);
+          const int at_s = TILES == 1 ? done & 1 : t;  // S tile and its barriers
+          const uint32_t t_s = TILES == 1 ? t_s0 + at_s * KEYS : t_s0;
+          wait_bar(s_full + at_s, TILES == 1 ? (done >> 1) & 1 : ph_s, a.status);
           ph_s ^= 1;
+          ++done;
           tc_fence_after();
 #pragma unroll
           for (int i = 0; i < KEYS; i += 32) tmem_ld32_async(t_s + i, s + i);
@@ -404,6 +417,12 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           const bool move = (mx[0] - m) * c > 8.f || mx[0] != mx[0];
           if (__any_sync(0xffffffffu, move)) {
             if (j > 0) {
+              if constexpr (TILES == 1) {
+                // The product of block done - 2.  Its phase is the one running or the one before: the product before it came
+                // before these scores, the one after it needs this thread's weights.
+                wait_bar(pv_done, (done - 2) & 1, a.status);
+                tc_fence_after();
+              }
               const float f = move ? exp2_ftz((m - mx[0]) * c) : 1.f;
               l *= f;
 #pragma unroll 1
@@ -458,19 +477,24 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           part(0, S::kEarly);
           tmem_st_wait();
           tc_fence_before();
-          mbar_arrive(p_early + t);
+          mbar_arrive(p_early + at_s);
           part(S::kEarly, KEYS);
           tmem_st_wait();
           tc_fence_before();
-          mbar_arrive(p_late + t);
+          mbar_arrive(p_late + at_s);
           float l0, l1;
           untwo(add2(sum[0], sum[1]), l0, l1);
           l += l0 + l1;
         }
         // the sums
         if (count > 0) {
-          wait_bar(s_full + t, ph_s, a.status);
-          ph_s ^= 1;
+          if constexpr (TILES == 1) {
+            wait_bar(o_full, ph_o, a.status);
+            ph_o ^= 1;
+          } else {
+            wait_bar(s_full + t, ph_s, a.status);
+            ph_s ^= 1;
+          }
           tc_fence_after();
         }
         const bool listed = *reinterpret_cast<volatile int*>(any_odd) != 0;
@@ -540,6 +564,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       constexpr uint32_t id_s = idesc_of<T>(KEYS, false), id_o = idesc_of<T>(D, true);
       const uint64_t q_desc = umma_desc_sw128(smem_u32(smem)), k_desc = umma_desc_sw128(ring), v_desc = desc_v<KEYS>(ring);
       uint32_t ph_p[TILES] = {}, ph_q[TILES] = {}, ph_full = 0, ph_v = 0;  // the last two: a bit a stage
+      int done = 0;  // one tile: blocks so far
 #pragma unroll 1
       for (int64_t group = group_of; group * kRows < rows; group += groups_hint) {
         const Group<TILES, KEYS> w(a, group, rows, pos0, cap, split);
@@ -549,18 +574,19 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             wait_bar(kv_full + st, (ph_full >> st) & 1, a.status);
             ph_full ^= 1u << st;
           };
-          auto qk = [&](int t, int st) {
+          // S tile i = q tile t times the K tile in a stage; O tile t += W tile i times a V tile
+          auto qk = [&](int t, int i, int st) {
             const uint64_t qd = q_desc + (uint64_t)(t * (S::kQ >> 4)), kd = k_desc + (uint64_t)(st * (S::kStage >> 4));
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-              umma_bf16(tmem + t * KEYS, qd + (((k >> 2) * (kTileRows * 128) + (k & 3) * 32) >> 4),
+              umma_bf16(tmem + i * KEYS, qd + (((k >> 2) * (kTileRows * 128) + (k & 3) * 32) >> 4),
                         kd + (((k >> 2) * (KEYS * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
-            umma_commit(s_full + t);
+            umma_commit(s_full + i);
           };
-          auto pv = [&](int t, uint64_t vd, int from, int to, bool fresh) {
+          auto pv = [&](int t, int i, uint64_t vd, int from, int to, bool fresh) {
 #pragma unroll
             for (int k = from; k < to; ++k)
-              umma_ts(tmem + TILES * KEYS + t * D, tmem + t * KEYS + k * 8, vd + k * 128, id_o, !fresh || k > 0);
+              umma_ts(tmem + S::kO + t * D, tmem + i * KEYS + k * 8, vd + k * 128, id_o, !fresh || k > 0);
           };
 #pragma unroll
           for (int t = 0; t < TILES; ++t) {
@@ -568,55 +594,94 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             wait_bar(q_full + t, ph_q[t], a.status);
             ph_q[t] ^= 1;
           }
-          int ks = loads % NS;  // stage of the next K tile
-          if (blocks > 0) {
-            wait_tile(ks);
-            tc_fence_after();
-#pragma unroll
-            for (int t = 0; t < TILES; ++t)
-              if (w.count[t] > 0) qk(t, ks);
-            umma_commit(kv_empty + ks);
-          }
+          if constexpr (TILES == 1) {
+            // One row tile has no other to fill its softmax's time; its next scores are computed ahead, into the other S tile.
+            auto k_stage = [&](int j) { return (loads + 2 * j) % NS; };
 #pragma unroll 1
-          for (int j = 0; j < blocks; ++j) {
-            const int vs = ks + 1 == NS ? 0 : ks + 1;
-            ks = vs + 1 == NS ? 0 : vs + 1;
-            const bool guarded = w.guarded(w.b0 + j);
-            bool v_due = true, next = j + 1 < blocks;  // V's, the next K's tile: not seen to be there yet
-            const uint64_t vd = v_desc + (uint64_t)(vs * (S::kStage >> 4));
-            auto take_v = [&](bool ready) {
-              if (!ready) wait_bar(guarded ? v_ok + vs : kv_full + vs, ((guarded ? ph_v : ph_full) >> vs) & 1, a.status);
-              (guarded ? ph_v : ph_full) ^= 1u << vs;
-              v_due = false;
-            };
-            auto take_k = [&](bool ready) {
-              if (!ready) wait_bar(kv_full + ks, (ph_full >> ks) & 1, a.status);
-              ph_full ^= 1u << ks;
-              next = false;
-            };
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-              if (j >= w.count[t]) continue;
-              const uint32_t there = test_bars(p_early + t, ph_p[t], p_late + t, ph_p[t], guarded ? v_ok + vs : kv_full + vs,
-                                               ((guarded ? ph_v : ph_full) >> vs) & 1, kv_full + ks, (ph_full >> ks) & 1);
-              if (v_due) take_v(there & 4);
-              if (!(there & 1)) wait_bar(p_early + t, ph_p[t], a.status);
+            for (int j = 0; j < 2 && j < blocks; ++j) {
+              wait_tile(k_stage(j));
               tc_fence_after();
-              pv(t, vd, 0, S::kEarly / 16, j == 0);
-              if (next) take_k(there & 8);
-              if (!(there & 2)) wait_bar(p_late + t, ph_p[t], a.status);
-              ph_p[t] ^= 1;
-              tc_fence_after();
-              pv(t, vd, S::kEarly / 16, KEYS / 16, false);
-              if (j + 1 < w.count[t])
-                qk(t, ks);
-              else
-                umma_commit(s_full + t);
+              qk(0, (done + j) & 1, k_stage(j));
+              umma_commit(kv_empty + k_stage(j));
             }
-            if (v_due) take_v(false);
-            if (next) take_k(false);
-            umma_commit(kv_empty + vs);
-            if (j + 1 < blocks) umma_commit(kv_empty + ks);
+#pragma unroll 1
+            for (int j = 0; j < blocks; ++j, ++done) {
+              const int at_s = done & 1, ph = (done >> 1) & 1, vs = (loads + 2 * j + 1) % NS, ks = k_stage(j + 2);
+              const bool guarded = w.guarded(w.b0 + j);
+              uint64_t* v_bar = guarded ? v_ok + vs : kv_full + vs;
+              const uint32_t v_ph = ((guarded ? ph_v : ph_full) >> vs) & 1;
+              (guarded ? ph_v : ph_full) ^= 1u << vs;
+              const uint32_t there = test_bars(p_early + at_s, ph, p_late + at_s, ph, v_bar, v_ph, kv_full + ks, (ph_full >> ks) & 1);
+              if (!(there & 4)) wait_bar(v_bar, v_ph, a.status);
+              if (!(there & 1)) wait_bar(p_early + at_s, ph, a.status);
+              tc_fence_after();
+              const uint64_t vd = v_desc + (uint64_t)(vs * (S::kStage >> 4));
+              pv(0, at_s, vd, 0, S::kEarly / 16, j == 0);
+              if (!(there & 2)) wait_bar(p_late + at_s, ph, a.status);
+              tc_fence_after();
+              pv(0, at_s, vd, S::kEarly / 16, KEYS / 16, false);
+              umma_commit(pv_done);
+              if (j + 1 == blocks) umma_commit(o_full);
+              umma_commit(kv_empty + vs);
+              if (j + 2 < blocks) {
+                if (!(there & 8)) wait_bar(kv_full + ks, (ph_full >> ks) & 1, a.status);
+                ph_full ^= 1u << ks;
+                tc_fence_after();
+                qk(0, at_s, ks);
+                umma_commit(kv_empty + ks);
+              }
+            }
+          } else {
+            int ks = loads % NS;  // stage of the next K tile
+            if (blocks > 0) {
+              wait_tile(ks);
+              tc_fence_after();
+#pragma unroll
+              for (int t = 0; t < TILES; ++t)
+                if (w.count[t] > 0) qk(t, t, ks);
+              umma_commit(kv_empty + ks);
+            }
+#pragma unroll 1
+            for (int j = 0; j < blocks; ++j) {
+              const int vs = ks + 1 == NS ? 0 : ks + 1;
+              ks = vs + 1 == NS ? 0 : vs + 1;
+              const bool guarded = w.guarded(w.b0 + j);
+              bool v_due = true, next = j + 1 < blocks;  // V's, the next K's tile: not seen to be there yet
+              const uint64_t vd = v_desc + (uint64_t)(vs * (S::kStage >> 4));
+              auto take_v = [&](bool ready) {
+                if (!ready) wait_bar(guarded ? v_ok + vs : kv_full + vs, ((guarded ? ph_v : ph_full) >> vs) & 1, a.status);
+                (guarded ? ph_v : ph_full) ^= 1u << vs;
+                v_due = false;
+              };
+              auto take_k = [&](bool ready) {
+                if (!ready) wait_bar(kv_full + ks, (ph_full >> ks) & 1, a.status);
+                ph_full ^= 1u << ks;
+                next = false;
+              };
+#pragma unroll
+              for (int t = 0; t < TILES; ++t) {
+                if (j >= w.count[t]) continue;
+                const uint32_t there = test_bars(p_early + t, ph_p[t], p_late + t, ph_p[t], guarded ? v_ok + vs : kv_full + vs,
+                                                 ((guarded ? ph_v : ph_full) >> vs) & 1, kv_full + ks, (ph_full >> ks) & 1);
+                if (v_due) take_v(there & 4);
+                if (!(there & 1)) wait_bar(p_early + t, ph_p[t], a.status);
+                tc_fence_after();
+                pv(t, t, vd, 0, S::kEarly / 16, j == 0);
+                if (next) take_k(there & 8);
+                if (!(there & 2)) wait_bar(p_late + t, ph_p[t], a.status);
+                ph_p[t] ^= 1;
+                tc_fence_after();
+                pv(t, t, vd, S::kEarly / 16, KEYS / 16, false);
+                if (j + 1 < w.count[t])
+                  qk(t, t, ks);
+                else
+                  umma_commit(s_full + t);
+              }
+              if (v_due) take_v(false);
+              if (next) take_k(false);
+              umma_commit(kv_empty + vs);
+              if (j + 1 < blocks) umma_commit(kv_empty + ks);
+            }
           }
         }
         __syncwarp();
