@@ -24,7 +24,17 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-_NONE = (0, 0, 0, 0)
+_POSITIONS = (torch.int64, torch.int32)
+_NONE = (0, 0, 0)
+
+
+def _heads(x: torch.Tensor, four: bool):
+    """x with contiguous heads, and its (batch, token, head) strides."""
+    s = x.stride()
+    if s[-1] != 1:
+        x = x.contiguous()
+        s = x.stride()
+    return x, s if four else (0, *s)
 
 
 def _enter(device: torch.device):
@@ -162,60 +172,46 @@ class RotaryEmbedding:
         self._launch(q, k, positions, False, (q, k))
 
     def _launch(self, q, k, positions, inverse, out=None):
-        dev, shape, dt = q.device, q.shape, q.dtype
+        dev, shape, dt, D = q.device, q.shape, q.dtype, self.head_dim
         if dev.type != "cuda":
             raise RuntimeError("RotaryEmbedding runs on CUDA only; got a tensor on " + str(dev))
-        n = len(shape)
-        if n not in (3, 4) or shape[-1] != self.head_dim:
-            raise ValueError(f"q must be [(batch,) tokens, heads, {self.head_dim}], got {list(shape)}")
+        four = len(shape) == 4
+        if not (four or len(shape) == 3) or shape[-1] != D:
+            raise ValueError(f"q must be [(batch,) tokens, heads, {D}], got {list(shape)}")
+        B, L, Hq = shape[:3] if four else (1, *shape[:2])
         code = _DTYPES.get(dt)
         if code is None:
             raise TypeError(f"RotaryEmbedding takes bf16, fp16 or fp32, got {dt}")
+        at = positions.shape
+        if positions.device != dev or positions.dtype not in _POSITIONS:
+            raise ValueError(f"positions must be int64 or int32 on {dev}, got {positions.dtype} on {positions.device}")
+        if at != (L,) and not (four and at == (B, L)):
+            raise ValueError(f"positions {list(at)} do not go with q {list(shape)}")
+        pb, pt = positions.stride() if len(at) == 2 else (0, positions.stride(0))
+        q, sq = _heads(q, four)
+        qo = out[0] if out else torch.empty_like(q, memory_format=torch.contiguous_format)
+        so = (L * Hq * D, Hq * D, D)
+        kp, sk, ko, sko, Hk, k2 = None, _NONE, None, _NONE, 0, None
         if k is not None:
             ks = k.shape
-            if k.dtype is not dt or k.device != dev or ks[:-2] != shape[:-2] or ks[-1] != self.head_dim:
+            Hk = ks[-2] if len(ks) == len(shape) else -1
+            if k.dtype is not dt or k.device != dev or ks != ((B, L, Hk, D) if four else (L, Hk, D)):
                 raise ValueError(f"k {list(ks)} {k.dtype} on {k.device} does not go with q {list(shape)} {dt} on {dev}")
-        if positions.device != dev or positions.dtype not in (torch.int64, torch.int32):
-            raise ValueError(f"positions must be int64 or int32 on {dev}, got {positions.dtype} on {positions.device}")
-        if positions.shape != shape[:-2] and positions.shape != shape[-3:-2]:
-            raise ValueError(f"positions {list(positions.shape)} do not go with q {list(shape)}")
-        sq = q.stride()
-        if sq[-1] != 1:
-            q = q.contiguous()
-            sq = q.stride()
-        B, L, Hq = (shape[0] if n == 4 else 1), shape[-3], shape[-2]
-        sk, Hk, k2, sk2 = _NONE, 0, None, _NONE
-        if k is not None:
-            sk, Hk = k.stride(), ks[-2]
-            if sk[-1] != 1:
-                k = k.contiguous()
-                sk = k.stride()
-        if out is None:
-            q2 = torch.empty_like(q, memory_format=torch.contiguous_format)
-            sq2 = (L * Hq * self.head_dim, Hq * self.head_dim, self.head_dim, 1)
-            if k is not None:
-                k2 = torch.empty_like(k, memory_format=torch.contiguous_format)
-                sk2 = (L * Hk * self.head_dim, Hk * self.head_dim, self.head_dim, 1)
-        else:
-            q2, k2 = out
-            sq2 = sq if n == 4 else (0, *sq)
-            if k2 is not None:
-                sk2 = sk if n == 4 else (0, *sk)
-            if q2.data_ptr() != q.data_ptr() or (k is not None and k2.data_ptr() != k.data_ptr()):
+            k, sk = _heads(k, four)
+            k2 = out[1] if out else torch.empty_like(k, memory_format=torch.contiguous_format)
+            sko = (L * Hk * D, Hk * D, D)
+            kp, ko = k.data_ptr(), k2.data_ptr()
+        if out:
+            so, sko = sq, sk
+            if qo.data_ptr() != q.data_ptr() or kp != ko:
                 raise ValueError("rotate_ needs contiguous heads")
-        if n == 3:
-            sq = (0, *sq)
-            if k is not None:
-                sk = (0, *sk)
-        pb, pt = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
         back = _enter(dev)
         rc = _lib.load().ppmoe_rotary(
-            self._ptr, inverse, q.data_ptr(), sq[0], sq[1], sq[2], q2.data_ptr(), sq2[0], sq2[1], sq2[2], Hq,
-            None if k is None else k.data_ptr(), sk[0], sk[1], sk[2], None if k is None else k2.data_ptr(),
-            sk2[0], sk2[1], sk2[2], Hk, B, L, self.head_dim, positions.data_ptr(),
+            self._ptr, inverse, q.data_ptr(), sq[0], sq[1], sq[2], qo.data_ptr(), so[0], so[1], so[2], Hq, kp,
+            sk[0], sk[1], sk[2], ko, sko[0], sko[1], sko[2], Hk, B, L, D, positions.data_ptr(),
             positions.dtype is torch.int64, pb, pt, code, _stream(dev))
         if back is not None:
             torch.cuda.set_device(back)
         if rc:
             raise _lib.PPMoEError("ppmoe_rotary", rc, _lib.load().ppmoe_last_error().decode())
-        return q2, k2
+        return qo, k2
