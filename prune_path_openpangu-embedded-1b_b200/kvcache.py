@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .rotary import _NONE, RotaryEmbedding, _enter, _stream
+from .rotary import _NONE, RotaryEmbedding, _enter, _stream, _written
 
 __all__ = ["PagedKVCache"]
 
@@ -51,6 +51,8 @@ class PagedKVCache:
         cls._check(k.shape[2], k.shape[3], k.dtype)
         if k.numel() == 0:
             raise ValueError("the cache has no pages")
+        if k.requires_grad or v.requires_grad:
+            raise ValueError("the cache writes into its tensors: they cannot require gradients")
         for t in (k, v):
             if t.stride(3) != 1 or any(s % 8 or s == 0 for n, s in zip(t.shape[:3], t.stride()) if n > 1) or t.data_ptr() % 16:
                 raise ValueError("cache tensors need contiguous heads, 16-byte alignment and strides of whole 16 bytes")
@@ -177,8 +179,8 @@ class PagedKVCache:
         ``h // (q_heads / kv_heads)``).  A row at a negative position gives zeros; rows outside every
         sequence are not written.  ``max_new`` / ``max_length``: the most new rows and the greatest length of
         a sequence as far as the host knows (default: the largest possible); they choose how the work is
-        laid out, never what is computed.  ``scale`` defaults to ``head_dim ** -0.5``.  ``out`` may be ``q``.  Records no gradients, and
-        refuses rows that ask for one."""
+        laid out, never what is computed.  ``scale`` defaults to ``head_dim ** -0.5``.  ``out`` may be ``q``.
+        Records no gradients, and refuses rows that ask for one."""
         q, sq = self._rows("q", q)
         T, Hq, D = q.shape
         if Hq < 1 or Hq % self.kv_heads:
@@ -211,6 +213,7 @@ class PagedKVCache:
             raise ValueError(f"out must be {list(q.shape)} {q.dtype} on {q.device} with contiguous heads")
         if any(n > 1 and x == 0 for n, x in zip(out.shape, s)):
             raise ValueError("out repeats elements")
+        _written(out)
         return s
 
     def check_device_status(self) -> None:

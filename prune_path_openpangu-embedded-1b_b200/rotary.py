@@ -28,6 +28,14 @@ _POSITIONS = (torch.int64, torch.int32)
 _NONE = (0, 0, 0)
 
 
+def _written(x: torch.Tensor) -> None:
+    """Tells autograd that a kernel writes into ``x``, so that a backward pass that saved it complains."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("a tensor that requires a gradient cannot be written to: use torch.no_grad()")
+    if not x.is_inference():
+        torch.autograd.graph.increment_version(x)
+
+
 def _heads(x: torch.Tensor, four: bool):
     """x with contiguous heads, and its (batch, token, head) strides."""
     s = x.stride()
@@ -163,12 +171,13 @@ class RotaryEmbedding:
     def rotate_(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor) -> None:
         """The same in place (no gradients; ``q`` and ``k`` must not overlap)."""
         for x in (q, k):
-            if x is not None and torch.is_grad_enabled() and x.requires_grad:
-                raise RuntimeError("rotate_ records no gradients: call the embedding itself, or use torch.no_grad()")
             if x is not None and any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
                 raise ValueError("rotate_ needs tensors without repeated elements")
         if k is not None and k.untyped_storage().data_ptr() == q.untyped_storage().data_ptr() and k.data_ptr() == q.data_ptr():
             raise ValueError("rotate_ needs q and k of their own")
+        for x in (q, k):
+            if x is not None:
+                _written(x)
         self._launch(q, k, positions, False, (q, k))
 
     def _launch(self, q, k, positions, inverse, out=None):

@@ -469,6 +469,16 @@ def test_refusals(cuda):
         cache.append(q, k, k, *ok, rotary=emb(128))
     with pytest.raises(ValueError):
         cache.append(None, k, k, *ok, out=q)
+    with pytest.raises(RuntimeError):
+        cache.attend(q, *ok, out=torch.empty_like(q).requires_grad_())
+    with pytest.raises(ValueError):
+        type(cache).from_tensors(b.k.clone().requires_grad_(), b.v)
+    version = q._version
+    cache.attend(q, *ok, out=q)
+    assert q._version > version
+    with torch.inference_mode():
+        x = q * 1
+        cache.attend(x, *ok, out=x)
 
 
 # ------------------------------------------------------------------ GPU: together

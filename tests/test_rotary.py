@@ -166,6 +166,16 @@ def test_in_place(cuda):
         e.rotate_(ref, ref, pos)
     with pytest.raises(RuntimeError):
         e.rotate_(ref.clone().requires_grad_(), None, pos)
+    w = torch.ones(10, 7, 64, dtype=torch.float16, device=cuda, requires_grad=True)
+    x = ref.clone()
+    y = (w * x).sum()  # saves x
+    e.rotate_(x, None, pos)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        z = ref * 1
+        e.rotate_(z, None, pos)
+    assert torch.equal(z, x)
 
 
 @pytest.mark.gpu
