@@ -212,6 +212,8 @@ int ppmoe_decode(const void* x, int tokens, const void* packed, int hidden, int 
 // decode's griddepcontrol.wait also covers the previous decode (which used the same
 // workspace).  Overwriting x_dev early is safe: this grid starts only after every CTA of the
 // previous decode has signalled its dependents, which each does long after its rows landed.
+// (No other kernel of the library signals early unless one of its own launches follows: after any of them
+// this grid starts when that kernel has ended.)
 __global__ void x_stage_kernel(const uint4* src_host, uint4* __restrict__ dst, int n16) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int i = threadIdx.x; i < n16; i += blockDim.x) dst[i] = src_host[i];

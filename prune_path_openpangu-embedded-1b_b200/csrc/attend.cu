@@ -95,7 +95,7 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
   const int split = blockIdx.x % a.nsplit;
   const int kvh = (blockIdx.x / a.nsplit) % a.pages.kv_heads;
   const int b = blockIdx.x / (a.nsplit * a.pages.kv_heads);
-  pdl_launch_dependents();
+  if (a.joins) pdl_launch_dependents();
   const Seq sq = load_seq(a, b);
   if (sq.rows <= 0) return;
   const int cap = key_cap(a, sq.length);
@@ -619,7 +619,7 @@ static int launch(AttendArgs& a, const Plan& p, cudaStream_t st) {
       rc = launch_thin<T, D, 1>(a, st);
     if (rc) return rc;
   }
-  if (joins(p)) {
+  if (a.joins) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)((int64_t)a.tokens * a.q_heads));
     cfg.blockDim = dim3(kJoinWarps * 32);
@@ -705,6 +705,7 @@ extern "C" int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t 
   a.o_wide = on(out, o_t, o_h, 8);
   a.o_wide32 = on(out, o_t, o_h, 16);
   a.nsplit = p.nsplit;
+  a.joins = joins(p);
   a.part_o = static_cast<float*>(ws);
   a.part_ml = a.part_o + (size_t)p.nsplit * tokens * q_heads * head_dim;
   a.status = static_cast<uint32_t*>(cache->status);

@@ -21,6 +21,7 @@ struct AttendArgs {
   int o_wide;      // rows of out start on 16-byte boundaries
   int o_wide32;    // ... on 32-byte boundaries
   int nsplit;      // parts of the keys; above 1 they meet in ws
+  int joins;       // the next launch on the stream is attend_join_kernel, which may start early
   float* part_o;   // [nsplit][tokens][q_heads][D]: sum of 2^(x - m) v
   float* part_ml;  // [nsplit][tokens][q_heads][2]: m, l
   Seqs seqs;

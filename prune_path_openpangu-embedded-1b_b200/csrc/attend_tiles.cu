@@ -264,7 +264,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   int* odd = reinterpret_cast<int*>(smem + S::kList);  // [nan, +inf, -inf][D]: first key with one in that column
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_launch_dependents();
+  if (a.joins) pdl_launch_dependents();  // (anyone else's launch may write q or read out before its own wait)
   // blocks of work, the rows with most keys first: group (slowest, descending), sequence, kv head, part
   int x = blockIdx.x;
   const int split = x % a.nsplit;

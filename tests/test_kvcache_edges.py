@@ -1,0 +1,44 @@
+"""Paged cache and attention where they meet the rest of a program: launches behind them on the stream, autograd,
+values and sizes at the borders of what they take."""
+import pytest
+import torch
+
+from conftest import pkg
+from gpu_helpers import make_module
+from paged_helpers import Batch, assert_attention, exact_attention
+
+
+# ------------------------------------------------------------------ GPU: what follows on the stream
+@pytest.mark.gpu
+@pytest.mark.parametrize("shared", ["out", "q"])
+@pytest.mark.parametrize("seqs,new,length,hk,hints", [
+    (16, 1, 8000, 12, dict(max_new=1)),                    # few rows, parts that meet in clusters
+    (1, 16, 8000, 1, dict(max_new=1, max_length=1)),    # few rows, one CTA going through all of them
+    (1, 16, 8000, 1, dict(max_new=16, max_length=1)),   # tiles in one part
+    (1, 16, 8000, 1, dict(max_new=16, max_length=8000)),  # tiles whose parts are joined
+])
+def test_a_decode_from_host_memory_follows(cuda, shared, seqs, new, length, hk, hints):
+    """ppmoe_decode_host's staging copy starts before its wait; where its staging buffer is the attention's output
+    or queries, it has to come after the attention all the same."""
+    P = pkg()
+    b = Batch([new] * seqs, [length] * seqs, hk, 128, 64, torch.bfloat16, cuda, seed=21)
+    q = b.normal(12, 2.0)
+    want = exact_attention(b, q)
+    tokens = q.shape[0]
+    layer = P.synth.make_layer(8, 1536, 64, 96)
+    m = make_module(layer, 0.95, cuda)
+    x = P.synth.make_tokens(8, tokens, 1536)
+    ref = m.forward_decode(x.to(cuda)).cpu()
+    xh, oh = x.pin_memory(), torch.empty(tokens, 1536, dtype=torch.bfloat16).pin_memory()
+    out, od, ws = torch.empty_like(q), torch.empty(tokens, 1536, dtype=torch.bfloat16, device=cuda), m.workspace(tokens)
+    staging = out if shared == "out" else q
+    cache, s = b.cache(), torch.cuda.current_stream()
+    cache.attend(q, b.starts, b.lens, b.table, out=out, **hints)
+    P._lib.call("ppmoe_decode_host", xh.data_ptr(), tokens, m.packed().data_ptr(), 1536, 64, 96, 0.95, None, oh.data_ptr(),
+                staging.data_ptr(), od.data_ptr(), ws.data_ptr(), ws.numel(), s.cuda_stream)
+    s.synchronize()
+    m.check_device_status()
+    assert torch.equal(staging.view(tokens, 1536).cpu(), x)
+    assert torch.equal(oh, ref)
+    if shared == "q":
+        assert_attention(out, *want)
