@@ -161,6 +161,7 @@ class PagedKVCache:
             qp, op = q.data_ptr(), out.data_ptr()
         elif out is not None:
             raise ValueError("out without q")
+        _written(self._k, self._v)
         back = _enter(self.device)
         rc = _lib.load().ppmoe_kv_append(
             self._ptr, None if rotary is None else rotary._ptr, qp, sq[0], sq[1], op, so[0], so[1], Hq, k.data_ptr(),

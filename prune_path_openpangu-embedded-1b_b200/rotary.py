@@ -28,12 +28,12 @@ _POSITIONS = (torch.int64, torch.int32)
 _NONE = (0, 0, 0)
 
 
-def _written(x: torch.Tensor) -> None:
-    """Tells autograd that a kernel writes into ``x``, so that a backward pass that saved it complains."""
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("a tensor that requires a gradient cannot be written to: use torch.no_grad()")
-    if not x.is_inference():
-        torch.autograd.graph.increment_version(x)
+def _written(*tensors: torch.Tensor) -> None:
+    """Tells autograd that a kernel writes into these, so that a backward pass that saved one complains."""
+    for x in tensors:
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("a tensor that requires a gradient cannot be written to: use torch.no_grad()")
+    torch.autograd.graph.increment_version(tensors)  # (leaves inference tensors out)
 
 
 def _heads(x: torch.Tensor, four: bool):
@@ -175,9 +175,7 @@ class RotaryEmbedding:
                 raise ValueError("rotate_ needs tensors without repeated elements")
         if k is not None and k.untyped_storage().data_ptr() == q.untyped_storage().data_ptr() and k.data_ptr() == q.data_ptr():
             raise ValueError("rotate_ needs q and k of their own")
-        for x in (q, k):
-            if x is not None:
-                _written(x)
+        _written(*(x for x in (q, k) if x is not None))
         self._launch(q, k, positions, False, (q, k))
 
     def _launch(self, q, k, positions, inverse, out=None):

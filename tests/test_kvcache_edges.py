@@ -12,7 +12,7 @@ from paged_helpers import Batch, assert_attention, exact_attention
 @pytest.mark.gpu
 @pytest.mark.parametrize("shared", ["out", "q"])
 @pytest.mark.parametrize("seqs,new,length,hk,hints", [
-    (16, 1, 8000, 12, dict(max_new=1)),                    # few rows, parts that meet in clusters
+    (16, 1, 8000, 12, dict(max_new=1)),                 # few rows, parts that meet in clusters
     (1, 16, 8000, 1, dict(max_new=1, max_length=1)),    # few rows, one CTA going through all of them
     (1, 16, 8000, 1, dict(max_new=16, max_length=1)),   # tiles in one part
     (1, 16, 8000, 1, dict(max_new=16, max_length=8000)),  # tiles whose parts are joined
@@ -42,3 +42,23 @@ def test_a_decode_from_host_memory_follows(cuda, shared, seqs, new, length, hk, 
     assert torch.equal(oh, ref)
     if shared == "q":
         assert_attention(out, *want)
+
+
+# ------------------------------------------------------------------ GPU: autograd
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_append_tells_autograd(cuda, which):
+    """A backward pass that saved the cache's tensors (its own, or the given ones) must not use what an append wrote."""
+    b = Batch([2], [20], 1, 64, 16, torch.bfloat16, cuda, seed=22)
+    cache, k, v = b.cache(), b.normal(1), b.normal(1)
+    for saved in (getattr(cache, which), getattr(b, which)):
+        w = torch.ones_like(saved, requires_grad=True)
+        y = (w * saved).sum()
+        cache.append(None, k, v, b.starts, b.lens, b.table)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        cache.append(None, k, v, b.starts, b.lens, b.table)
+    cache.k.requires_grad_()
+    with pytest.raises(RuntimeError, match="no_grad"):
+        cache.append(None, k, v, b.starts, b.lens, b.table)
