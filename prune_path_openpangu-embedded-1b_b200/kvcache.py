@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .rotary import _NONE, RotaryEmbedding, _enter, _stream, _written
+from .rotary import _NONE, RotaryEmbedding, _enter, _has_tangent, _stream, _written
 
 __all__ = ["PagedKVCache"]
 
@@ -106,6 +106,8 @@ class PagedKVCache:
         """x and its strides, checked."""
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient, and the cache records none: call it under torch.no_grad()")
+        if _has_tangent(x):
+            raise RuntimeError(f"{name} has a forward-mode tangent, and the cache records none: pass its primal")
         shape = x.shape
         if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {self.head_dim}], got {list(shape)}")
@@ -140,7 +142,7 @@ class PagedKVCache:
         ``[tokens, kv_heads, head_dim]`` to their places, and returns ``q [tokens, q_heads, head_dim]``
         rotated likewise: a new tensor, or ``out`` (which may be ``q``).  ``q`` None returns None.  Rows
         outside every sequence are not written, in ``out`` neither.  The rows of one call must go to
-        different places.  Records no gradients, and refuses rows that ask for one."""
+        different places.  Records no derivatives, and refuses rows that ask for one."""
         k, sk = self._rows("k", k, self.kv_heads)
         v, sv = self._rows("v", v, self.kv_heads)
         T = k.shape[0]
@@ -181,7 +183,7 @@ class PagedKVCache:
         sequence are not written.  ``max_new`` / ``max_length``: the most new rows and the greatest length of
         a sequence as far as the host knows (default: the largest possible); they choose how the work is
         laid out, never what is computed.  ``scale`` defaults to ``head_dim ** -0.5``.  ``out`` may be ``q``.
-        Records no gradients, and refuses rows that ask for one."""
+        Records no derivatives, and refuses rows that ask for one."""
         q, sq = self._rows("q", q)
         T, Hq, D = q.shape
         if Hq < 1 or Hq % self.kv_heads:

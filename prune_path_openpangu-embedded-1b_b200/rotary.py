@@ -12,6 +12,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -28,11 +29,19 @@ _POSITIONS = (torch.int64, torch.int32)
 _NONE = (0, 0, 0)
 
 
+def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether forward-mode differentiation follows one of these (such a tensor requires no gradient)."""
+    return (forward_ad._current_level >= 0
+            and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors))
+
+
 def _written(*tensors: torch.Tensor) -> None:
     """Tells autograd that a kernel writes into these, so that a backward pass that saved one complains."""
     for x in tensors:
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("a tensor that requires a gradient cannot be written to: use torch.no_grad()")
+    if _has_tangent(*tensors):
+        raise RuntimeError("a tensor with a forward-mode tangent cannot be written to")
     torch.autograd.graph.increment_version(tensors)  # (leaves inference tensors out)
 
 
@@ -55,14 +64,27 @@ def _enter(device: torch.device):
 
 
 class _Rotate(torch.autograd.Function):
-    """The rotation by the positions' angles or, inverse, by their negatives; each is the other's gradient."""
+    """The rotation by the positions' angles or, inverse, by their negatives; each is the other's gradient.  It is
+    linear: tangents (forward mode) are rotated as the values are."""
 
     @staticmethod
     def forward(ctx, emb, q, k, positions, inverse):
         ctx.emb, ctx.inverse = emb, inverse
         ctx.save_for_backward(positions)
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(positions)
+            ctx.like = q.detach(), None if k is None else k.detach()
         ctx.set_materialize_grads(False)
         return emb._launch(q, k, positions, inverse)
+
+    @staticmethod
+    def jvp(ctx, _emb, tq, tk, _positions, _inverse):
+        (positions,) = ctx.saved_tensors
+        if tq is None:  # an output beside one with a tangent has one too
+            tq = torch.zeros_like(ctx.like[0])
+        if tk is None and ctx.like[1] is not None:
+            tk = torch.zeros_like(ctx.like[1])
+        return _Rotate.apply(ctx.emb, tq, tk, positions, ctx.inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -76,7 +98,7 @@ class _Rotate(torch.autograd.Function):
         if first is None:
             return None, None, None, None, None
         rest = None if dq is None else dk
-        if torch.is_grad_enabled():  # a gradient of the gradient is wanted
+        if torch.is_grad_enabled() or _has_tangent(first, rest):  # a derivative of the gradient is wanted
             a, b = _Rotate.apply(ctx.emb, first, rest, positions, not ctx.inverse)
         else:
             a, b = ctx.emb._launch(first, rest, positions, not ctx.inverse)
@@ -163,13 +185,14 @@ class RotaryEmbedding:
                  ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         """Rotated copies of ``q [(batch,) tokens, q_heads, head_dim]`` and ``k`` (same leading sizes, its
         own number of heads; or None).  ``positions [(batch,) tokens]`` or ``[tokens]``, int64 or int32.
-        Any strides with contiguous heads; differentiable in ``q`` and ``k``."""
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        Any strides with contiguous heads; differentiable in ``q`` and ``k``, in reverse and in forward mode."""
+        if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) or _has_tangent(q, k):
             return _Rotate.apply(self, q, k, positions, False)
         return self._launch(q, k, positions, False)
 
     def rotate_(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor) -> None:
-        """The same in place (no gradients; ``q`` and ``k`` must not overlap)."""
+        """The same in place (records no derivatives, and refuses tensors that ask for one; ``q`` and ``k`` must not
+        overlap)."""
         for x in (q, k):
             if x is not None and any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
                 raise ValueError("rotate_ needs tensors without repeated elements")

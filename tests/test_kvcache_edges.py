@@ -2,6 +2,7 @@
 values and sizes at the borders of what they take."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from conftest import pkg
 from gpu_helpers import make_module
@@ -62,3 +63,19 @@ def test_append_tells_autograd(cuda, which):
     cache.k.requires_grad_()
     with pytest.raises(RuntimeError, match="no_grad"):
         cache.append(None, k, v, b.starts, b.lens, b.table)
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused(cuda):
+    b = Batch([2], [20], 1, 64, 16, torch.bfloat16, cuda, seed=23)
+    cache, q, k, v = b.cache(), b.normal(2), b.normal(1), b.normal(1)
+    at = b.starts, b.lens, b.table
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x.clone(), torch.ones_like(x))  # noqa: E731
+        for call in (lambda: cache.attend(dual(q), *at), lambda: cache.append(dual(q), k, v, *at), lambda: cache.append(q, dual(k), v, *at),
+                     lambda: cache.append(q, k, dual(v), *at), lambda: cache.attend(q, *at, out=dual(q)),
+                     lambda: cache.append(q, k, v, *at, out=dual(q))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        cache.append(q, k, v, *at)
+        cache.attend(q, *at)
