@@ -394,7 +394,7 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
         const int64_t t = sq.first + tok;
         const int h = kvh * a.group + r - tok * a.group;
         const int64_t at = ((int64_t)split * a.tokens + t) * a.q_heads + h;
-        const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+        const float inv = inverse_sum(sum, pos0 + tok);
 #pragma unroll 1
         for (int c = col; c < col + C; c += 8) {
           float acc[8];
@@ -456,7 +456,7 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
         }
         const int tok = r / a.group;
         store_row<T, 8>(static_cast<T*>(a.out) + (sq.first + tok) * a.o_t + (int64_t)(kvh * a.group + r - tok * a.group) * a.o_h + c,
-                        acc, sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum, a.o_wide);
+                        acc, inverse_sum(sum, pos0 + tok), a.o_wide);
       }
       cluster_sync();  // every part has been read
     }
@@ -521,7 +521,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __gr
   l = 0.f;
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) l += s_l[w];
-  const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
+  int pos = 0;
+  if (l == 0.f) {  // (all threads alike)
+    const int b = find_seq_warp(a.seqs.starts, a.seqs.batch, t);
+    pos = a.seqs.lengths[b] - a.seqs.starts[b + 1] + t;
+  }
+  const float inv = inverse_sum(l, pos);
   T* out = static_cast<T*>(a.out) + t * a.o_t + h * a.o_h;
   for (int c = threadIdx.x; c < D; c += kJoinWarps * 32) {
     float v = 0.f;

@@ -55,6 +55,12 @@ __device__ __forceinline__ int key_cap(const AttendArgs& a, int length) {
   return length < cap ? length : (int)cap;
 }
 
+// What the sum of a row at position pos is multiplied by.  Its weights sum to 0 where it sees no key (its sum is 0 too)
+// and where every score that it sees is -inf: softmax has no answer there, so NaN.
+__device__ __forceinline__ float inverse_sum(float l, int pos) {
+  return l > 0.f ? 1.f / l : l == 0.f && pos < 0 ? 0.f : CUDART_NAN_F;
+}
+
 // C rounded values of one row piece, scaled by inv.
 template <typename T, int C>
 __device__ __forceinline__ void store_row(T* out, const float (&v)[C], float inv, bool wide) {

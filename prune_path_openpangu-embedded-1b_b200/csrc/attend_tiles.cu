@@ -498,7 +498,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           tc_fence_after();
         }
         const bool listed = *reinterpret_cast<volatile int*>(any_odd) != 0;
-        const float inv = a.nsplit > 1 ? 1.f : l > 0.f ? 1.f / l : l == l ? 0.f : l;
+        const float inv = a.nsplit > 1 ? 1.f : inverse_sum(l, pos0 + tok);
         const int64_t token = sq.first + tok;
         const int h = kvh * a.group + r - tok * a.group;
         const int64_t at = ((int64_t)split * a.tokens + token) * a.q_heads + h;

@@ -1,5 +1,7 @@
 """Paged cache and attention where they meet the rest of a program: launches behind them on the stream, autograd,
 values and sizes at the borders of what they take."""
+import math
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -79,3 +81,44 @@ def test_tangents_are_refused(cuda):
                 call()
         cache.append(q, k, v, *at)
         cache.attend(q, *at)
+
+
+# ------------------------------------------------------------------ GPU: values
+PLANS = [  # new rows, keys, hints: each way a call is laid out
+    pytest.param(1, 300, dict(max_new=1, max_length=1), id="few rows in one part"),
+    pytest.param(2, 900, dict(max_new=2, max_length=900), id="few rows in a cluster"),
+    pytest.param(3, 9000, dict(max_new=3, max_length=9000), id="few rows joined"),
+    pytest.param(70, 300, dict(max_new=70, max_length=300), id="one row tile"),
+    pytest.param(70, 300, dict(max_new=1, max_length=300), id="few rows, many times"),
+    pytest.param(60, 6000, dict(max_new=60, max_length=6000), id="one row tile joined"),
+    pytest.param(300, 900, dict(max_new=300, max_length=900), id="two row tiles"),
+    pytest.param(300, 900, dict(max_new=40, max_length=900), id="one row tile, groups in turn"),
+    pytest.param(300, 900, dict(max_new=70, max_length=900), id="two row tiles, groups in turn"),
+    pytest.param(300, 5000, dict(max_new=300, max_length=5000), id="two row tiles joined"),
+]
+
+
+def store(b, s):
+    """Sequence s's keys and values to its pages."""
+    pos = torch.arange(b.lengths[s], device=b.device)
+    at = b.table[s][pos // b.page].long(), slice(None), pos % b.page
+    b.k[at], b.v[at] = b.keys[s], b.values[s]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("new,length,hints", PLANS)
+def test_scores_of_minus_infinity(cuda, dtype, dim, new, length, hints):
+    """Rows that see such scores alone are NaN, as softmax has it; beside others these keys weigh nothing; a row
+    without keys stays 0."""
+    b = Batch([new, new, new, 2], [length, length, new, 1], 2, dim, 32, dtype, cuda, seed=24)
+    q = b.normal(4, 2.0)
+    q[..., 1] = q[..., 1].abs() + 0.5
+    b.keys[0][..., 1] = -math.inf              # every key
+    b.keys[1][:length - new // 2 - 1, 1, 1] = -math.inf  # one kv head; the last rows see others
+    b.keys[2][:new // 2, 0, 1] = -math.inf        # from the sequence's start
+    for s in range(3):
+        store(b, s)
+    out, size = exact_attention(b, q)
+    assert out[:new].isnan().all() and out[3 * new - 1].isfinite().all() and (out[-2] == 0).all() and out[-1].isfinite().all()
+    assert_attention(b.cache().attend(q, b.starts, b.lens, b.table, **hints), out, size)
