@@ -8,7 +8,7 @@ from torch.autograd import forward_ad
 
 from conftest import pkg
 from gpu_helpers import make_module
-from paged_helpers import Batch, assert_attention, exact_attention
+from paged_helpers import GARBAGE, Batch, assert_attention, exact_attention
 
 
 # ------------------------------------------------------------------ GPU: what follows on the stream
@@ -122,3 +122,83 @@ def test_scores_of_minus_infinity(cuda, dtype, dim, new, length, hints):
     out, size = exact_attention(b, q)
     assert out[:new].isnan().all() and out[3 * new - 1].isfinite().all() and (out[-2] == 0).all() and out[-1].isfinite().all()
     assert_attention(b.cache().attend(q, b.starts, b.lens, b.table, **hints), out, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("new,length,hints", PLANS)
+def test_values_that_are_not_finite(cuda, dtype, dim, new, length, hints):
+    """inf and NaN in places that rows of one tile, of both, of one part or of all see: they reach the rows that see
+    them, in their column, and no others."""
+    b = Batch([new, new, 3], [length, new, 40], 2, dim, 32, dtype, cuda, seed=25)
+    for s in (0, 1):
+        n = b.lengths[s]
+        p = n - new  # the first new row's position
+        marks = [[(n - 1, math.nan)], [(n - 1, math.inf)], [(p + new // 2, -math.inf)], [(p + min(10, new - 1), math.inf)],
+                 [(p, math.inf), (n - 1, -math.inf)], [(n // 3, math.inf)], [(n // 3, math.inf), (n - 1, -math.inf)],
+                 [(min(p + 70, n - 1), math.nan)], [(n // 2, math.nan)], [(n // 2, -math.inf), (min(p + 150, n - 1), -math.inf)]]
+        for column, places in enumerate(marks):
+            for at, value in places:
+                b.values[s][at, column % 2, column if column % 3 else dim - 1 - column] = value
+        store(b, s)
+    q = b.normal(4, 2.0)
+    out, size = exact_attention(b, q)
+    assert out.isnan().any() and out.isinf().any() and out[-3:].isfinite().all()
+    cache = b.cache()
+    assert_attention(cache.attend(q, b.starts, b.lens, b.table, **hints), out, size)
+    cache.check_device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,length,hints", PLANS)
+def test_keys_that_are_not_finite(cuda, new, length, hints):
+    """A NaN score makes the rows that see it NaN, one of +inf too (inf - inf); rows before them are as ever."""
+    b = Batch([new, new, new], [length, length, new], 1, 64, 16, torch.float16, cuda, seed=26)
+    q = b.normal(3, 2.0)
+    q[..., 9] = q[..., 9].abs() + 0.5
+    b.keys[0][length - (new + 1) // 2, 0, 9] = math.nan
+    b.keys[1][length // 2, 0, 9] = math.inf
+    b.keys[2][0, 0, 9] = math.nan
+    for s in range(3):
+        store(b, s)
+    out = b.cache().attend(q, b.starts, b.lens, b.table, **hints)
+    want = exact_attention(b, q)
+    for s, first in enumerate((length - (new + 1) // 2, length // 2, 0)):
+        first = max(first - (b.lengths[s] - new), 0)  # new rows before the key
+        assert out[s * new + first:(s + 1) * new].isnan().all()
+        assert_attention(out[s * new:s * new + first], *(x[s * new:s * new + first] for x in want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,length,hints", PLANS)
+def test_huge_scores(cuda, dtype, new, length, hints):
+    """Whole-number scores times 2^20: exact in fp32, up to 2^36; each row's weight is shared by its largest."""
+    b = Batch([new], [length], 1, 64, 64, dtype, cuda, seed=27)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    b.keys[0] = torch.randint(-32, 33, (length, 1, 64), generator=g, device=cuda).to(dtype)
+    store(b, 0)
+    q = torch.randint(-32, 33, (new, 2, 64), generator=g, device=cuda).to(dtype)
+    got = b.cache().attend(q, b.starts, b.lens, b.table, scale=2.0 ** 20, **hints)
+    assert_attention(got, *exact_attention(b, q, 2.0 ** 20))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,length,hints", PLANS)
+def test_a_missing_page(cuda, new, length, hints):
+    """Ids that the cache does not have are reported; the rows before them and the other sequences are as ever."""
+    P = pkg()
+    b = Batch([new, new], [length, length], 2, 64, 32, torch.bfloat16, cuda, seed=28)
+    cache, q = b.cache(), b.normal(4, 2.0)
+    want = exact_attention(b, q)
+    last = (length - 1) // 32
+    before = max(last * 32 - (length - new), 0)  # sequence 0's rows that do not reach its last page
+    for spoil in (GARBAGE, -1, b.k.shape[0]):
+        table = b.table.clone()
+        table[0, last] = spoil
+        out = cache.attend(q, b.starts, b.lens, table, **hints)
+        with pytest.raises(P._lib.PPMoEError, match="without a page"):
+            cache.check_device_status()
+        assert_attention(out[:before], *(x[:before] for x in want))
+        assert_attention(out[new:], *(x[new:] for x in want))
+    cache.check_device_status()
