@@ -11,7 +11,10 @@
 //
 // A masked key must not reach a row even where its value is not finite (0 * inf = NaN): tiles that
 // some row sees in part are searched for such values.  They are taken out of the product, and
-// added (they are what the sum becomes) to the rows that see their key.
+// added (they are what the sum becomes) to the rows that see their key.  In other tiles the product carries them, but an
+// infinity under a weight, or a running sum's factor, that vanished in its type becomes NaN there: sums that are NaN
+// over weights that are not are put right at the end from a list of the values that are not finite, so
+// that an answer does not depend on the tiles, parts and order it was computed in.
 #include "attend.cuh"
 
 namespace ppmoe {
@@ -108,6 +111,8 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
   float* j_o = reinterpret_cast<float*>(smem + S::kQ);  // [warps][R][D + 4]
   float* j_ml = j_o + kThinWarps * R * (D + 4);         // [warps][R][2]
   float* c_ml = j_ml + kThinWarps * R * 2;              // [R][2]: of all warps, for the cluster
+  const bool clustered = a.nsplit > 1 && a.nsplit <= kMaxCluster, joined = a.nsplit > kMaxCluster;  // how parts meet
+  static_assert(S::kQ >= 3 * D * 4, "room for the list of values that are not finite");
 
   for (int r0 = 0; r0 < rows; r0 += R) {
     const int last = r0 + R - 1 < rows ? r0 + R - 1 : rows - 1;
@@ -377,6 +382,7 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
       }
     }
     __syncthreads();
+    uint32_t mend = 0;  // which of this thread's pieces of 8 columns have sums that are NaN over weights that are not
     {
       constexpr int TPR = kThinWarps * 32 / R, C = D / TPR;  // threads of a row, columns of one thread
       const int row = tid / TPR, col = (tid % TPR) * C, r = r0 + row;
@@ -404,9 +410,10 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
 #pragma unroll
             for (int w = 0; w < kThinWarps; ++w) acc[i] += f[w] * j_o[(w * R + row) * (D + 4) + c + i];
           }
-          if (a.nsplit == 1) {
+          if (any_nan(acc) && (sum > 0.f || (sum == 0.f && joined))) mend |= 1u << ((c - col) / 8);
+          if (!clustered && !joined) {
             store_row<T, 8>(static_cast<T*>(a.out) + t * a.o_t + h * a.o_h + c, acc, inv, a.o_wide);
-          } else if (a.nsplit <= kMaxCluster) {  // (over what this thread alone has read)
+          } else if (clustered) {  // (over what this thread alone has read)
             *reinterpret_cast<float4*>(j_o + row * (D + 4) + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
             *reinterpret_cast<float4*>(j_o + row * (D + 4) + c + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
           } else {
@@ -415,13 +422,14 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
           }
         }
         if (a.nsplit > 1 && col == 0)
-          *reinterpret_cast<float2*>(a.nsplit <= kMaxCluster ? c_ml + row * 2 : a.part_ml + at * 2) = make_float2(top, sum);
+          *reinterpret_cast<float2*>(clustered ? c_ml + row * 2 : a.part_ml + at * 2) = make_float2(top, sum);
       }
     }
-    if (a.nsplit > 1 && a.nsplit <= kMaxCluster) {
+    if (clustered) {
+      mend = 0;
       cluster_sync();
       const int n = min(R, rows - r0) * (D / 8);  // pieces of 8 columns, shared out over the cluster's threads
-      for (int i = tid + split * kThinWarps * 32; i < n; i += a.nsplit * kThinWarps * 32) {
+      for (int i = tid + split * kThinWarps * 32, at = 1; i < n; i += a.nsplit * kThinWarps * 32, at <<= 1) {
         const int row = i / (D / 8), c = i % (D / 8) * 8, r = r0 + row;
         // (parts past the last read the last again and count nothing: all loads are in flight at once)
         float2 ml[kMaxCluster];
@@ -439,10 +447,9 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
         for (int w = 0; w < kMaxCluster; ++w) top = fmaxf(top, ml[w].x);
 #pragma unroll
         for (int w = 0; w < kMaxCluster; ++w) {
-          // a part without keys has a sum of 0 (one whose every score is NaN has a sum of NaN)
-          const bool real = w < a.nsplit && !(ml[w].x == -CUDART_INF_F && ml[w].y == 0.f);
+          // (a part without a score above -inf has sums of 0, or NaN where a score or a value made them so)
           const float f = ml[w].x == -CUDART_INF_F ? 1.f : exp2_ftz(ml[w].x - top);
-          if (real) {
+          if (w < a.nsplit) {
             sum += f * ml[w].y;
             acc[0] += f * x[w].x;
             acc[1] += f * x[w].y;
@@ -454,13 +461,28 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
             acc[7] += f * y[w].w;
           }
         }
+        if (any_nan(acc) && sum > 0.f) mend |= at;
         const int tok = r / a.group;
         store_row<T, 8>(static_cast<T*>(a.out) + (sq.first + tok) * a.o_t + (int64_t)(kvh * a.group + r - tok * a.group) * a.o_h + c,
                         acc, inverse_sum(sum, pos0 + tok), a.o_wide);
       }
       cluster_sync();  // every part has been read
     }
-    __syncthreads();  // before the next rows' copies
+    if (__syncthreads_or(mend != 0)) {  // (and before the next rows' copies)
+      int* list = reinterpret_cast<int*>(smem);  // where q was
+      const int from = joined ? min(split * per * KEYS, keys) : 0, to = joined ? min(blk_end * KEYS, keys) : keys;
+      list_values<T, D, kThinWarps * 32>(a, b, kvh, from, to, list);
+      for (int p = 0; mend >> p; ++p) {
+        if (!(mend >> p & 1)) continue;
+        constexpr int TPR = kThinWarps * 32 / R;
+        const int piece = clustered ? tid + (split + p * a.nsplit) * kThinWarps * 32 : 0;
+        const int row = clustered ? piece / (D / 8) : tid / TPR;
+        const int col = clustered ? piece % (D / 8) * 8 : tid % TPR * (D / TPR) + p * 8;
+        const int r = r0 + row;
+        mend_row<T, D>(a, list, sq.first, r, kvh, joined ? split : -1, min(pos0 + r / a.group, cap - 1), col, 8);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -532,6 +554,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const __gr
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) v += s_o[w][c];
+    if (v != v && l > 0.f) {  // an infinity in a part whose factor vanished, perhaps: it stays one
+      v = 0.f;
+      for (int s = 0; s < a.nsplit; ++s) {
+        const float ms = a.part_ml[(s * items + item) * 2], x = a.part_o[(s * items + item) * D + c];
+        const float f = ms == -CUDART_INF_F ? 0.f : exp2_ftz(ms - m);
+        v += f == 0.f && fabsf(x) == CUDART_INF_F ? x : f * x;
+      }
+    }
     out[c] = from_f32<T>(v * inv);
   }
 }

@@ -35,6 +35,20 @@ __device__ __forceinline__ float exp2_ftz(float x) {
   return y;
 }
 
+// Largest of three, NaN where one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+template <int N>
+__device__ __forceinline__ bool any_nan(const float (&v)[N]) {
+  float top = v[0];
+#pragma unroll
+  for (int i = 1; i < N; i += 2) top = max3(top, v[i], v[i + 1 < N ? i + 1 : i]);
+  return top != top;
+}
+
 // Sequence b as the kernels see it: its first packed row, its new rows (held to the rows there are), its length.
 struct Seq {
   int first, rows, length;
@@ -106,6 +120,75 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t v) {  // bits 15 and 31
   constexpr uint32_t m = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
   constexpr uint32_t one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
   return ((v & m) + one) & 0x80008000u;
+}
+
+// Values that are not finite are listed apart: list [NaN, +inf, -inf][D], the first key with one in each column.
+// What column col of a row that sees keys up to lim gets from them.
+template <int D>
+__device__ __forceinline__ float listed_value(const int* list, int col, int lim) {
+  float add = 0.f;
+  if (list[D + col] <= lim) add += CUDART_INF_F;
+  if (list[2 * D + col] <= lim) add -= CUDART_INF_F;
+  return list[col] <= lim ? CUDART_NAN_F : add;
+}
+// Lists one: the bits of key `key`'s value in column col.
+template <typename T, int D>
+__device__ __forceinline__ void list_value(int* list, uint16_t bits, int key, int col) {
+  const float f = to_f32<T>(*reinterpret_cast<const T*>(&bits));
+  atomicMin(list + (f != f ? 0 : f > 0.f ? 1 : 2) * D + col, key);
+}
+// Where a row's weights are fine and a sum over them is NaN, an infinity may have met a weight or a factor that vanished
+// (0 * inf); what the sum has to be then follows from the values that are not finite alone.  THREADS threads (a warp or
+// the CTA) list those of keys [from, to).
+template <typename T, int D, int THREADS>
+__device__ __noinline__ void list_values(const AttendArgs& a, int b, int kvh, int from, int to, int* list) {
+  auto sync = [] {
+    if constexpr (THREADS == 32)
+      __syncwarp();
+    else
+      __syncthreads();
+  };
+  const int me = threadIdx.x % THREADS;
+  for (int i = me; i < 3 * D; i += THREADS) list[i] = INT_MAX;
+  sync();
+  constexpr int CH = D / 8;
+  const int32_t* table = a.seqs.table + b * a.seqs.table_stride;
+#pragma unroll 4
+  for (int64_t i = (int64_t)from * CH + me; i < (int64_t)to * CH; i += THREADS) {
+    const int key = (int)(i / CH), col = (int)(i % CH) * 8, page = table[key >> a.pages.page_shift];
+    if ((uint32_t)page >= (uint32_t)a.pages.num_pages) continue;
+    const int64_t row = key & ((1 << a.pages.page_shift) - 1);
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.pages.v) + page * a.pages.v_page +
+                                                         kvh * a.pages.v_head + row * a.pages.v_row + col));
+    if (!(not_finite2<T>(v.x) | not_finite2<T>(v.y) | not_finite2<T>(v.z) | not_finite2<T>(v.w))) continue;
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint16_t bits = (uint16_t)(u[e >> 1] >> (16 * (e & 1)));
+      if (not_finite16<T>(bits)) list_value<T, D>(list, bits, key, col + e);
+    }
+  }
+  sync();
+}
+// ... and one thread puts right n columns from col on of row r (of those of kv head kvh, which sees keys up to lim): of the
+// result, or (part >= 0) of a part on its way to the join.
+template <typename T, int D>
+__device__ __noinline__ void mend_row(const AttendArgs& a, const int* list, int64_t first, int r, int kvh, int part, int lim,
+                                      int col, int n) {
+  const int64_t t = first + r / a.group;
+  const int h = kvh * a.group + r % a.group;
+  auto go = [&](auto* row) {
+    using V = std::remove_pointer_t<decltype(row)>;
+#pragma unroll 1
+    for (int c = col; c < col + n; ++c) {
+      const float v = to_f32<V>(row[c]), right = listed_value<D>(list, c, lim);
+      if (v != v && right != 0.f) row[c] = from_f32<V>(right);
+    }
+  };
+  if (part >= 0)
+    go(a.part_o + (((int64_t)part * a.tokens + t) * a.q_heads + h) * D);
+  else
+    go(static_cast<T*>(a.out) + t * a.o_t + h * a.o_h);
 }
 
 int attend_tiles_launch(AttendArgs& a, int head_dim, int page_size, bool half, int tiles, int groups, cudaStream_t st);

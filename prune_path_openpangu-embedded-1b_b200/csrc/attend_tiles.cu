@@ -177,12 +177,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// Largest of three, NaN where one is.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 
 // What every warp of a CTA derives alike for one group of TILES row tiles.
 template <int TILES, int KEYS>
@@ -503,6 +497,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const int h = kvh * a.group + r - tok * a.group;
         const int64_t at = ((int64_t)split * a.tokens + token) * a.q_heads + h;
         T* out = static_cast<T*>(a.out) + token * a.o_t + h * a.o_h;
+        bool nan = false;  // some sum is
         constexpr int W = D / 2;  // columns held at once
 #pragma unroll 1
         for (int i = 0; i < D; i += W) {
@@ -517,13 +512,11 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
             for (int e = 0; e < W; ++e) o[e] = 0.f;
           }
+          nan |= any_nan(o);
           if (listed) {
 #pragma unroll 1
             for (int e = 0; e < W; ++e) {
-              float add = 0.f;
-              if (odd[D + i + e] <= lim) add += CUDART_INF_F;
-              if (odd[2 * D + i + e] <= lim) add -= CUDART_INF_F;
-              if (odd[i + e] <= lim) add = CUDART_NAN_F;
+              const float add = listed_value<D>(odd, i + e, lim);
               if (!(add == 0.f)) {
 #pragma unroll
                 for (int z = 0; z < W; ++z) o[z] = z == e ? o[z] + add : o[z];
@@ -554,6 +547,14 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
         }
         if (a.nsplit > 1 && r < rows) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m * c, l);
+        nan &= r < rows && (l > 0.f || (l == 0.f && a.nsplit > 1));
+        // Sums to put right (attend.cuh), by each warp for itself.  16 prompts of 512 take 37.5 us in a graph with this look at
+        // the sums and 36.6 without; joined with the barrier behind it, and by the whole CTA, 38.
+        if (__any_sync(0xffffffffu, nan)) {
+          int* list = reinterpret_cast<int*>(smem + t * S::kQ + (warp & 3) * (S::kQ / 4));  // this tile's q has been read
+          list_values<T, D, 32>(a, b, kvh, w.b0 * KEYS, min((w.b0 + count) * KEYS, w.keys), list);
+          if (nan) mend_row<T, D>(a, list, sq.first, r, kvh, a.nsplit > 1 ? split : -1, lim, 0, D);
+        }
       }
       next_group(group);
     }
@@ -789,8 +790,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               for (int e = 0; e < 8; ++e) {
                 const uint16_t bits = p[e];
                 if (!not_finite16<T>(bits)) continue;
-                const float f = to_f32<T>(*reinterpret_cast<const T*>(&bits));
-                atomicMin(odd + (f != f ? 0 : f > 0.f ? 1 : 2) * D + col + e, key0 + key);
+                list_value<T, D>(odd, bits, key0 + key, col + e);
                 p[e] = 0;
               }
             }

@@ -202,3 +202,35 @@ def test_a_missing_page(cuda, new, length, hints):
         assert_attention(out[:before], *(x[:before] for x in want))
         assert_attention(out[new:], *(x[new:] for x in want))
     cache.check_device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("new,length,hints", PLANS)
+def test_infinite_values_of_vanishing_weight(cuda, dtype, dim, new, length, hints):
+    """An infinity that a row sees reaches it however small its weight is, and however that came about: its own score
+    2^-200 of the row's largest or -inf, a later key that takes all the weight, a part that weighs nothing beside another."""
+    b = Batch([new, new, 1], [length, new, 9], 2, dim, 32, dtype, cuda, seed=29)
+    q = b.normal(4, 2.0)
+    q[..., 2] = 32.0
+    for s in (0, 1):
+        n = b.lengths[s]
+        p = n - new
+        k, v = b.keys[s], b.values[s]
+        k[..., 2] = 0.0
+        low, early, high, late = n // 3, n // 4, p + new // 2, p + min(10, new - 1)
+        k[low, :, 2], k[high, :, 2] = -64.0, 64.0
+        v[low, 0, 0], v[low, 1, 0] = math.inf, -math.inf
+        v[early, :, 1] = math.inf
+        v[late, 0, 3] = math.inf
+        v[low, 0, 4], v[early, 0, 4] = math.inf, -math.inf
+        v[early, 1, 5], v[late, 1, 5] = -math.inf, -math.inf
+        if n > 40:
+            k[n // 5, :, 2], v[n // 5, 0, 6] = -math.inf, math.inf
+        store(b, s)
+    out, size = exact_attention(b, q)
+    assert out[-2].isinf().any() and out[-1].isfinite().all()
+    got = b.cache().attend(q, b.starts, b.lens, b.table, **hints)
+    assert_attention(got, out, size)
+    assert torch.equal(b.cache().attend(q, b.starts, b.lens, b.table, out=q, **hints).isnan(), out.isnan())  # (q: read again)
+    assert_attention(q, out, size)
