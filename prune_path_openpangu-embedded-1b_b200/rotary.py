@@ -118,7 +118,8 @@ class RotaryEmbedding:
     * ``{"type": "yarn", "factor": s, "original_length": n}`` (and optionally ``beta_fast`` 32,
       ``beta_slow`` 1, ``gain``): pairs that turn more than ``beta_fast`` times within ``n`` positions
       are left alone, those under ``beta_slow`` are divided by ``s``, the ones between are blended by
-      their index; rotated values are multiplied by ``gain`` (default ``0.1 ln s + 1``).
+      their index; rotated values are multiplied by ``gain`` (default ``0.1 ln s + 1``, and 1 for ``s``
+      below 1).
 
     The object holds numbers only (``turns``: turns per position of each pair, fp64 on the host);
     a captured launch keeps its own copy of them.  bf16, fp16 and fp32; values are rounded once.
@@ -168,7 +169,7 @@ class RotaryEmbedding:
             low, high = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rotary_dim - 1)
             keep = [1.0 - min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0) for i in pairs]
             freq = [f * k + f / factor * (1.0 - k) for f, k in zip(freq, keep)]
-            self.gain = float(sc.pop("gain", 0.1 * math.log(factor) + 1.0))
+            self.gain = float(sc.pop("gain", 0.1 * math.log(max(factor, 1.0)) + 1.0))
         if sc:
             raise ValueError(f"unknown scaling entries {sorted(sc)}")
         turns = [f / (2.0 * math.pi) for f in freq]

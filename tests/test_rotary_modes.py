@@ -1,4 +1,6 @@
 """Rotary position embedding under forward-mode differentiation, and as an object of its own."""
+import math
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -67,6 +69,12 @@ def test_mixed_modes_on_cpu(monkeypatch):
         (dq,) = torch.autograd.grad(e(x, None, pos)[0], x, forward_ad.make_dual(w, t))
         dq, tangent = forward_ad.unpack_dual(dq)
         assert torch.equal(dq, back(w)) and torch.equal(tangent, back(t))
+
+
+@pytest.mark.parametrize("factor,gain", [(0.5, 1.0), (1.0, 1.0), (2.0, 0.1 * math.log(2.0) + 1.0)])
+def test_yarn_gain(factor, gain):
+    """The published rule multiplies values only where the context is made longer."""
+    assert emb(64, scaling={"type": "yarn", "factor": factor, "original_length": 4096}).gain == gain
 
 
 # ------------------------------------------------------------------ GPU
