@@ -121,8 +121,8 @@ class RotaryEmbedding:
       their index; rotated values are multiplied by ``gain`` (default ``0.1 ln s + 1``, and 1 for ``s``
       below 1).
 
-    The object holds numbers only (``turns``: turns per position of each pair, fp64 on the host);
-    a captured launch keeps its own copy of them.  bf16, fp16 and fp32; values are rounded once.
+    The object holds numbers only, which do not change (``turns``: turns per position of each pair, fp64 on the
+    host); a captured launch keeps its own copy of them.  bf16, fp16 and fp32; values are rounded once.
     To capture a backward pass into a CUDA graph, let no eager graph of the same leaves live: autograd would
     wait for the stream that one was made on, which a capture does not allow.
     """
@@ -138,8 +138,8 @@ class RotaryEmbedding:
             raise ValueError(f"layout={layout!r} must be 'half' or 'interleaved'")
         if not (base > 0 and math.isfinite(base)):
             raise ValueError(f"base={base} must be positive and finite")
-        self.head_dim, self.rotary_dim, self.layout = head_dim, rotary_dim, layout
-        self.gain = 1.0
+        self._head_dim = head_dim
+        gain = 1.0
         pairs = range(rotary_dim // 2)
         sc = dict(scaling or {})
         kind = sc.pop("type", None)
@@ -169,13 +169,31 @@ class RotaryEmbedding:
             low, high = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rotary_dim - 1)
             keep = [1.0 - min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0) for i in pairs]
             freq = [f * k + f / factor * (1.0 - k) for f, k in zip(freq, keep)]
-            self.gain = float(sc.pop("gain", 0.1 * math.log(max(factor, 1.0)) + 1.0))
+            gain = float(sc.pop("gain", 0.1 * math.log(max(factor, 1.0)) + 1.0))
         if sc:
             raise ValueError(f"unknown scaling entries {sorted(sc)}")
-        turns = [f / (2.0 * math.pi) for f in freq]
-        self.turns = torch.tensor(turns, dtype=torch.float64)
-        self._c = _lib.Rotation(rotary_dim, layout == "interleaved", self.gain)
-        self._c.turns[:rotary_dim // 2] = turns
+        self._c = _lib.Rotation(rotary_dim, layout == "interleaved", gain)  # (what the launches read)
+        self._c.turns[:rotary_dim // 2] = [f / (2.0 * math.pi) for f in freq]
+
+    @property
+    def head_dim(self) -> int:
+        return self._head_dim
+
+    @property
+    def rotary_dim(self) -> int:
+        return self._c.rotary_dim
+
+    @property
+    def layout(self) -> str:
+        return "interleaved" if self._c.interleaved else "half"
+
+    @property
+    def gain(self) -> float:
+        return self._c.gain
+
+    @property
+    def turns(self) -> torch.Tensor:
+        return torch.tensor(self._c.turns[:self._c.rotary_dim // 2], dtype=torch.float64)
 
     @property
     def _ptr(self) -> int:  # (of this object's own structure: copies have theirs)
@@ -203,7 +221,7 @@ class RotaryEmbedding:
         self._launch(q, k, positions, False, (q, k))
 
     def _launch(self, q, k, positions, inverse, out=None):
-        dev, shape, dt, D = q.device, q.shape, q.dtype, self.head_dim
+        dev, shape, dt, D = q.device, q.shape, q.dtype, self._head_dim
         if dev.type != "cuda":
             raise RuntimeError("RotaryEmbedding runs on CUDA only; got a tensor on " + str(dev))
         four = len(shape) == 4

@@ -1,5 +1,7 @@
 """Rotary position embedding under forward-mode differentiation, and as an object of its own."""
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -75,6 +77,20 @@ def test_mixed_modes_on_cpu(monkeypatch):
 def test_yarn_gain(factor, gain):
     """The published rule multiplies values only where the context is made longer."""
     assert emb(64, scaling={"type": "yarn", "factor": factor, "original_length": 4096}).gain == gain
+
+
+def test_an_embedding_does_not_change():
+    """What the launches read is what the attributes say, in copies too; none can be set."""
+    e = emb(64, rotary_dim=32, layout="interleaved", scaling={"type": "yarn", "factor": 4.0, "original_length": 4096})
+    for x in (e, copy.deepcopy(e), pickle.loads(pickle.dumps(e))):
+        assert (x.head_dim, x.rotary_dim, x.layout, x.gain) == (64, 32, "interleaved", 0.1 * math.log(4.0) + 1.0)
+        assert torch.equal(x.turns, e.turns) and x.turns.dtype == torch.float64 and x.turns.shape == (16,)
+        for name, value in (("head_dim", 32), ("rotary_dim", 16), ("layout", "half"), ("gain", 2.0), ("turns", torch.zeros(16))):
+            with pytest.raises(AttributeError):
+                setattr(x, name, value)
+    before = e.turns
+    e.turns.zero_()
+    assert torch.equal(e.turns, before)
 
 
 # ------------------------------------------------------------------ GPU
