@@ -148,7 +148,7 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
         if (real) {
           const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = q_pair(h[2 * e] | (uint32_t)h[2 * e + 1] << 16, a.q_sign);
+          for (int e = 0; e < 4; ++e) v[e] = q_pair<T>(h[2 * e] | (uint32_t)h[2 * e + 1] << 16, a.q_sign);
         }
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(d), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
       }

@@ -95,11 +95,6 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 
-// What q is multiplied by (-1, 0 or 1), on a packed pair.
-__device__ __forceinline__ uint32_t q_pair(uint32_t v, int sign) {
-  return sign > 0 ? v : sign < 0 ? v ^ 0x80008000u : 0u;
-}
-
 // Fp16 weights below 2^-24 would vanish; lifting every weight by 2^7 (it cancels against l) keeps
 // those down to 2^-31 of the largest, and weights of up to 2^8 (attend_tiles.cu) below fp16's
 // largest number.  bf16 has fp32's exponents and needs none.
@@ -120,6 +115,12 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t v) {  // bits 15 and 31
   constexpr uint32_t m = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
   constexpr uint32_t one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
   return ((v & m) + one) & 0x80008000u;
+}
+
+// A packed pair of q times -1, 0 or 1 (0 times what is not finite is NaN).
+template <typename T>
+__device__ __forceinline__ uint32_t q_pair(uint32_t v, int sign) {
+  return sign > 0 ? v : sign < 0 ? v ^ 0x80008000u : (not_finite2<T>(v) >> 15) * 0x7fffu;
 }
 
 // Values that are not finite are listed apart: list [NaN, +inf, -inf][D], the first key with one in each column.

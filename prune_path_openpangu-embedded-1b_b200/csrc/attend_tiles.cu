@@ -297,8 +297,8 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         uint4 v = make_uint4(0, 0, 0, 0);
         if (base + rr < rows) {
           const uint16_t* h = reinterpret_cast<const uint16_t*>(q + at.off);
-          v = make_uint4(q_pair(h[0] | (uint32_t)h[1] << 16, a.q_sign), q_pair(h[2] | (uint32_t)h[3] << 16, a.q_sign),
-                         q_pair(h[4] | (uint32_t)h[5] << 16, a.q_sign), q_pair(h[6] | (uint32_t)h[7] << 16, a.q_sign));
+          v = make_uint4(q_pair<T>(h[0] | (uint32_t)h[1] << 16, a.q_sign), q_pair<T>(h[2] | (uint32_t)h[3] << 16, a.q_sign),
+                         q_pair<T>(h[4] | (uint32_t)h[5] << 16, a.q_sign), q_pair<T>(h[6] | (uint32_t)h[7] << 16, a.q_sign));
         }
         *reinterpret_cast<uint4*>(q_s + sw128_offset(rr, ch & 7)) = v;
       }

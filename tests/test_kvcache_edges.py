@@ -234,3 +234,19 @@ def test_infinite_values_of_vanishing_weight(cuda, dtype, dim, new, length, hint
     assert_attention(got, out, size)
     assert torch.equal(b.cache().attend(q, b.starts, b.lens, b.table, out=q, **hints).isnan(), out.isnan())  # (q: read again)
     assert_attention(q, out, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,length,hints", PLANS)
+def test_a_scale_of_zero(cuda, dtype, new, length, hints):
+    """The mean of the values; queries that are not finite are no less so for it (0 * inf, 0 * NaN)."""
+    b = Batch([new], [length], 1, 64, 32, dtype, cuda, seed=30)
+    q = b.normal(4, 2.0)
+    q[:, 1, 5], q[:, 2, 60] = math.nan, -math.inf
+    q[0, 3, 0] = math.inf
+    got = b.cache().attend(q, b.starts, b.lens, b.table, scale=0.0, **hints)
+    out, size = exact_attention(b, q.nan_to_num(0.0, 0.0, 0.0), 0.0)
+    assert got[:, 1:3].isnan().all() and got[0, 3].isnan().all()
+    assert_attention(got[:, 0], out[:, 0], size[:, 0])
+    assert_attention(got[1:, 3], out[1:, 3], size[1:, 3])
