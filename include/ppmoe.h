@@ -318,7 +318,8 @@ PPMOE_API int ppmoe_kv_append(const ppmoe_kv_cache* cache, const ppmoe_rotation*
  * position is left (p(t) < 0).  max_new and max_length: the longest run of new rows and the longest
  * length of the batch, as far as the host knows; they choose the kernel and its split, and a
  * wrong value costs time, not correctness.  ws: ppmoe_attend_workspace_bytes of the same
- * numbers, 32-byte aligned, contents of no importance before or after the call. */
+ * numbers, 32-byte aligned, contents of no importance before or after the call.  max_pages * page_size: at most
+ * 2^31 - 8193. */
 PPMOE_API size_t ppmoe_attend_workspace_bytes(int tokens, int q_heads, int kv_heads, int head_dim, int batch,
                                               int max_new, int64_t max_length);
 PPMOE_API int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t q_t, int64_t q_h, int q_heads,

@@ -708,6 +708,11 @@ extern "C" int ppmoe_attend(const ppmoe_kv_cache* cache, const void* q, int64_t 
               (long long)batch * kv_heads, (long long)tokens * q_heads);
     return PPMOE_ERR_UNSUPPORTED;
   }
+  // (the kernels count keys in 32 bits, up to some blocks past the last)
+  if ((int64_t)max_pages * cache->page_size > INT32_MAX - 8192) {
+    set_error("ppmoe_attend: a table of %d pages of %d names too many positions (at most 2^31 - 8193)", max_pages, cache->page_size);
+    return PPMOE_ERR_UNSUPPORTED;
+  }
   if (!q || !out) {
     set_error("ppmoe_attend: null pointer");
     return PPMOE_ERR_INVALID_ARG;

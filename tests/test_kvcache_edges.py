@@ -1,5 +1,6 @@
 """Paged cache and attention where they meet the rest of a program: launches behind them on the stream, autograd,
 values and sizes at the borders of what they take."""
+import ctypes
 import math
 
 import pytest
@@ -9,6 +10,16 @@ from torch.autograd import forward_ad
 from conftest import pkg
 from gpu_helpers import make_module
 from paged_helpers import GARBAGE, Batch, assert_attention, exact_attention
+
+
+# ------------------------------------------------------------------ CPU
+def test_a_table_of_too_many_positions():
+    """Counting keys in 32 bits would run over: refused before anything is launched."""
+    lib = pkg()._lib.load()
+    for page, pages in ((256, (1 << 23) - 31), (16, 1 << 27)):
+        cache = pkg()._lib.KVCache(1024, 1024, 2 * page * 64, page * 64, 64, 2 * page * 64, page * 64, 64, 4, page, 2, 64, 0, 256)
+        rc = lib.ppmoe_attend(ctypes.byref(cache), 16, 256, 64, 4, 1, 16, 16, 16, pages, 1, pages, 0.125, 1, 64, 16, 256, 64, None, 0, None)
+        assert rc == -2 and b"positions" in lib.ppmoe_last_error()
 
 
 # ------------------------------------------------------------------ GPU: what follows on the stream
