@@ -53,6 +53,8 @@ class PagedKVCache:
             raise ValueError("the cache has no pages")
         if k.requires_grad or v.requires_grad:
             raise ValueError("the cache writes into its tensors: they cannot require gradients")
+        if k.data_ptr() == v.data_ptr():
+            raise ValueError("keys and values need memory of their own")
         for t in (k, v):
             if t.stride(3) != 1 or any(s % 8 or s == 0 for n, s in zip(t.shape[:3], t.stride()) if n > 1) or t.data_ptr() % 16:
                 raise ValueError("cache tensors need contiguous heads, 16-byte alignment and strides of whole 16 bytes")

@@ -22,6 +22,14 @@ def test_a_table_of_too_many_positions():
         assert rc == -2 and b"positions" in lib.ppmoe_last_error()
 
 
+def test_keys_and_values_of_one_memory():
+    """An append would write both to the same places."""
+    x = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    for v in (x, x.view_as(x)):
+        with pytest.raises(ValueError, match="memory of their own"):
+            pkg().kvcache.PagedKVCache.from_tensors(x, v)
+
+
 # ------------------------------------------------------------------ GPU: what follows on the stream
 @pytest.mark.gpu
 @pytest.mark.parametrize("shared", ["out", "q"])
