@@ -140,6 +140,8 @@ class SyntheticDecoder:
     def prefill(self, ids):
         cfg = self.cfg
         B, T = ids.shape
+        if T > cfg.max_seq:
+            raise ValueError(f"prompt {T} exceeds max_seq {cfg.max_seq}")
         if cfg.kv == "paged":
             self._pages(B)
             x = self.embed[ids]
