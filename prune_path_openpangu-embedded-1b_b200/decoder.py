@@ -193,35 +193,34 @@ class SyntheticDecoder:
         tok = self.prefill(ids)
         e1.record()
         out = [tok]
-        if use_graph and (self.graph is None or self._gB != B):
-            self._pos = torch.zeros(1, dtype=torch.long, device=self.dev)  # graph inputs: fixed tensors
-            self._tok = torch.zeros(B, dtype=torch.long, device=self.dev)
-        elif not use_graph:
-            self._pos = torch.zeros(1, dtype=torch.long, device=self.dev)
-            self._tok = torch.zeros(B, dtype=torch.long, device=self.dev)
-        self._pos.fill_(T)
-        self._tok.copy_(tok)
+        if use_graph and self.graph is not None and self._gB == B:
+            pos, last = self._inputs  # the tensors that the captured step reads
+        else:
+            pos = torch.zeros(1, dtype=torch.long, device=self.dev)
+            last = torch.zeros(B, dtype=torch.long, device=self.dev)
+        pos.fill_(T)
+        last.copy_(tok)
         if use_graph:
             if self.graph is None or self._gB != B:
                 s = torch.cuda.Stream(self.dev)
                 s.wait_stream(torch.cuda.current_stream(self.dev))
                 with torch.cuda.stream(s):
-                    self._next = self._step(self._tok, self._pos)  # warm-up outside capture
+                    self._next = self._step(last, pos)  # warm-up outside capture
                 torch.cuda.current_stream(self.dev).wait_stream(s)
                 self.graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(self.graph):
-                    self._next = self._step(self._tok, self._pos)
-                self._gB = B
+                    self._next = self._step(last, pos)
+                self._gB, self._inputs = B, (pos, last)
                 # the warm-up wrote position T into the caches: harmless, rewritten below
         for _ in range(new_tokens - 1):
             if use_graph:
                 self.graph.replay()
                 nxt = self._next
             else:
-                nxt = self._step(self._tok, self._pos)
+                nxt = self._step(last, pos)
             out.append(nxt.clone())
-            self._tok.copy_(nxt)
-            self._pos += 1
+            last.copy_(nxt)
+            pos += 1
         e2.record()
         torch.cuda.synchronize()
         return torch.stack(out, 1), e0.elapsed_time(e1), e1.elapsed_time(e2)
