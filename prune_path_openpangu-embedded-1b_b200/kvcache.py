@@ -222,8 +222,9 @@ class PagedKVCache:
         return s
 
     def check_device_status(self) -> None:
-        """Synchronise and raise if a call met a position without a page (its row was not stored, or what
-        it gave is not defined); clears the status."""
+        """Wait for the device, all its streams, and raise if a call met a position without a page (its row was
+        not stored, or what it gave is not defined); clears the status."""
+        torch.cuda.synchronize(self.device)
         back = _enter(self.device)
         try:
             _lib.call("ppmoe_workspace_status", self._status.data_ptr(), _stream(self.device))

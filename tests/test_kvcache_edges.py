@@ -256,6 +256,24 @@ def test_infinite_values_of_vanishing_weight(cuda, dtype, dim, new, length, hint
 
 
 @pytest.mark.gpu
+def test_a_missing_page_on_another_stream(cuda):
+    """The status is that of every call before it, on whichever stream."""
+    b = Batch([2], [20], 1, 64, 16, torch.bfloat16, cuda, seed=31)
+    cache, k, v = b.cache(), b.normal(1), b.normal(1)
+    cache.append(None, k, v, b.starts, b.lens, b.table)
+    cache.check_device_status()
+    nowhere = torch.full_like(b.table, -1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)  # some 25 ms
+        cache.append(None, k, v, b.starts, b.lens, nowhere)
+    with pytest.raises(pkg()._lib.PPMoEError, match="without a page"):
+        cache.check_device_status()
+    cache.check_device_status()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("new,length,hints", PLANS)
 def test_a_scale_of_zero(cuda, dtype, new, length, hints):
