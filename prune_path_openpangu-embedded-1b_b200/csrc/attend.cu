@@ -412,7 +412,7 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
           }
           if (any_nan(acc) && (sum > 0.f || (sum == 0.f && joined))) mend |= 1u << ((c - col) / 8);
           if (!clustered && !joined) {
-            store_row<T, 8>(static_cast<T*>(a.out) + t * a.o_t + h * a.o_h + c, acc, inv, a.o_wide);
+            store_row<T>(static_cast<T*>(a.out) + t * a.o_t + h * a.o_h + c, acc, inv, a.o_wide);
           } else if (clustered) {  // (over what this thread alone has read)
             *reinterpret_cast<float4*>(j_o + row * (D + 4) + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
             *reinterpret_cast<float4*>(j_o + row * (D + 4) + c + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
@@ -463,7 +463,7 @@ attend_thin_kernel(const __grid_constant__ AttendArgs a) {
         }
         if (any_nan(acc) && sum > 0.f) mend |= at;
         const int tok = r / a.group;
-        store_row<T, 8>(static_cast<T*>(a.out) + (sq.first + tok) * a.o_t + (int64_t)(kvh * a.group + r - tok * a.group) * a.o_h + c,
+        store_row<T>(static_cast<T*>(a.out) + (sq.first + tok) * a.o_t + (int64_t)(kvh * a.group + r - tok * a.group) * a.o_h + c,
                         acc, inverse_sum(sum, pos0 + tok), a.o_wide);
       }
       cluster_sync();  // every part has been read
@@ -581,8 +581,8 @@ static Plan make_plan(int tokens, int q_heads, int kv_heads, int head_dim, int b
   // 4000 keys, in us, here and there: 20 rows of 64 values 23 and 39; of 128 (8 kv heads) 65 (two row
   // tiles at once, 16 keys at a time) and 57.
   if (rows <= (head_dim == 64 ? 32 : 16)) {
-    // Up to two CTAs an SM a part may be as short as 128 keys (one block of each warp): there latency
-    // counts; beyond, parts of 768 keys or more, up to 1184 CTAs, so that ragged lengths even out.
+    // Parts of 128 keys (two blocks of each warp) as far as they make two CTAs an SM, since there latency
+    // counts; parts of 768 as far as they make 1184 CTAs, so that ragged lengths even out; whichever are more.
     p.tiles = 0;
     p.groups = rows <= 16 ? 1 : 2;
     const int64_t n1 = std::min(up(max_length, 128), up(296, base));

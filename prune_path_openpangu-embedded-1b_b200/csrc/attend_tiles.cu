@@ -16,12 +16,13 @@
 // zero (pages end inside a tile), values that are not finite are taken out and listed.
 //
 // Long contexts are bound by the chain score -> softmax -> product of each tile, which the other tile's overlaps:
-// 3000 cycles a block of 128 keys, of which the tensor pipe is busy for 2048 (62% measured, the special
-// function pipe 62%); over seconds the power limit takes another tenth.  2048 rows over 34816 keys, 32 query
+// 3000 cycles a block of 128 keys, of which the tensor pipe is busy for 2048 (68%; over a launch, with its start and the
+// tail of its last wave, 62% measured, the special function pipe the same); over seconds the power limit takes
+// another tenth.  2048 rows over 34816 keys, 32 query
 // and 8 kv heads of 128, bf16: 945 us cold, 1000-1025 us sustained (1.2 and 1.1 PFLOP/s).  Tried and slower: a
 // products' warp for each tile (1283 us: the tiles' products interleave and both softmaxes wait at once),
 // persistent CTAs with the next item's loads ahead (1033; prompts of 512 44-48 us for 41), part of the
-// exponentials as polynomials.  Short prompts are bound by a CTA's start and end (7 + 3 thousand cycles).
+// exponentials as polynomials.  Short prompts are bound by a CTA's start and end (7 + 2 thousand cycles).
 #include <cuda.h>
 #include <mutex>
 #include "attend.cuh"
@@ -580,7 +581,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const uint64_t qd = q_desc + (uint64_t)(t * (S::kQ >> 4)), kd = k_desc + (uint64_t)(st * (S::kStage >> 4));
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-              umma_bf16(tmem + i * KEYS, qd + (((k >> 2) * (kTileRows * 128) + (k & 3) * 32) >> 4),
+              umma_f16(tmem + i * KEYS, qd + (((k >> 2) * (kTileRows * 128) + (k & 3) * 32) >> 4),
                         kd + (((k >> 2) * (KEYS * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
             umma_commit(s_full + i);
           };

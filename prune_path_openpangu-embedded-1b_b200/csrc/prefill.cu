@@ -129,7 +129,7 @@ router_gemm_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_consta
       const uint32_t sa = smem_u32(smem + s * stage_bytes);
       const uint64_t ad = umma_desc_sw128(sa), bd = umma_desc_sw128(sa + a_bytes);
 #pragma unroll
-      for (int k = 0; k < kBK / 16; ++k) umma_bf16(tmem, ad + 2 * k, bd + 2 * k, idesc, (j | k) != 0);
+      for (int k = 0; k < kBK / 16; ++k) umma_f16(tmem, ad + 2 * k, bd + 2 * k, idesc, (j | k) != 0);
       umma_commit(&empty[s]);
     }
     umma_commit(tfull);
@@ -517,8 +517,8 @@ gu_gemm_pair_kernel(const __grid_constant__ CUtensorMap mapGU, const GUPairArgs 
                        bd = umma_desc_sw128(sa + 2 * a_bytes);
 #pragma unroll
         for (int k = 0; k < kBK / 16; ++k) {
-          umma_bf16(tmem, ad0 + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
-          if (two) umma_bf16(tmem + 256, ad1 + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
+          umma_f16(tmem, ad0 + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
+          if (two) umma_f16(tmem + 256, ad1 + 2 * k, bd + 2 * k, idesc, (kb | k) != 0);
         }
         umma_commit(&empty[s]);
       }
@@ -656,7 +656,7 @@ down_gemm_kernel(const __grid_constant__ CUtensorMap mapA2, const __grid_constan
           const int kb = k16 >> 2, kk = k16 & 3;
           const uint64_t ad = umma_desc_sw128(smem_u32(sA + ab * a_bytes + kb * a_kb)) + 2 * kk;
           const uint64_t bd = umma_desc_sw128(smem_u32(sB + s * b_bytes + kb * b_kb)) + 2 * kk;
-          umma_bf16(tmem + acc * 256, ad, bd, idesc, k16 != 0);
+          umma_f16(tmem + acc * 256, ad, bd, idesc, k16 != 0);
         }
         umma_commit(&bempty[s]);
         umma_commit(&tfull[acc]);

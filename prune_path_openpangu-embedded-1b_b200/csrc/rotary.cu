@@ -18,7 +18,7 @@ namespace ppmoe {
 
 constexpr int kMaxPairs = 128;  // head_dim <= 256
 constexpr int kRotThreads = 128;
-constexpr int kRotTokens = 4;   // most tokens of one CTA
+constexpr int kRotTokens = 2;   // most tokens of one CTA
 
 // One tensor of heads: rows of head_dim contiguous values; strides in elements.
 struct HeadsView {
@@ -34,8 +34,7 @@ struct RotaryArgs {
   const void* positions;  // rotary only
   int64_t pos_b, pos_t;
   int pos64;
-  int batch;
-  int64_t length, tokens;  // tokens = batch * length
+  int64_t length, tokens;  // rows of one sequence of the batch, of all
   int head_dim, pairs;     // rotated values: 2 * pairs of head_dim
   float gain, sign;
   int per_cta;
@@ -211,7 +210,7 @@ static int launch_v(RotaryArgs& a, bool interleaved, cudaStream_t st) {
 
 template <bool APPEND>
 static int launch(RotaryArgs& a, bool interleaved, int dtype, bool wide, cudaStream_t st) {
-  a.per_cta = a.tokens <= 1024 ? 1 : 2;  // (few tokens: as many SMs as there are)
+  a.per_cta = a.tokens <= 1024 ? 1 : kRotTokens;  // (few tokens: as many SMs as there are)
   if (dtype == PPMOE_BF16)
     return wide ? launch_v<__nv_bfloat16, 8, APPEND>(a, interleaved, st)
                 : launch_v<__nv_bfloat16, 1, APPEND>(a, interleaved, st);
@@ -329,7 +328,6 @@ extern "C" int ppmoe_rotary(const ppmoe_rotation* rotation, int inverse, const v
   a.pos64 = positions64;
   a.pos_b = pos_b;
   a.pos_t = pos_t;
-  a.batch = batch;
   a.length = length;
   a.sign = inverse ? -1.f : 1.f;
   const bool wide = head_dim % (2 * v) == 0 && rotation->rotary_dim % (2 * v) == 0 &&
@@ -362,7 +360,6 @@ extern "C" int ppmoe_kv_append(const ppmoe_kv_cache* cache, const ppmoe_rotation
   a.q = {q, q_out, 0, q_t, q_h, 0, qo_t, qo_h, q_heads};
   a.k = {k, nullptr, 0, k_t, k_h, 0, 0, 0, kv_heads};
   a.v = {v, nullptr, 0, v_t, v_h, 0, 0, 0, kv_heads};
-  a.batch = 1;
   a.length = a.tokens = tokens;
   a.sign = 1.f;
   a.status = static_cast<uint32_t*>(cache->status);
