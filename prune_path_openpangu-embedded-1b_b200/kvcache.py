@@ -15,6 +15,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .rotary import _NONE, RotaryEmbedding, _enter, _has_tangent, _stream, _written
@@ -108,7 +109,7 @@ class PagedKVCache:
         """x and its strides, checked."""
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient, and the cache records none: call it under torch.no_grad()")
-        if _has_tangent(x):
+        if forward_ad._current_level >= 0 and _has_tangent(x):
             raise RuntimeError(f"{name} has a forward-mode tangent, and the cache records none: pass its primal")
         shape = x.shape
         if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
@@ -150,10 +151,11 @@ class PagedKVCache:
         T = k.shape[0]
         if v.shape[0] != T or (q is not None and q.shape[0] != T):
             raise ValueError("q, k and v must have the same number of rows")
-        if rotary is not None and rotary.head_dim != self.head_dim:
+        if rotary is not None and rotary._head_dim != self.head_dim:
             raise ValueError(f"rotary has head_dim={rotary.head_dim}, the cache {self.head_dim}")
         batch = self._batch(starts, lengths, table)
         Hq, qp, op, sq, so = 0, None, None, _NONE, _NONE
+        written = self._k, self._v
         if q is not None:
             q, sq = self._rows("q", q)
             Hq = q.shape[1]
@@ -162,10 +164,11 @@ class PagedKVCache:
                 so = (Hq * self.head_dim, self.head_dim)
             else:
                 so = self._out(out, q)
+                written += (out,)
             qp, op = q.data_ptr(), out.data_ptr()
         elif out is not None:
             raise ValueError("out without q")
-        _written(self._k, self._v)
+        _written(*written)
         back = _enter(self.device)
         rc = _lib.load().ppmoe_kv_append(
             self._ptr, None if rotary is None else rotary._ptr, qp, sq[0], sq[1], op, so[0], so[1], Hq, k.data_ptr(),
@@ -199,6 +202,7 @@ class PagedKVCache:
             so = (Hq * D, D)
         else:
             so = self._out(out, q)
+            _written(out)
         scale = D ** -0.5 if scale is None else float(scale)
         lib = _lib.load()
         n = lib.ppmoe_attend_workspace_bytes(T, Hq, self.kv_heads, D, batch[4], new, length)
@@ -218,7 +222,6 @@ class PagedKVCache:
             raise ValueError(f"out must be {list(q.shape)} {q.dtype} on {q.device} with contiguous heads")
         if any(n > 1 and x == 0 for n, x in zip(out.shape, s)):
             raise ValueError("out repeats elements")
-        _written(out)
         return s
 
     def check_device_status(self) -> None:

@@ -31,18 +31,19 @@ _NONE = (0, 0, 0)
 
 def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether forward-mode differentiation follows one of these (such a tensor requires no gradient)."""
-    return (forward_ad._current_level >= 0
+    return (forward_ad._current_level >= 0  # (asked first where a call's host time counts)
             and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors))
 
 
 def _written(*tensors: torch.Tensor) -> None:
     """Tells autograd that a kernel writes into these, so that a backward pass that saved one complains."""
-    for x in tensors:
-        if x.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("a tensor that requires a gradient cannot be written to: use torch.no_grad()")
-    if _has_tangent(*tensors):
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x.requires_grad:
+                raise RuntimeError("a tensor that requires a gradient cannot be written to: use torch.no_grad()")
+    if forward_ad._current_level >= 0 and _has_tangent(*tensors):
         raise RuntimeError("a tensor with a forward-mode tangent cannot be written to")
-    torch.autograd.graph.increment_version(tensors)  # (leaves inference tensors out)
+    torch._C._increment_version(tensors)  # (leaves inference tensors out; what autograd.graph's function calls)
 
 
 def _heads(x: torch.Tensor, four: bool):
