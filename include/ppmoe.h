@@ -315,7 +315,7 @@ PPMOE_API int ppmoe_kv_append(const ppmoe_kv_cache* cache, const ppmoe_rotation*
 
 /* Attention: out[t][h] = sum over positions j <= p(t) of softmax_j(scale q[t][h] . k_j) v_j over
  * the cache of t's sequence, with query head h reading kv head h / (q_heads / kv_heads); 0 where no
- * position is left (p(t) < 0).  max_new and max_length: the longest run of new rows and the longest
+ * position is left (p(t) < 0), NaN where every score is -inf.  max_new and max_length: the longest run of new rows and the longest
  * length of the batch, as far as the host knows; they choose the kernel and its split, and a
  * wrong value costs time, not correctness.  ws: ppmoe_attend_workspace_bytes of the same
  * numbers, 32-byte aligned, contents of no importance before or after the call.  max_pages * page_size: at most

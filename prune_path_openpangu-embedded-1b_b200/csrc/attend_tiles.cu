@@ -16,13 +16,13 @@
 // zero (pages end inside a tile), values that are not finite are taken out and listed.
 //
 // Long contexts are bound by the chain score -> softmax -> product of each tile, which the other tile's overlaps:
-// 3000 cycles a block of 128 keys, of which the tensor pipe is busy for 2048 (68%; over a launch, with its start and the
-// tail of its last wave, 62% measured, the special function pipe the same); over seconds the power limit takes
-// another tenth.  2048 rows over 34816 keys, 32 query
-// and 8 kv heads of 128, bf16: 945 us cold, 1000-1025 us sustained (1.2 and 1.1 PFLOP/s).  Tried and slower: a
-// products' warp for each tile (1283 us: the tiles' products interleave and both softmaxes wait at once),
-// persistent CTAs with the next item's loads ahead (1033; prompts of 512 44-48 us for 41), part of the
-// exponentials as polynomials.  Short prompts are bound by a CTA's start and end (7 + 2 thousand cycles).
+// 3000 cycles a block of 128 keys, of which the tensor pipe is busy for 2048 (68%; over a launch, with its start and
+// the tail of its last wave, 62% measured, the special function pipe the same); over seconds the power limit takes
+// another tenth.  2048 rows over 34816 keys, 32 query and 8 kv heads of 128, bf16: 930-945 us cold, 1000-1087 us
+// sustained (1.2 and 1.1 PFLOP/s).  Tried and slower: a products' warp for each tile (1283 us: the tiles' products
+// interleave and both softmaxes wait at once), part of the exponentials as polynomials, and, with the one-tile CTAs of
+// then (one S tile), persistent CTAs with the next item's loads ahead (1033; prompts of 512 44-48 us for 41).
+// Short prompts are bound by a CTA's start and end (7 + 2 thousand cycles).
 #include <cuda.h>
 #include <mutex>
 #include "attend.cuh"
@@ -552,6 +552,7 @@ attend_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         // Sums to put right (attend.cuh), by each warp for itself.  16 prompts of 512 take 37.5 us in a graph with this look at
         // the sums and 36.6 without; joined with the barrier behind it, and by the whole CTA, 38.
         if (__any_sync(0xffffffffu, nan)) {
+          static_assert(S::kQ / 4 >= 3 * D * 4, "room for a list");
           int* list = reinterpret_cast<int*>(smem + t * S::kQ + (warp & 3) * (S::kQ / 4));  // this tile's q has been read
           list_values<T, D, 32>(a, b, kvh, w.b0 * KEYS, min((w.b0 + count) * KEYS, w.keys), list);
           if (nan) mend_row<T, D>(a, list, sq.first, r, kvh, a.nsplit > 1 ? split : -1, lim, 0, D);

@@ -3,8 +3,8 @@
 //
 // Pair i of a head at position p turns by 2 pi p turns[i]:
 //   y1 = g (x1 cos - x2 sin),  y2 = g (x2 cos + x1 sin)     (gradient: the same with -angle)
-// The angle is reduced in fp64 (p turns[i] minus the nearest integer), so far positions lose
-// nothing, and its sine and cosine are taken in fp32; values are rounded once, at the store.
+// The angle is reduced in fp64 (p turns[i] minus the nearest integer: up to |p| = 2^31 within 2^-21 radians) and its
+// sine and cosine are taken in fp32; values are rounded once, at the store.
 //
 // Bound by memory: every value is read and written once.  Taking the angle from the position costs one
 // fp64 product and one sincospi per pair and token, shared by all heads, and no table that would have

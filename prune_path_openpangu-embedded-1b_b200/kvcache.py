@@ -185,9 +185,10 @@ class PagedKVCache:
         """Attention of the rows ``q [tokens, q_heads, head_dim]`` over their sequences' positions up to
         their own (``q_heads`` a multiple of ``kv_heads``; query head ``h`` reads kv head
         ``h // (q_heads / kv_heads)``).  A row at a negative position gives zeros; rows outside every
-        sequence are not written.  ``max_new`` / ``max_length``: the most new rows and the greatest length of
-        a sequence as far as the host knows (default: the largest possible); they choose how the work is
-        laid out, never what is computed.  ``scale`` defaults to ``head_dim ** -0.5``.  ``out`` may be ``q``.
+        sequence are not written.  A row whose every score is -inf is NaN.  ``max_new`` / ``max_length``: the
+        most new rows and the greatest length of a sequence as far as the host knows (default: the largest
+        possible, all rows in one sequence: a decode step wants ``max_new=1``); they choose how the work is laid
+        out, never what is computed.  ``scale`` defaults to ``head_dim ** -0.5``.  ``out`` may be ``q``.
         Records no derivatives, and refuses rows that ask for one."""
         q, sq = self._rows("q", q)
         T, Hq, D = q.shape

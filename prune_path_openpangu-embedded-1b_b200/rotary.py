@@ -3,7 +3,8 @@
 A head's first ``rotary_dim`` values are pairs; pair ``i`` at position ``p`` is turned by the angle
 ``p * f_i``, ``f_i = base ** (-2 i / rotary_dim)``, optionally scaled for contexts longer than the
 trained ones.  The kernel takes the angle from the position itself (reduced in fp64, sine and
-cosine in fp32), so there is no table of a largest position and far positions lose nothing.
+cosine in fp32), so there is no table of a largest position, and up to 2^31 positions out an angle is
+off by less than 2^-19 radians (the fp64 roundings of ``f_i`` and of ``p * f_i``; they grow with ``p``).
 """
 from __future__ import annotations
 
